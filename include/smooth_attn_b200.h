@@ -57,7 +57,8 @@ SA_API const char* sa_last_cuda_error(void);
  * completed) since the last reset, else SA_OK.  Synchronises the device.
  * Otherwise SA_ERR_BOUNDS if (debug library only) a device-side index check
  * failed, otherwise SA_ERR_ARG if sa_paged_decode met a block_table entry
- * outside [0, num_blocks) since the last reset.
+ * outside [0, num_blocks), or sa_qk_norm_rope a position outside its tables,
+ * since the last reset.
  * reset != 0 clears the recorded status.  (No reference counterpart: the
  * reference's Triton kernels have no bounded waits.)
  */
@@ -316,6 +317,55 @@ SA_API int sa_out_proj(const void* a, const void* w, void* out, int64_t M, int64
 SA_API int sa_rope_rotate(const void* x, void* out, const void* cos_table, const void* sin_table, int cs_dtype,
                           int64_t B, int64_t H, int64_t T, int64_t D, const int64_t* x_strides, int dtype,
                           void* stream);
+
+/*
+ * Root-mean-square norm of every query and key head row, then the rotation of
+ * its position, in one pass over both:
+ *   n = x * rsqrt(mean(x^2) + eps) * weight       (normalize != 0, else n = x)
+ *   y[i] = n[i] c - n[i + R/2] s,  y[i + R/2] = n[i + R/2] c + n[i] s   (i < R/2)
+ *   y[j] = n[j]                                                 (R <= j < D)
+ * all in fp32, rounded once.  q, q_out: [B, Hq, T, D]; k, k_out: [B, Hkv, T,
+ * D]; strides {batch, head, seq, dim} in elements, dim stride 1, the others
+ * multiples of 16 bytes, bases 16-byte aligned.  dtype SA_F32, SA_F16 or
+ * SA_BF16; D a multiple of 16 up to 256; R = rotary_dim a multiple of 16 up to
+ * D (0: no rotation).  q_weight / k_weight: [D] of w_dtype, NULL for 1.
+ * cos_table / sin_table: contiguous [num_pos, R/2] of cs_dtype.  positions:
+ * the table row of token (b, t) at b * pos_batch_stride + t, entries of
+ * pos_bytes (4 or 8) bytes; pos_bytes = 0: row t.  A position outside
+ * [0, num_pos) is read as 0 and reported by sa_device_status (SA_ERR_ARG).
+ * Hq or Hkv may be 0.  (No reference counterpart: the reference rotates inside
+ * its attention kernel, src/smooth_attn/kernels.py:2147-2159, and has no head
+ * norm.)
+ */
+SA_API int sa_qk_norm_rope(const void* q, const void* k, void* q_out, void* k_out, const void* q_weight,
+                           const void* k_weight, int w_dtype, const void* cos_table, const void* sin_table,
+                           int cs_dtype, const void* positions, int pos_bytes, int64_t pos_batch_stride,
+                           int64_t num_pos, int64_t B, int64_t Hq, int64_t Hkv, int64_t T, int64_t D,
+                           int64_t rotary_dim, const int64_t* q_strides, const int64_t* k_strides,
+                           const int64_t* qo_strides, const int64_t* ko_strides, float eps, int normalize, int dtype,
+                           void* stream);
+
+/* Workspace bytes of sa_qk_norm_rope_bwd for the current device (needed only
+ * where a weight's gradient is asked for), or < 0. */
+SA_API int64_t sa_qk_norm_rope_bwd_workspace_size(int64_t D);
+
+/*
+ * Backward of sa_qk_norm_rope: dq, dk from dq_out, dk_out and the forward's own
+ * inputs (nothing else is saved), and the weights' gradients
+ *   dweight = sum over rows of (rotation^T dy) * x * rsqrt(mean(x^2) + eps)
+ * of w_dtype where dq_weight / dk_weight are given.  These are summed in fp32
+ * in a fixed order through `workspace` (sa_qk_norm_rope_bwd_workspace_size
+ * bytes, 16-byte aligned, contents undefined on entry), so they are bitwise
+ * the same from run to run.  Strides as sa_qk_norm_rope.
+ */
+SA_API int sa_qk_norm_rope_bwd(const void* q, const void* k, const void* dq_out, const void* dk_out, void* dq, void* dk,
+                               const void* q_weight, const void* k_weight, int w_dtype, void* dq_weight,
+                               void* dk_weight, const void* cos_table, const void* sin_table, int cs_dtype,
+                               const void* positions, int pos_bytes, int64_t pos_batch_stride, int64_t num_pos,
+                               void* workspace, int64_t workspace_bytes, int64_t B, int64_t Hq, int64_t Hkv, int64_t T,
+                               int64_t D, int64_t rotary_dim, const int64_t* q_strides, const int64_t* k_strides,
+                               const int64_t* dqo_strides, const int64_t* dko_strides, const int64_t* dq_strides,
+                               const int64_t* dk_strides, float eps, int normalize, int dtype, void* stream);
 
 /* Workspace bytes of sa_rope_flash_fwd (the rotated Q and K), or < 0. */
 SA_API int64_t sa_rope_flash_fwd_workspace_size(int64_t B, int64_t Hq, int64_t Hkv, int64_t T, int64_t D);

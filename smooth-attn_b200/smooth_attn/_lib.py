@@ -67,6 +67,12 @@ SIGNATURES = {
                                   _f, _i64, _int, _int, _int, _p]),
     "sa_out_proj": (_int, [_p, _p, _p, _i64, _i64, _i64, _i64, _i64, _i64, _int, _p]),
     "sa_rope_rotate": (_int, [_p, _p, _p, _p, _int, _i64, _i64, _i64, _i64, _i64p, _int, _p]),
+    "sa_qk_norm_rope": (_int, [_p, _p, _p, _p, _p, _p, _int, _p, _p, _int, _p, _int, _i64, _i64,
+                               _i64, _i64, _i64, _i64, _i64, _i64, _i64p, _i64p, _i64p, _i64p, _f, _int, _int, _p]),
+    "sa_qk_norm_rope_bwd_workspace_size": (_i64, [_i64]),
+    "sa_qk_norm_rope_bwd": (_int, [_p, _p, _p, _p, _p, _p, _p, _p, _int, _p, _p, _p, _p, _int, _p, _int, _i64, _i64,
+                                   _p, _i64, _i64, _i64, _i64, _i64, _i64, _i64,
+                                   _i64p, _i64p, _i64p, _i64p, _i64p, _i64p, _f, _int, _int, _p]),
     "sa_rope_flash_fwd_workspace_size": (_i64, [_i64, _i64, _i64, _i64, _i64]),
     "sa_rope_flash_fwd": (_int, [_p, _p, _p, _p, _p, _p, _p, _int, _p, _i64,
                                  _i64, _i64, _i64, _i64, _i64, _i64p, _i64p, _i64p, _i64p,

@@ -25,6 +25,9 @@ the backward ops take an empty ``o_lo`` for "none".
 * ``rope_flash_fwd(q, k, v, cos, sin, scale, window_size) -> o``
 * ``out_proj(a, w) -> a @ w`` (the RoPE projection GEMM)
 * ``fp8_flash_fwd(q, k, v, scale, window_size) -> o``
+* ``qk_norm_rope(q, k, q_weight, k_weight, cos, sin, positions, eps) -> (q, k)``
+* ``qk_norm_rope_bwd(q, k, dq_out, dk_out, q_weight, k_weight, cos, sin, positions, eps, need_dw)
+  -> (dq, dk, dq_weight, dk_weight)`` (an empty gradient for a weight that is None or not needed)
 * ``paged_decode(q, k_cache, v_cache, block_table, context_lens, scale, block_size) -> out``
 """
 
@@ -34,6 +37,7 @@ import torch
 from torch import Tensor
 
 from . import kernels as K
+from . import qk_rope as R
 
 NS = "smooth_attn_b200"
 
@@ -183,3 +187,32 @@ def paged_decode(q: Tensor, k_cache: Tensor, v_cache: Tensor, block_table: Tenso
 def _(q, k_cache, v_cache, block_table, context_lens, scale, block_size):
     B, H, _, D = q.shape
     return torch.empty(B, H, D, device=q.device, dtype=torch.bfloat16)
+
+
+# ------------------------------------------------------------------ head norm and rotation
+
+
+@torch.library.custom_op(f"{NS}::qk_norm_rope", mutates_args=(), device_types="cuda")
+def qk_norm_rope(q: Tensor, k: Tensor, q_weight: Tensor | None, k_weight: Tensor | None, cos: Tensor | None,
+                 sin: Tensor | None, positions: Tensor | None, eps: float | None) -> tuple[Tensor, Tensor]:
+    return R._fwd_direct(q, k, q_weight, k_weight, cos, sin, positions, eps)
+
+
+@qk_norm_rope.register_fake
+def _(q, k, q_weight, k_weight, cos, sin, positions, eps):
+    return tuple(torch.empty(t.shape, device=q.device, dtype=q.dtype) for t in (q, k))
+
+
+@torch.library.custom_op(f"{NS}::qk_norm_rope_bwd", mutates_args=(), device_types="cuda")
+def qk_norm_rope_bwd(q: Tensor, k: Tensor, dq_out: Tensor, dk_out: Tensor, q_weight: Tensor | None,
+                     k_weight: Tensor | None, cos: Tensor | None, sin: Tensor | None, positions: Tensor | None,
+                     eps: float | None, need_dw: bool) -> tuple[Tensor, Tensor, Tensor, Tensor]:
+    dq, dk, dwq, dwk = R._bwd_direct(q, k, dq_out, dk_out, q_weight, k_weight, cos, sin, positions, eps, need_dw)
+    return (dq, dk, dwq if dwq is not None else q.new_empty(0), dwk if dwk is not None else q.new_empty(0))
+
+
+@qk_norm_rope_bwd.register_fake
+def _(q, k, dq_out, dk_out, q_weight, k_weight, cos, sin, positions, eps, need_dw):
+    dw = tuple(torch.empty(w.shape, device=q.device, dtype=w.dtype) if need_dw and w is not None else q.new_empty(0)
+               for w in (q_weight, k_weight))
+    return tuple(torch.empty(t.shape, device=q.device, dtype=q.dtype) for t in (q, k)) + dw
