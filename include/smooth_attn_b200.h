@@ -57,8 +57,9 @@ SA_API const char* sa_last_cuda_error(void);
  * completed) since the last reset, else SA_OK.  Synchronises the device.
  * Otherwise SA_ERR_BOUNDS if (debug library only) a device-side index check
  * failed, otherwise SA_ERR_ARG if sa_paged_decode met a block_table entry
- * outside [0, num_blocks), or sa_qk_norm_rope a position outside its tables,
- * since the last reset.
+ * outside [0, num_blocks) since the last reset, or another call the bad
+ * index that its declaration below says is reported (a position outside the
+ * tables, a slot past the cache, too many pages given back).
  * reset != 0 clears the recorded status.  (No reference counterpart: the
  * reference's Triton kernels have no bounded waits.)
  */
@@ -452,6 +453,117 @@ SA_API int sa_paged_decode(const void* q, const void* k_cache, const void* v_cac
                            int64_t workspace_bytes, int64_t B, int64_t Hq, int64_t Hkv, int64_t num_blocks,
                            int64_t block_size, int64_t max_blocks, int64_t D, float scale, int dtype,
                            void* stream);
+
+/*
+ * Places the next tokens of B requests in a paged cache.  Request b holds
+ * context_lens[b] tokens, in pages block_table[b, 0 .. held) with held =
+ * ceil(context_lens[b] / block_size), and brings new_lens[b] more; they are
+ * the first sum(new_lens) of num_tokens flat tokens, in request order.  With
+ * need[b] = ceil((ctx + new) / block_size) - held, its new pages are
+ * free_pages[free_head[0] + sum of need before b ..], as far as the list of
+ * num_free pages reaches, and go to block_table[b, held ..] (row stride
+ * table_stride).  Outputs: slots[num_tokens] = page * block_size + offset,
+ * positions[num_tokens] = the token's position in its sequence; -1 and 0 for a
+ * token without a place (row or list full, behind the last request);
+ * cu_seqlens[B + 1], clamped to num_tokens; context_lens_out[B] counts the
+ * placed tokens; free_head_out[1].  The inputs other than block_table are not
+ * changed and no output may alias one.  Negative lengths count as 0.  B <= 16384.
+ * One launch.  (No reference counterpart: the reference is handed a table.)
+ */
+SA_API int sa_paged_assign_slots(int32_t* block_table, int64_t table_stride, const int32_t* context_lens,
+                                 const int32_t* new_lens, const int32_t* free_pages, int64_t num_free,
+                                 const int32_t* free_head, int64_t* slots, int32_t* positions, int32_t* cu_seqlens,
+                                 int32_t* context_lens_out, int32_t* free_head_out, int64_t B, int64_t num_tokens,
+                                 int64_t max_blocks, int64_t block_size, void* stream);
+
+/*
+ * Gives the pages of the requests with done[b] != 0 back: in request and page
+ * order they go to free_pages[free_head[0] - total .. free_head[0]), so they are
+ * taken next; context_lens_out is context_lens with 0 for them, free_head_out
+ * the list's new head.  More pages than the list has room for in front of its
+ * head are left out and reported by sa_device_status (SA_ERR_ARG).  No output
+ * may alias an input.  B <= 16384.  (No reference counterpart.)
+ */
+SA_API int sa_paged_release_pages(const int32_t* block_table, int64_t table_stride, const int32_t* context_lens,
+                                  const uint8_t* done, int32_t* free_pages, int64_t num_free,
+                                  const int32_t* free_head, int32_t* context_lens_out, int32_t* free_head_out,
+                                  int64_t B, int64_t max_blocks, int64_t block_size, void* stream);
+
+/*
+ * sa_qk_norm_rope of N flat tokens whose keys and values go into a paged
+ * cache.  q [N, Hq, D], k and v [N, Hkv, D] with strides {token, head, dim} in
+ * elements (dim stride 1, the others multiples of 8); q_out: contiguous
+ * [N, Hq, D]; k_cache, v_cache: contiguous [num_blocks, Hkv, block_size, D].
+ * Token n's k (normalised, rotated) and v (copied) rows go to slot slots[n] =
+ * page * block_size + offset.  A negative slot is padding: q_out's row is
+ * zeros, the caches are left as they are; a slot past the cache is treated the
+ * same and reported by sa_device_status (SA_ERR_ARG), as is a position outside
+ * the tables (read as 0).  A slot must not appear twice in a call.  positions:
+ * [N] of pos_bytes (4 or 8; 0: token n reads row n).  dtype SA_BF16 or SA_F16;
+ * the other arguments as sa_qk_norm_rope.  (No reference counterpart.)
+ */
+SA_API int sa_qk_norm_rope_paged_append(const void* q, const void* k, const void* v, void* q_out, void* k_cache,
+                                        void* v_cache, const int64_t* slots, const void* q_weight,
+                                        const void* k_weight, int w_dtype, const void* cos_table,
+                                        const void* sin_table, int cs_dtype, const void* positions, int pos_bytes,
+                                        int64_t num_pos, int64_t N, int64_t Hq, int64_t Hkv, int64_t D,
+                                        int64_t rotary_dim, int64_t num_blocks, int64_t block_size,
+                                        const int64_t* q_strides, const int64_t* k_strides, const int64_t* v_strides,
+                                        float eps, int normalize, int dtype, void* stream);
+
+/*
+ * Mean key of full pages: key_means[page, h] = mean over the page's block_size
+ * rows of k_cache[page, h], summed in fp32, rounded once.  Of sequence b the
+ * pages block_table[b, j], start_lens[b] / block_size <= j < context_lens[b] /
+ * block_size, are set (start_lens NULL: from 0); other rows are left alone.
+ * k_cache: contiguous [num_blocks, Hkv, block_size, D]; key_means: contiguous
+ * [num_blocks, Hkv, D]; block_table: contiguous [B, max_blocks].  An entry
+ * outside [0, num_blocks) is skipped and reported by sa_device_status
+ * (SA_ERR_ARG).  dtype SA_BF16 or SA_F16; D in {32, 64, 128, 256}; B * Hkv <=
+ * 65535.  (No reference counterpart.)
+ */
+SA_API int sa_paged_key_means(const void* k_cache, void* key_means, const int32_t* block_table,
+                              const int32_t* context_lens, const int32_t* start_lens, int64_t B, int64_t Hkv,
+                              int64_t num_blocks, int64_t block_size, int64_t max_blocks, int64_t D, int dtype,
+                              void* stream);
+
+/* Workspace bytes of sa_paged_select, or < 0. */
+SA_API int64_t sa_paged_select_workspace_size(int64_t B, int64_t Hkv, int64_t max_blocks);
+
+/*
+ * The pages of each sequence and key head that a decode over num_pages of them
+ * reads: the last one, and the num_pages - 1 others of the highest
+ *   score(page) = sum over the group's query heads of
+ *                 squareplus(2 scale q . key_means[page] - 1)^2
+ * in 64 bits, ties to the lowest page, NaN above all.  q: contiguous [B, Hq, D];
+ * pages: [B, Hkv, num_pages] indices into the block table's row, ascending, then
+ * -1; lens: [B, Hkv] tokens in them.  num_pages <= max_blocks.  workspace:
+ * 256-byte aligned, contents undefined on entry.  Block table entries outside
+ * the cache are read as page 0 and reported by sa_device_status (SA_ERR_ARG).
+ * Types and limits as sa_paged_key_means.  (No reference counterpart.)
+ */
+SA_API int sa_paged_select(const void* q, const void* key_means, const int32_t* block_table,
+                           const int32_t* context_lens, int32_t* pages, int32_t* lens, void* workspace,
+                           int64_t workspace_bytes, int64_t B, int64_t Hq, int64_t Hkv, int64_t num_blocks,
+                           int64_t block_size, int64_t max_blocks, int64_t num_pages, int64_t D, double scale,
+                           int dtype, void* stream);
+
+/* Workspace bytes of sa_sparse_paged_decode, or < 0. */
+SA_API int64_t sa_sparse_paged_decode_workspace_size(int64_t B, int64_t Hq, int64_t Hkv, int64_t max_blocks,
+                                                     int64_t num_pages, int64_t block_size, int64_t D, int dtype);
+
+/*
+ * sa_paged_decode over the pages that sa_paged_select chooses (pages:
+ * nullable).  The normaliser runs over the chosen pages' tokens.  workspace:
+ * 256-byte aligned, contents undefined on entry (the decode's tickets are
+ * cleared here), not shared by calls that may overlap on the GPU.  (No
+ * reference counterpart: the reference's decode reads every page.)
+ */
+SA_API int sa_sparse_paged_decode(const void* q, const void* k_cache, const void* v_cache, const void* key_means,
+                                  void* out, const int32_t* block_table, const int32_t* context_lens, int32_t* pages,
+                                  void* workspace, int64_t workspace_bytes, int64_t B, int64_t Hq, int64_t Hkv,
+                                  int64_t num_blocks, int64_t block_size, int64_t max_blocks, int64_t num_pages,
+                                  int64_t D, double scale, int dtype, void* stream);
 
 #ifdef __cplusplus
 }

@@ -30,6 +30,8 @@ int paged_tc_timeouts(int reset, cudaStream_t st);   // paged_tc.cu
 int paged_tc_bad_pages(int reset, cudaStream_t st);  // paged_tc.cu
 int proj_timeouts(int reset, cudaStream_t st);       // proj.cu
 int qk_bad_positions(int reset, cudaStream_t st);    // qk_norm_rope.cu
+int paged_cache_bad_entries(int reset, cudaStream_t st);  // paged_cache.cu
+int paged_select_bad_pages(int reset, cudaStream_t st);   // paged_select.cu
 // index checks that failed, per file (debug library; always 0 in release)
 int norm_bounds(int reset, cudaStream_t st);
 int flash_fwd_bounds(int reset, cudaStream_t st);
@@ -40,6 +42,8 @@ int rope_bounds(int reset, cudaStream_t st);
 int fp8_bounds(int reset, cudaStream_t st);
 int proj_bounds(int reset, cudaStream_t st);
 int qk_norm_rope_bounds(int reset, cudaStream_t st);
+int paged_cache_bounds(int reset, cudaStream_t st);
+int paged_select_bounds(int reset, cudaStream_t st);
 
 // Waits that the probe kernel below gave up on.
 __device__ unsigned g_probe_timeouts;
@@ -78,10 +82,12 @@ static int collect(int reset, cudaStream_t st) {
   const int n = norm_timeouts(reset, st) + flash_timeouts(reset, st) + flash_bwd_timeouts(reset, st) +
                 paged_timeouts(reset, st) + paged_tc_timeouts(reset, st) + probe_timeouts(reset, st) +
                 proj_timeouts(reset, st);
-  const int bad = paged_bad_pages(reset, st) + paged_tc_bad_pages(reset, st) + qk_bad_positions(reset, st);
+  const int bad = paged_bad_pages(reset, st) + paged_tc_bad_pages(reset, st) + qk_bad_positions(reset, st) +
+                  paged_cache_bad_entries(reset, st) + paged_select_bad_pages(reset, st);
   const int oob = norm_bounds(reset, st) + flash_fwd_bounds(reset, st) + flash_bwd_bounds(reset, st) +
                   paged_bounds(reset, st) + paged_tc_bounds(reset, st) + rope_bounds(reset, st) +
-                  fp8_bounds(reset, st) + proj_bounds(reset, st) + qk_norm_rope_bounds(reset, st);
+                  fp8_bounds(reset, st) + proj_bounds(reset, st) + qk_norm_rope_bounds(reset, st) +
+                  paged_cache_bounds(reset, st) + paged_select_bounds(reset, st);
   return n ? SA_ERR_TIMEOUT : oob ? SA_ERR_BOUNDS : bad ? SA_ERR_ARG : SA_OK;
 }
 }  // namespace sa

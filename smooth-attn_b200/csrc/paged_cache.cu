@@ -1,0 +1,456 @@
+// A paged key-value cache's bookkeeping and its writer, sm_100a: slots and
+// block tables from request lengths, pages given back, and the append of new
+// tokens (head norm and rotation on the way).  (No reference counterpart: the
+// reference's paged decode, src/smooth_attn/kernels.py:2681-2829, is handed a
+// filled cache and a block table built on the host.)
+//
+// Slots.  Request b holds context_lens[b] tokens in pages block_table[b, ..]
+// and gets new_lens[b] more, taken from a flat buffer of N tokens in request
+// order (cu = exclusive scan of new_lens).  With held = ceil(ctx / bs) pages
+// and need = ceil((ctx + new) / bs) - held further ones, an exclusive scan of
+// `need` says where in the pool's list its new pages begin: first come, first
+// served.  What does not fit (the table's row, the pool, the buffer) is left
+// out: those tokens get slot -1 and are not counted in the new length.
+// Both scans are over B <= 16384 requests, a few microseconds' work of one
+// block, so every block does them again for itself instead of waiting for
+// another: one launch, no workspace, nothing to reset.  A token finds its
+// request by a binary search of cu in shared memory, and the first token of a
+// new page writes the table's entry.  Bound: the launch and the two scans for
+// small batches, the 12 bytes written per token for large ones.
+//
+// Append.  One warp owns 32 / L tokens (L lanes a row, qk_rope.cuh) and some of
+// the q, k or v heads: q rows go to a dense buffer, k and v rows to their
+// slot's page.  Bound: HBM (each row read and written once).
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <cuda_runtime.h>
+#include <stdint.h>
+
+#include <algorithm>
+
+#include "qk_rope.cuh"
+#include "smooth_attn_b200.h"
+
+int sa_record_cuda_error(cudaError_t e);
+
+namespace sa {
+namespace pgc {
+
+static __device__ unsigned g_bad_entries;  // slots past the cache, positions past the tables, a pool given too much back
+
+constexpr int kThreads = 512;
+constexpr int kMaxRequests = 16384;
+
+// Exclusive scan of one int64 per thread over the block; returns the sum before this thread, total in *all.
+__device__ __forceinline__ int64_t block_scan(int64_t v, int64_t* all, int64_t* warp_sums) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, nw = blockDim.x >> 5;
+  int64_t inc = v;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int64_t u = __shfl_up_sync(0xffffffffu, inc, o);
+    if (lane >= o) inc += u;
+  }
+  if (lane == 31) warp_sums[warp] = inc;
+  __syncthreads();
+  if (warp == 0) {
+    int64_t s = lane < nw ? warp_sums[lane] : 0;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int64_t u = __shfl_up_sync(0xffffffffu, s, o);
+      if (lane >= o) s += u;
+    }
+    if (lane < nw) warp_sums[lane] = s;
+  }
+  __syncthreads();
+  const int64_t before = warp ? warp_sums[warp - 1] : 0;
+  *all = warp_sums[nw - 1];
+  __syncthreads();
+  return before + inc - v;
+}
+
+struct AssignArgs {
+  int32_t* table;
+  int64_t ld;
+  const int32_t* ctx;
+  const int32_t* fresh;  // new_lens
+  const int32_t* pool;
+  const int32_t* head;
+  long long* slots;
+  int32_t* positions;
+  int32_t* cu;
+  int32_t* ctx_out;
+  int32_t* head_out;
+  int64_t num_free;
+  int B, N, max_blocks, bs;
+};
+
+__global__ void __launch_bounds__(kThreads) paged_assign_kernel(AssignArgs a) {
+  extern __shared__ int32_t sm[];  // cu[B + 1], at[B], fits[B]
+  __shared__ int64_t warp_sums[32];
+  int32_t* cu = sm;
+  int32_t* at = cu + a.B + 1;
+  int32_t* fits = at + a.B;
+  const int64_t cap = (int64_t)a.max_blocks * a.bs;
+  const int per = (a.B + kThreads - 1) / kThreads;
+  const int b0 = min(a.B, (int)threadIdx.x * per), b1 = min(a.B, b0 + per);
+  auto held_tokens = [&](int b) { return max((int64_t)0, min(cap, (int64_t)a.ctx[b])); };
+
+  int64_t sum = 0, all;
+  for (int b = b0; b < b1; ++b) sum += max(0, a.fresh[b]);
+  int64_t run = block_scan(sum, &all, warp_sums);
+  sum = 0;
+  for (int b = b0; b < b1; ++b) {
+    const int64_t lo = min((int64_t)a.N, run);
+    run += max(0, a.fresh[b]);
+    const int64_t ctx = held_tokens(b);
+    const int64_t want = min(min((int64_t)a.N, run) - lo, cap - ctx);
+    cu[b] = (int32_t)lo;
+    fits[b] = (int32_t)want;
+    sum += (ctx + want + a.bs - 1) / a.bs - (ctx + a.bs - 1) / a.bs;
+  }
+  if (threadIdx.x == 0) cu[a.B] = (int32_t)min((int64_t)a.N, all);
+  const int64_t head = max((int64_t)0, min(a.num_free, (int64_t)*a.head));
+  run = head + block_scan(sum, &all, warp_sums);
+  for (int b = b0; b < b1; ++b) {
+    const int64_t ctx = held_tokens(b), held = (ctx + a.bs - 1) / a.bs;
+    const int64_t need = (ctx + fits[b] + a.bs - 1) / a.bs - held;
+    const int64_t have = max((int64_t)0, min(need, a.num_free - run));
+    fits[b] = (int32_t)min((int64_t)fits[b], (held + have) * a.bs - ctx);
+    at[b] = (int32_t)min(run, a.num_free);
+    run += need;
+  }
+  __syncthreads();
+  if (blockIdx.x == 0) {
+    for (int b = threadIdx.x; b <= a.B; b += kThreads) {
+      a.cu[b] = cu[b];
+      if (b < a.B) a.ctx_out[b] = (int32_t)(held_tokens(b) + fits[b]);
+    }
+    if (threadIdx.x == 0) *a.head_out = (int32_t)min(head + all, a.num_free);
+  }
+
+  for (int64_t i = (int64_t)blockIdx.x * kThreads + threadIdx.x; i < a.N; i += (int64_t)gridDim.x * kThreads) {
+    int64_t slot = -1;
+    int pos = 0;
+    if (i < cu[a.B]) {
+      int lo = 0, hi = a.B;  // the last b with cu[b] <= i: the one that holds token i (empty ones lie before it)
+      while (hi - lo > 1) {
+        const int mid = (lo + hi) >> 1;
+        if (cu[mid] <= i) lo = mid;
+        else hi = mid;
+      }
+      const int off = (int)i - cu[lo];
+      if (off < fits[lo]) {
+        const int ctx = (int)held_tokens(lo);
+        const int held = (ctx + a.bs - 1) / a.bs;
+        pos = ctx + off;
+        const int pi = pos / a.bs;
+        int page;
+        if (!SA_DCHECK(pi < a.max_blocks)) continue;
+        if (pi < held) {
+          page = a.table[lo * a.ld + pi];
+        } else {
+          page = a.pool[at[lo] + pi - held];
+          if (pos == pi * a.bs) a.table[lo * a.ld + pi] = page;
+        }
+        slot = page < 0 ? -1 : (int64_t)page * a.bs + (pos - pi * a.bs);
+      }
+    }
+    a.slots[i] = slot;
+    a.positions[i] = pos;
+  }
+}
+
+struct ReleaseArgs {
+  const int32_t* table;
+  int64_t ld;
+  const int32_t* ctx;
+  const uint8_t* done;
+  int32_t* pool;
+  const int32_t* head;
+  int32_t* ctx_out;
+  int32_t* head_out;
+  int64_t num_free;
+  int B, max_blocks, bs;
+};
+
+// Every block scans the ended requests' page counts; a warp copies one
+// request's pages to the list's entries in front of its head.
+__global__ void __launch_bounds__(kThreads) paged_release_kernel(ReleaseArgs a) {
+  extern __shared__ int64_t off[];  // [B]
+  __shared__ int64_t warp_sums[32];
+  const int64_t cap = (int64_t)a.max_blocks * a.bs;
+  const int per = (a.B + kThreads - 1) / kThreads;
+  const int b0 = min(a.B, (int)threadIdx.x * per), b1 = min(a.B, b0 + per);
+  auto pages_of = [&](int b) {
+    return a.done[b] ? (int)((max((int64_t)0, min(cap, (int64_t)a.ctx[b])) + a.bs - 1) / a.bs) : 0;
+  };
+  int64_t sum = 0, all;
+  for (int b = b0; b < b1; ++b) sum += pages_of(b);
+  int64_t run = block_scan(sum, &all, warp_sums);
+  for (int b = b0; b < b1; ++b) {
+    off[b] = run;
+    run += pages_of(b);
+  }
+  __syncthreads();
+  const int64_t head = max((int64_t)0, min(a.num_free, (int64_t)*a.head));
+  const int64_t first = head - all;
+  if (blockIdx.x == 0) {
+    for (int b = threadIdx.x; b < a.B; b += kThreads) a.ctx_out[b] = a.done[b] ? 0 : a.ctx[b];
+    if (threadIdx.x == 0) {
+      *a.head_out = (int32_t)max((int64_t)0, first);
+      if (first < 0) atomicAdd(&g_bad_entries, 1u);  // more pages than the pool had given out
+    }
+  }
+  const int lane = threadIdx.x & 31;
+  for (int64_t b = (int64_t)blockIdx.x * (kThreads / 32) + (threadIdx.x >> 5); b < a.B;
+       b += (int64_t)gridDim.x * (kThreads / 32)) {
+    const int n = pages_of((int)b);
+    for (int j = lane; j < n; j += 32) {
+      const int64_t to = first + off[b] + j;
+      if (to >= 0 && SA_DCHECK(to < a.num_free && j < a.max_blocks)) a.pool[to] = a.table[b * a.ld + j];
+    }
+  }
+}
+
+// ---- append -------------------------------------------------------------------
+
+using namespace qkr;
+
+constexpr int kWarps = 8;
+
+struct AppendSide {
+  const void* x;
+  const void* w;
+  int64_t xt, xh;  // token and head strides
+  int H, chunks;
+};
+
+struct AppendArgs {
+  AppendSide s[3];  // q, k, v
+  void* q_out;      // [N, Hq, D]
+  void* cache[2];   // k, v: [num_blocks, Hkv, bs, D]
+  const long long* slots;
+  int64_t N, groups, num_slots;
+  int w_dtype, hc, bs;
+};
+
+template <typename E, int L>
+__global__ void __launch_bounds__(kWarps * 32) qk_norm_rope_append(AppendArgs a, Tables tb) {
+  const int per = a.s[0].chunks + a.s[1].chunks + a.s[2].chunks;
+  const int64_t task = (int64_t)blockIdx.x * kWarps + (threadIdx.x >> 5);
+  if (task >= a.groups * per) return;  // the whole warp
+  const int64_t group = task / per;
+  int chunk = (int)(task - group * per), side = 0;
+  while (chunk >= a.s[side].chunks) chunk -= a.s[side++].chunks;
+  const AppendSide& sd = a.s[side];
+
+  const int64_t n = group * (32 / L) + (threadIdx.x & 31) / L;
+  const Lane ln = lane_of<L>(tb);
+  int64_t slot = n < a.N ? __ldg(a.slots + n) : -1;
+  if (slot >= a.num_slots) {
+    if (ln.o1 == 0 && side == 0 && chunk == 0) atomicAdd(&g_bad_entries, 1u);
+    slot = -1;
+  }
+  const bool mapped = slot >= 0;
+  const bool on = ln.active && mapped;
+  const E* x = static_cast<const E*>(sd.x) + n * sd.xt;
+  E* y;
+  int64_t yh;
+  if (side == 0) {
+    y = static_cast<E*>(a.q_out) + n * sd.H * tb.D;
+    yh = tb.D;
+  } else {
+    const int64_t page = mapped ? slot / a.bs : 0;
+    y = static_cast<E*>(a.cache[side - 1]) + (page * sd.H * a.bs + (mapped ? slot - page * a.bs : 0)) * tb.D;
+    yh = (int64_t)a.bs * tb.D;
+  }
+  float c[8], s[8], w1[8], w2[8];
+  Lane la = ln;
+  la.active = on;
+  if (side < 2) {
+    const int64_t p = on && tb.R > 0 ? (tb.pos_bytes ? read_pos(tb.pos, tb.pos_bytes, n) : n) : 0;
+    load_angles(tb, la, p, &g_bad_entries, c, s);
+    load_weights(sd.w, a.w_dtype, la, w1, w2);
+  }
+  const int h0 = chunk * a.hc, h1 = min(sd.H, h0 + a.hc);
+  constexpr int U = 4;  // heads in flight
+  for (int h = h0; h < h1; h += U) {
+    Raw8<E> p[U], q[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      if (on && h + u < h1) {
+        p[u].load(x + (h + u) * sd.xh + ln.o1);
+        q[u].load(x + (h + u) * sd.xh + ln.o2);
+      } else {
+        p[u].zero();
+        q[u].zero();
+      }
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      if (h + u >= h1) break;  // uniform over the warp
+      if (side < 2) norm_rope<E, L>(tb, p[u], q[u], w1, w2, c, s);
+      if (side == 0 && !mapped) p[u].zero(), q[u].zero();  // a padding token's q row is zeros
+      const bool write = side == 0 ? ln.active && n < a.N : on;
+      if (write && SA_DCHECK(h + u < sd.H && ln.o2 + 8 <= tb.D)) {
+        p[u].store(y + (h + u) * yh + ln.o1);
+        q[u].store(y + (h + u) * yh + ln.o2);
+      }
+    }
+  }
+}
+
+static int sm_count() {
+  int dev = 0, n = 148;
+  if (cudaGetDevice(&dev) != cudaSuccess || cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess) {
+    cudaGetLastError();
+    n = 148;
+  }
+  return n;
+}
+
+template <typename E>
+static int launch_append(const AppendArgs& a, const Tables& tb, cudaStream_t st) {
+  const int64_t tasks = a.groups * (a.s[0].chunks + a.s[1].chunks + a.s[2].chunks);
+  const int64_t blocks = (tasks + kWarps - 1) / kWarps;
+  if (blocks > INT32_MAX) return SA_ERR_UNSUPPORTED;
+  switch (lanes_for(tb.D)) {
+    case 1: qk_norm_rope_append<E, 1><<<(unsigned)blocks, kWarps * 32, 0, st>>>(a, tb); break;
+    case 2: qk_norm_rope_append<E, 2><<<(unsigned)blocks, kWarps * 32, 0, st>>>(a, tb); break;
+    case 4: qk_norm_rope_append<E, 4><<<(unsigned)blocks, kWarps * 32, 0, st>>>(a, tb); break;
+    case 8: qk_norm_rope_append<E, 8><<<(unsigned)blocks, kWarps * 32, 0, st>>>(a, tb); break;
+    default: qk_norm_rope_append<E, 16><<<(unsigned)blocks, kWarps * 32, 0, st>>>(a, tb); break;
+  }
+  return sa_record_cuda_error(cudaGetLastError());
+}
+
+// Opt-in to `bytes` of dynamic shared memory (the requests' scans).
+template <typename F> static int opt_in(F* f, size_t bytes) {
+  if (bytes <= 48 * 1024) return SA_OK;
+  return sa_record_cuda_error(cudaFuncSetAttribute(f, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes));
+}
+
+static int check_requests(int64_t B, int64_t max_blocks, int64_t bs, int64_t ld, int64_t num_free) {
+  if (B < 0 || max_blocks <= 0 || bs <= 0 || ld < max_blocks || num_free < 0) return SA_ERR_ARG;
+  if (B > kMaxRequests || max_blocks > INT32_MAX || bs > (1 << 16) || max_blocks * bs > ((int64_t)1 << 30) ||
+      num_free > INT32_MAX)
+    return SA_ERR_UNSUPPORTED;
+  return SA_OK;
+}
+
+}  // namespace pgc
+
+int paged_cache_bad_entries(int reset, cudaStream_t st) {
+  unsigned v = 0;
+  cudaMemcpyFromSymbolAsync(&v, pgc::g_bad_entries, sizeof(v), 0, cudaMemcpyDeviceToHost, st);
+  cudaStreamSynchronize(st);
+  if (reset) {
+    const unsigned z = 0;
+    cudaMemcpyToSymbolAsync(pgc::g_bad_entries, &z, sizeof(z), 0, cudaMemcpyHostToDevice, st);
+    cudaStreamSynchronize(st);
+  }
+  return (int)v;
+}
+
+}  // namespace sa
+
+extern "C" int sa_paged_assign_slots(int32_t* block_table, int64_t table_stride, const int32_t* context_lens,
+                                     const int32_t* new_lens, const int32_t* free_pages, int64_t num_free,
+                                     const int32_t* free_head, int64_t* slots, int32_t* positions,
+                                     int32_t* cu_seqlens, int32_t* context_lens_out, int32_t* free_head_out,
+                                     int64_t B, int64_t num_tokens, int64_t max_blocks, int64_t block_size,
+                                     void* stream) {
+  using namespace sa::pgc;
+  const int rc = check_requests(B, max_blocks, block_size, table_stride, num_free);
+  if (rc != SA_OK) return rc;
+  if (num_tokens < 0) return SA_ERR_ARG;
+  if (num_tokens > INT32_MAX - kThreads) return SA_ERR_UNSUPPORTED;
+  if (!free_head || !cu_seqlens || !free_head_out) return SA_ERR_ARG;
+  if (B > 0 && (!block_table || !context_lens || !new_lens || !context_lens_out)) return SA_ERR_ARG;
+  if (num_free > 0 && !free_pages) return SA_ERR_ARG;
+  if (num_tokens > 0 && (!slots || !positions)) return SA_ERR_ARG;
+  AssignArgs a{block_table, table_stride, context_lens, new_lens, free_pages, free_head,
+               reinterpret_cast<long long*>(slots), positions, cu_seqlens, context_lens_out, free_head_out, num_free,
+               (int)B, (int)num_tokens, (int)max_blocks, (int)block_size};
+  const size_t smem = (3 * (size_t)B + 1) * 4;
+  const int orc = opt_in(paged_assign_kernel, smem);
+  if (orc != SA_OK) return orc;
+  const int64_t blocks = std::max<int64_t>(1, std::min<int64_t>((num_tokens + 4 * kThreads - 1) / (4 * kThreads), 2ll * sm_count()));
+  paged_assign_kernel<<<(unsigned)blocks, kThreads, smem, static_cast<cudaStream_t>(stream)>>>(a);
+  return sa_record_cuda_error(cudaGetLastError());
+}
+
+extern "C" int sa_paged_release_pages(const int32_t* block_table, int64_t table_stride, const int32_t* context_lens,
+                                      const uint8_t* done, int32_t* free_pages, int64_t num_free,
+                                      const int32_t* free_head, int32_t* context_lens_out, int32_t* free_head_out,
+                                      int64_t B, int64_t max_blocks, int64_t block_size, void* stream) {
+  using namespace sa::pgc;
+  const int rc = check_requests(B, max_blocks, block_size, table_stride, num_free);
+  if (rc != SA_OK) return rc;
+  if (!free_head || !free_head_out) return SA_ERR_ARG;
+  if (B > 0 && (!block_table || !context_lens || !done || !context_lens_out)) return SA_ERR_ARG;
+  if (num_free > 0 && !free_pages) return SA_ERR_ARG;
+  ReleaseArgs a{block_table, table_stride, context_lens, done, free_pages, free_head, context_lens_out, free_head_out,
+                num_free, (int)B, (int)max_blocks, (int)block_size};
+  const size_t smem = (size_t)std::max<int64_t>(B, 1) * 8;
+  const int orc = opt_in(paged_release_kernel, smem);
+  if (orc != SA_OK) return orc;
+  const int64_t blocks = std::max<int64_t>(1, std::min<int64_t>((B + 15) / 16, sm_count()));
+  paged_release_kernel<<<(unsigned)blocks, kThreads, smem, static_cast<cudaStream_t>(stream)>>>(a);
+  return sa_record_cuda_error(cudaGetLastError());
+}
+
+extern "C" int sa_qk_norm_rope_paged_append(const void* q, const void* k, const void* v, void* q_out, void* k_cache,
+                                            void* v_cache, const int64_t* slots, const void* q_weight,
+                                            const void* k_weight, int w_dtype, const void* cos_table,
+                                            const void* sin_table, int cs_dtype, const void* positions,
+                                            int pos_bytes, int64_t num_pos, int64_t N, int64_t Hq, int64_t Hkv,
+                                            int64_t D, int64_t rotary_dim, int64_t num_blocks, int64_t block_size,
+                                            const int64_t* q_strides, const int64_t* k_strides,
+                                            const int64_t* v_strides, float eps, int normalize, int dtype,
+                                            void* stream) {
+  using namespace sa::pgc;
+  if (N < 0 || Hq < 0 || Hkv <= 0 || num_blocks < 0 || block_size <= 0) return SA_ERR_ARG;
+  if (dtype != SA_BF16 && dtype != SA_F16) return SA_ERR_UNSUPPORTED;
+  if (Hq > (1 << 20) || Hkv > (1 << 20) || N > ((int64_t)1 << 33) || block_size > (1 << 16) ||
+      num_blocks > ((int64_t)1 << 40))
+    return SA_ERR_UNSUPPORTED;
+  sa::qkr::Tables tb;
+  const int rc = sa::qkr::make_tables(&tb, cos_table, sin_table, cs_dtype, positions, pos_bytes, 0, num_pos, N, D,
+                                      rotary_dim, eps, normalize, q_weight, k_weight, w_dtype);
+  if (rc != SA_OK) return rc;
+  if (N == 0) return SA_OK;
+  if (!slots || !q_strides || !k_strides || !v_strides || !k || !v || (Hq > 0 && (!q || !q_out)) ||
+      (num_blocks > 0 && (!k_cache || !v_cache)))
+    return SA_ERR_ARG;
+  using sa::qkr::al16;
+  if (!al16(q) || !al16(k) || !al16(v) || !al16(q_out) || !al16(k_cache) || !al16(v_cache)) return SA_ERR_ALIGN;
+  const int64_t* st3[3] = {q_strides, k_strides, v_strides};
+  for (const int64_t* s : st3)
+    if (s[2] != 1 || s[0] % 8 != 0 || s[1] % 8 != 0) return SA_ERR_ALIGN;
+  AppendArgs a;
+  const int per = 32 / sa::qkr::lanes_for(D);
+  a.N = N;
+  a.groups = (N + per - 1) / per;
+  a.num_slots = num_blocks * block_size;
+  a.w_dtype = w_dtype;
+  a.bs = (int)block_size;
+  a.hc = sa::qkr::heads_per_warp(a.groups, Hq + 2 * Hkv, 16ll * sm_count());
+  a.q_out = q_out;
+  a.cache[0] = k_cache;
+  a.cache[1] = v_cache;
+  a.slots = reinterpret_cast<const long long*>(slots);
+  const void* xs[3] = {q, k, v};
+  const void* ws[3] = {q_weight, k_weight, nullptr};
+  for (int i = 0; i < 3; ++i) {
+    a.s[i].x = xs[i];
+    a.s[i].w = ws[i];
+    a.s[i].xt = st3[i][0];
+    a.s[i].xh = st3[i][1];
+    a.s[i].H = (int)(i == 0 ? Hq : Hkv);
+    a.s[i].chunks = (a.s[i].H + a.hc - 1) / a.hc;
+  }
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  return dtype == SA_BF16 ? launch_append<__nv_bfloat16>(a, tb, st) : launch_append<__half>(a, tb, st);
+}
+SA_BOUNDS_ACCESSOR(paged_cache_bounds)

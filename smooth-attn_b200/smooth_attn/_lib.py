@@ -31,6 +31,7 @@ SA_F32, SA_F16, SA_BF16 = 0, 1, 2
 _i64 = ctypes.c_int64
 _int = ctypes.c_int
 _f = ctypes.c_float
+_d = ctypes.c_double
 _p = ctypes.c_void_p
 _i64p = ctypes.POINTER(ctypes.c_int64)
 
@@ -83,6 +84,18 @@ SIGNATURES = {
     "sa_paged_decode_workspace_size": (_i64, [_i64, _i64, _i64, _i64, _i64, _i64, _int]),
     "sa_paged_decode": (_int, [_p, _p, _p, _p, _p, _p, _p, _i64,
                                _i64, _i64, _i64, _i64, _i64, _i64, _i64, _f, _int, _p]),
+    "sa_paged_assign_slots": (_int, [_p, _i64, _p, _p, _p, _i64, _p, _p, _p, _p, _p, _p, _i64, _i64, _i64, _i64, _p]),
+    "sa_paged_release_pages": (_int, [_p, _i64, _p, _p, _p, _i64, _p, _p, _p, _i64, _i64, _i64, _p]),
+    "sa_qk_norm_rope_paged_append": (_int, [_p, _p, _p, _p, _p, _p, _p, _p, _p, _int, _p, _p, _int, _p, _int, _i64,
+                                            _i64, _i64, _i64, _i64, _i64, _i64, _i64, _i64p, _i64p, _i64p, _f, _int,
+                                            _int, _p]),
+    "sa_paged_key_means": (_int, [_p, _p, _p, _p, _p, _i64, _i64, _i64, _i64, _i64, _i64, _int, _p]),
+    "sa_paged_select_workspace_size": (_i64, [_i64, _i64, _i64]),
+    "sa_paged_select": (_int, [_p, _p, _p, _p, _p, _p, _p, _i64,
+                               _i64, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _d, _int, _p]),
+    "sa_sparse_paged_decode_workspace_size": (_i64, [_i64, _i64, _i64, _i64, _i64, _i64, _i64, _int]),
+    "sa_sparse_paged_decode": (_int, [_p, _p, _p, _p, _p, _p, _p, _p, _p, _i64,
+                                      _i64, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _d, _int, _p]),
 }
 
 _lock = threading.Lock()

@@ -10,7 +10,8 @@ costs tens of microseconds, which would dominate the small decode calls).
 
 Each op's real implementation is the direct launcher; its fake
 implementation allocates outputs of the same shapes, dtypes and strides.
-Outputs never alias inputs.  Ops (namespace ``smooth_attn_b200``):
+Outputs never alias inputs; the paged cache's ops update the arguments marked
+* in place.  Ops (namespace ``smooth_attn_b200``):
 
 * ``norm_fwd(x, alpha, theta, power, causal, with_rowsum) -> (out, rowsum)``
 * ``norm_causal_bwd(x, g, rowsum, alpha, theta, power) -> dx``
@@ -28,6 +29,16 @@ the backward ops take an empty ``o_lo`` for "none".
 * ``qk_norm_rope(q, k, q_weight, k_weight, cos, sin, positions, eps) -> (q, k)``
 * ``qk_norm_rope_bwd(q, k, dq_out, dk_out, q_weight, k_weight, cos, sin, positions, eps, need_dw)
   -> (dq, dk, dq_weight, dk_weight)`` (an empty gradient for a weight that is None or not needed)
+* ``paged_assign_slots(*block_table, context_lens, new_lens, free_pages, free_head, num_tokens, block_size)
+  -> (slot_mapping, positions, cu_seqlens, context_lens, free_head)``
+* ``paged_release_pages(block_table, context_lens, done, *free_pages, free_head, block_size)
+  -> (context_lens, free_head)``
+* ``qk_norm_rope_paged_append(q, k, v, *k_cache, *v_cache, slot_mapping, cos, sin, positions, q_weight,
+  k_weight, eps) -> q``
+* ``paged_key_means(*key_means, k_cache, block_table, context_lens, start_lens)``
+* ``paged_select(q, key_means, block_table, context_lens, num_pages, scale, block_size) -> (pages, lens)``
+* ``sparse_paged_decode(q, k_cache, v_cache, key_means, block_table, context_lens, num_pages, scale,
+  block_size) -> (out, pages)``
 * ``paged_decode(q, k_cache, v_cache, block_table, context_lens, scale, block_size) -> out``
 """
 
@@ -37,6 +48,7 @@ import torch
 from torch import Tensor
 
 from . import kernels as K
+from . import paged_cache as P
 from . import qk_rope as R
 
 NS = "smooth_attn_b200"
@@ -216,3 +228,83 @@ def _(q, k, dq_out, dk_out, q_weight, k_weight, cos, sin, positions, eps, need_d
     dw = tuple(torch.empty(w.shape, device=q.device, dtype=w.dtype) if need_dw and w is not None else q.new_empty(0)
                for w in (q_weight, k_weight))
     return tuple(torch.empty(t.shape, device=q.device, dtype=q.dtype) for t in (q, k)) + dw
+
+
+# ------------------------------------------------------------------ paged cache
+
+
+@torch.library.custom_op(f"{NS}::paged_assign_slots", mutates_args=("block_table",), device_types="cuda")
+def paged_assign_slots(block_table: Tensor, context_lens: Tensor, new_lens: Tensor, free_pages: Tensor,
+                       free_head: Tensor, num_tokens: int,
+                       block_size: int) -> tuple[Tensor, Tensor, Tensor, Tensor, Tensor]:
+    # (outputs of a custom op may not share storage: the direct call's int32 ones do)
+    s = P._assign_direct(block_table, context_lens, new_lens, free_pages, free_head, num_tokens, block_size)
+    return (s.slot_mapping, s.positions.clone(), s.cu_seqlens.clone(), s.context_lens.clone(), s.free_head.clone())
+
+
+@paged_assign_slots.register_fake
+def _(block_table, context_lens, new_lens, free_pages, free_head, num_tokens, block_size):
+    B, dev = block_table.shape[0], block_table.device
+    return (torch.empty(num_tokens, device=dev, dtype=torch.int64),
+            *(torch.empty(n, device=dev, dtype=torch.int32) for n in (num_tokens, B + 1, B, 1)))
+
+
+@torch.library.custom_op(f"{NS}::paged_release_pages", mutates_args=("free_pages",), device_types="cuda")
+def paged_release_pages(block_table: Tensor, context_lens: Tensor, done: Tensor, free_pages: Tensor,
+                        free_head: Tensor, block_size: int) -> tuple[Tensor, Tensor]:
+    return P._release_direct(block_table, context_lens, done, free_pages, free_head, block_size)
+
+
+@paged_release_pages.register_fake
+def _(block_table, context_lens, done, free_pages, free_head, block_size):
+    return torch.empty_like(context_lens), torch.empty_like(free_head)
+
+
+@torch.library.custom_op(f"{NS}::qk_norm_rope_paged_append", mutates_args=("k_cache", "v_cache"), device_types="cuda")
+def qk_norm_rope_paged_append(q: Tensor, k: Tensor, v: Tensor, k_cache: Tensor, v_cache: Tensor, slot_mapping: Tensor,
+                              cos: Tensor | None, sin: Tensor | None, positions: Tensor | None,
+                              q_weight: Tensor | None, k_weight: Tensor | None, eps: float | None) -> Tensor:
+    return P._append_direct(q, k, v, k_cache, v_cache, slot_mapping, cos, sin, positions, q_weight, k_weight, eps)
+
+
+@qk_norm_rope_paged_append.register_fake
+def _(q, k, v, k_cache, v_cache, slot_mapping, cos, sin, positions, q_weight, k_weight, eps):
+    return torch.empty(q.shape, device=q.device, dtype=q.dtype)
+
+
+@torch.library.custom_op(f"{NS}::paged_key_means", mutates_args=("key_means",), device_types="cuda")
+def paged_key_means(key_means: Tensor, k_cache: Tensor, block_table: Tensor, context_lens: Tensor,
+                    start_lens: Tensor | None) -> None:
+    P._means_direct(key_means, k_cache, block_table, context_lens, start_lens)
+
+
+@paged_key_means.register_fake
+def _(key_means, k_cache, block_table, context_lens, start_lens):
+    return None
+
+
+@torch.library.custom_op(f"{NS}::paged_select", mutates_args=(), device_types="cuda")
+def paged_select(q: Tensor, key_means: Tensor, block_table: Tensor, context_lens: Tensor, num_pages: int, scale: float,
+                 block_size: int) -> tuple[Tensor, Tensor]:
+    return P._select_direct(q, key_means, block_table, context_lens, num_pages, scale, block_size)
+
+
+@paged_select.register_fake
+def _(q, key_means, block_table, context_lens, num_pages, scale, block_size):
+    B, Hkv = q.shape[0], key_means.shape[1]
+    return (torch.empty(B, Hkv, num_pages, device=q.device, dtype=torch.int32),
+            torch.empty(B, Hkv, device=q.device, dtype=torch.int32))
+
+
+@torch.library.custom_op(f"{NS}::sparse_paged_decode", mutates_args=(), device_types="cuda")
+def sparse_paged_decode(q: Tensor, k_cache: Tensor, v_cache: Tensor, key_means: Tensor, block_table: Tensor,
+                        context_lens: Tensor, num_pages: int, scale: float,
+                        block_size: int) -> tuple[Tensor, Tensor]:
+    return P._sparse_direct(q, k_cache, v_cache, key_means, block_table, context_lens, num_pages, scale, block_size)
+
+
+@sparse_paged_decode.register_fake
+def _(q, k_cache, v_cache, key_means, block_table, context_lens, num_pages, scale, block_size):
+    B, H, _, D = q.shape
+    return (torch.empty(B, H, D, device=q.device, dtype=torch.bfloat16),
+            torch.empty(B, key_means.shape[1], num_pages, device=q.device, dtype=torch.int32))

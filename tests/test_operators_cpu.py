@@ -138,3 +138,159 @@ def test_c_abi_refuses_rope_arguments_before_launch():
     assert bwd(dw=16, w=16, norm=0) == _lib.SA_ERR_ARG
     assert bwd(dw=16, w=16, ws=None) == _lib.SA_ERR_ARG and bwd(dw=16, w=16, nbytes=8) == _lib.SA_ERR_ARG
     assert bwd() == _lib.SA_ERR_ALIGN  # dk's channel stride
+
+
+# ------------------------------------------------------------------ paged cache
+
+
+def _i(*shape, dtype=torch.int32):
+    return torch.zeros(*shape, dtype=dtype, device="cuda")
+
+
+def test_paged_slots_refuse(fake):
+    f = sa.paged_assign_slots
+    t, n, p, h = _i(3, 4), _i(3), _i(9), _i(1)
+    for bad in (_i(3), _i(3, 4, dtype=torch.int64), _i(4, 3).T, _i(3, 0), torch.zeros(3, 4, dtype=torch.int32)):
+        with pytest.raises(ValueError):
+            f(bad, n, n, p, h, 3)
+    with pytest.raises(TypeError):
+        f([[1]], n, n, p, h, 3)
+    with pytest.raises(TypeError):
+        f(t, [1, 2, 3], n, p, h, 3)
+    for ctx, new, pool, head, N in ((_i(2), n, p, h, 3), (n, _i(4), p, h, 3), (n, n, _i(3, 3), h, 3),
+                                    (n, n, p, _i(2), 3), (n, n, p, h, -1), (n, n, p, h, 2 ** 31),
+                                    (n, _i(3, dtype=torch.float32), p, h, 3), (n.cpu(), n, p, h, 3)):
+        with pytest.raises(ValueError):
+            f(t, ctx, new, pool, head, N)
+    with pytest.raises(ValueError, match="block_size"):
+        f(t, n, n, p, h, 3, block_size=0)
+    with pytest.raises(ValueError, match="16384"):
+        f(_i(16385, 2), _i(16385), _i(16385), p, h, 3)
+    r, d = sa.paged_release_pages, torch.zeros(3, dtype=torch.bool, device="cuda")
+    for done, pool in ((n, p), (d[:2], p), (d, _i(9, dtype=torch.int64)), (d, _i(18)[::2]), (d, _i(3, 3)),
+                       (d.cpu(), p)):
+        with pytest.raises(ValueError):
+            r(t, n, done, pool, h)
+    s = f(t, n, n, p, h, 7)
+    assert [tuple(x.shape) for x in s] == [(7,), (7,), (4,), (3,), (1,)] and s.slot_mapping.dtype == torch.int64
+    ctx, head = r(t, n, d, p, h)
+    assert ctx.shape == (3,) and head.shape == (1,)
+
+
+def test_paged_append_refuses(fake):
+    f = sa.qk_norm_rope_paged_append
+    q, k, c = _t(5, 4, 64), _t(5, 2, 64), _t(6, 2, 16, 64)
+    s, cs, pos = _i(5, dtype=torch.int64), _t(9, 32, dtype=torch.float32), _i(5)
+    with pytest.raises(AssertionError):
+        f(q, k, _t(5, 3, 64), c, c, s)
+    with pytest.raises(AssertionError):
+        f(q[:4], k, k, c, c, s)
+    for args in ((q.float(), k.float(), k.float(), c, c, s), (q, k.half(), k, c, c, s), (q, k, k, c.half(), c.half(), s),
+                 (q, k, k, c, c[:5], s), (q, k, k, _t(6, 3, 16, 64), _t(6, 3, 16, 64), s),
+                 (q, k, k, c.transpose(1, 2), c, s), (q, k, k, c[0], c[0], s), (q, k, k, c, c, s.int()),
+                 (q, k, k, c, c, s[:4]), (q, k, k, c, c, s.cpu()), (q, k, k, c, c, s, cs, cs)):
+        with pytest.raises(ValueError):
+            f(*args)
+    with pytest.raises(ValueError):
+        f(q, k, k, c, c, s, cs, cs, positions=_i(4))
+    with pytest.raises(ValueError, match="backward"):
+        f(q.clone().requires_grad_(True), k, k, c, c, s)
+    with pytest.raises(ValueError, match="CUDA"):
+        f(*(torch.zeros(1, 1, 64, dtype=torch.bfloat16),) * 3, c, c, s)
+    assert f(q, k, k, c, c, s, cs, cs, positions=pos).shape == q.shape
+
+
+def test_page_choice_refuses(fake):
+    q, m, c, bt, cl = _t(2, 4, 1, 64), _t(6, 2, 64), _t(6, 2, 16, 64), _i(2, 3), _i(2)
+    f = sa.sp2norm_sparse_paged_attention
+    with pytest.raises(AssertionError):
+        f(q[:, :, 0], c, c, m, bt, cl, 2)
+    with pytest.raises(AssertionError):
+        f(_t(2, 3, 1, 64), c, c, m, bt, cl, 2)
+    for args in ((q.float(), c, c, m, bt, cl, 2), (q, c, c, m, bt, cl, 0), (q, c, c, m.half(), bt, cl, 2),
+                 (q, c, c[:5], m, bt, cl, 2), (q, c, c, _t(6, 2, 32), bt, cl, 2), (q, c, c, m[:, 0], bt, cl, 2),
+                 (q, c, c, m, bt[:1], cl, 2), (q, c, c, m, bt, cl[:1], 2), (q, c, c, m, bt[0], cl, 2),
+                 (q, c.transpose(1, 2), c, m, bt, cl, 2), (q, c, c, m, bt.cpu(), cl, 2),
+                 (_t(2, 4, 1, 96), c, c, m, bt, cl, 2)):
+        with pytest.raises(ValueError):
+            f(*args)
+    with pytest.raises(ValueError, match="block_size"):
+        f(q, c, c, m, bt, cl, 2, block_size=8)
+    out, pages = f(q, c, c, m, bt, cl, 9, return_pages=True)
+    assert out.shape == (2, 4, 64) and pages.shape == (2, 2, 3)
+    assert sa.sp2norm_paged_select(q, m, bt, cl, 2)[0].shape == (2, 2, 2)
+    g = sa.paged_key_means
+    for args in ((m, c.float(), bt, cl), (m[:5], c, bt, cl), (m.half(), c, bt, cl), (m, c[0], bt, cl),
+                 (m, c, bt[0], cl), (m, c, bt, cl[:1]), (m, c.transpose(1, 2), bt, cl)):
+        with pytest.raises(ValueError):
+            g(*args)
+    with pytest.raises(ValueError):
+        g(m, c, bt, cl, start_lens=_i(3))
+    assert g(m, c, bt, cl, start_lens=cl) is m
+
+
+def test_paged_operators_trace(fake):
+    q, k, c, m = _t(2, 4, 64), _t(2, 2, 64), _t(6, 2, 16, 64), _t(6, 2, 64)
+    bt, cl, p, h, d = _i(2, 3), _i(2), _i(9), _i(1), torch.zeros(2, dtype=torch.bool, device="cuda")
+
+    def f(q, k, c, v, m, bt, cl, p, h, d):
+        cl, h = sa.paged_release_pages(bt, cl, d, p, h)
+        s = sa.paged_assign_slots(bt, cl, torch.ones_like(cl), p, h, 2)
+        q = sa.qk_norm_rope_paged_append(q, k, k, c, v, s.slot_mapping)
+        sa.paged_key_means(m, c, bt, s.context_lens, start_lens=cl)
+        pages, _ = sa.sp2norm_paged_select(q[:, :, None], m, bt, s.context_lens, 2)
+        return sa.sp2norm_sparse_paged_attention(q[:, :, None], c, v, m, bt, s.context_lens, 2), pages
+
+    t = _targets(f, q, k, c, c.clone(), m, bt, cl, p, h, d)
+    for op in ("paged_release_pages", "paged_assign_slots", "qk_norm_rope_paged_append", "paged_key_means",
+               "paged_select", "sparse_paged_decode"):
+        assert t.count(f"smooth_attn_b200.{op}.default") == 1, op
+
+
+def test_c_abi_refuses_paged_arguments_before_launch():
+    lib = _lib.load()
+    A, U, L, OK = _lib.SA_ERR_ARG, _lib.SA_ERR_UNSUPPORTED, _lib.SA_ERR_ALIGN, _lib.SA_OK
+
+    def assign(B=2, N=2, mb=4, bs=16, ld=4, free=8, p=16, head=16):
+        return lib.sa_paged_assign_slots(p, ld, p, p, p, free, head, p, p, p, p, p, B, N, mb, bs, None)
+
+    assert assign(B=-1) == A and assign(mb=0) == A and assign(bs=0) == A and assign(ld=3) == A and assign(free=-1) == A
+    assert assign(B=16385) == U and assign(bs=1 << 17) == U and assign(mb=1 << 28, ld=1 << 28) == U
+    assert assign(N=-1) == A and assign(N=2 ** 31) == U and assign(p=None) == A and assign(head=None) == A
+    rel = lambda B=2, mb=4, ld=4, p=16, head=16: lib.sa_paged_release_pages(  # noqa: E731
+        p, ld, p, p, p, 8, head, p, p, B, mb, 16, None)
+    assert rel(B=-1) == A and rel(ld=3) == A and rel(B=16385) == U and rel(p=None) == A and rel(head=None) == A
+    s3 = _s(128, 64, 1)
+
+    def append(N=2, Hq=2, Hkv=2, D=64, dtype=_lib.SA_BF16, p=16, s=s3, bs=16, slots=16, nb=3):
+        return lib.sa_qk_norm_rope_paged_append(p, p, p, p, p, p, slots, None, None, 0, None, None, 0, None, 0, 0, N, Hq,
+                                                Hkv, D, 0, nb, bs, s, s, s, 1e-6, 1, dtype, None)
+
+    assert append(N=-1) == A and append(Hkv=0) == A and append(bs=0) == A and append(nb=-1) == A
+    assert append(dtype=_lib.SA_F32) == U and append(D=24) == U and append(p=None) == A and append(slots=None) == A
+    assert append(p=8) == L and append(s=_s(128, 60, 1)) == L and append(s=_s(128, 64, 2)) == L
+    assert append(N=0, p=None) == OK
+
+    def means(B=1, Hkv=2, nb=3, bs=16, mb=4, D=64, dtype=_lib.SA_BF16, p=16):
+        return lib.sa_paged_key_means(p, p, p, p, None, B, Hkv, nb, bs, mb, D, dtype, None)
+
+    assert means(B=-1) == A and means(nb=0) == A and means(mb=0) == A and means(p=None) == A and means(p=8) == L
+    assert means(D=48) == U and means(dtype=0) == U and means(B=65535) == U and means(nb=2 ** 31) == U
+    assert means(B=0, p=None) == OK
+
+    def sparse(B=1, Hq=4, Hkv=2, nb=3, bs=16, mb=4, K=2, D=64, scale=0.1, dtype=_lib.SA_BF16, p=16, ws=256,
+               nbytes=1 << 30):
+        a = lib.sa_paged_select(p, p, p, p, p, p, ws, nbytes, B, Hq, Hkv, nb, bs, mb, K, D, scale, dtype, None)
+        b = lib.sa_sparse_paged_decode(p, p, p, p, p, p, p, None, ws, nbytes, B, Hq, Hkv, nb, bs, mb, K, D, scale, dtype,
+                                       None)
+        assert a == b
+        return a
+
+    assert sparse(K=0) == A and sparse(K=5) == A and sparse(Hq=3) == A and sparse(Hq=0) == A
+    assert sparse(scale=float("nan")) == A and sparse(D=48) == U and sparse(dtype=0) == U and sparse(B=65536) == U
+    assert sparse(p=None) == A and sparse(ws=None) == A and sparse(nbytes=16) == A and sparse(p=8) == L
+    assert sparse(ws=128) == L and sparse(B=0, p=None) == OK
+    assert lib.sa_paged_select_workspace_size(2, 8, 512) == 2 * 8 * 512 * 8
+    assert lib.sa_paged_select_workspace_size(65536, 1, 1) == U
+    assert lib.sa_sparse_paged_decode_workspace_size(2, 32, 8, 512, 64, 16, 128, _lib.SA_BF16) > 2 * 8 * 512 * 8
+    assert lib.sa_sparse_paged_decode_workspace_size(2, 32, 8, 512, 0, 16, 128, _lib.SA_BF16) == A
