@@ -18,9 +18,9 @@
 // new page writes the table's entry.  Bound: the launch and the two scans for
 // small batches, the 12 bytes written per token for large ones.
 //
-// Append.  One warp owns 32 / L tokens (L lanes a row, qk_rope.cuh) and some of
-// the q, k or v heads: q rows go to a dense buffer, k and v rows to their
-// slot's page.  Bound: HBM (each row read and written once).
+// Append.  The walk of qk_rope.cuh over the q, k and v rows, each warp a part of
+// one of the three: q rows go to a dense buffer, k and v rows to their slot's
+// page.  Bound: HBM (each row read and written once).
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
@@ -216,13 +216,13 @@ __global__ void __launch_bounds__(kThreads) paged_release_kernel(ReleaseArgs a) 
 
 using namespace qkr;
 
-constexpr int kWarps = 8;
-
 struct AppendSide {
   const void* x;
   const void* w;
-  int64_t xt, xh;  // token and head strides
-  int H, chunks;
+  int64_t xt, xh;   // token and head strides
+  int64_t units;    // groups * per
+  int64_t warp0;    // first warp of this side
+  int H, C, per;    // heads, heads of a unit, units of a token group
 };
 
 struct AppendArgs {
@@ -230,104 +230,118 @@ struct AppendArgs {
   void* q_out;      // [N, Hq, D]
   void* cache[2];   // k, v: [num_blocks, Hkv, bs, D]
   const long long* slots;
-  int64_t N, groups, num_slots;
-  int w_dtype, hc, bs;
+  int64_t N, num_slots, warps;
+  int w_dtype, bs;
+  FastDiv by_bs;
 };
 
+constexpr int kAppendHeads = 2, kAppendRing = 6, kAppendBlocks = 4;
+
 template <typename E, int L>
-__global__ void __launch_bounds__(kWarps * 32) qk_norm_rope_append(AppendArgs a, Tables tb) {
-  const int per = a.s[0].chunks + a.s[1].chunks + a.s[2].chunks;
-  const int64_t task = (int64_t)blockIdx.x * kWarps + (threadIdx.x >> 5);
-  if (task >= a.groups * per) return;  // the whole warp
-  const int64_t group = task / per;
-  int chunk = (int)(task - group * per), side = 0;
-  while (chunk >= a.s[side].chunks) chunk -= a.s[side++].chunks;
+__global__ void __launch_bounds__(kWalkThreads, kAppendBlocks) qk_norm_rope_append(AppendArgs a, Tables tb) {
+  extern __shared__ __align__(16) uint4 ring[];
+  const int64_t warp = (int64_t)blockIdx.x * (kWalkThreads / 32) + (threadIdx.x >> 5);
+  const int side = warp >= a.s[2].warp0 ? 2 : warp >= a.s[1].warp0 ? 1 : 0;
   const AppendSide& sd = a.s[side];
-
-  const int64_t n = group * (32 / L) + (threadIdx.x & 31) / L;
+  const int64_t warps = (side == 2 ? a.warps : a.s[side + 1].warp0) - sd.warp0;
+  const Units un = make_units(warp - sd.warp0, warps, sd.units, sd.H, sd.C, sd.per);
+  if (un.count == 0) return;
   const Lane ln = lane_of<L>(tb);
-  int64_t slot = n < a.N ? __ldg(a.slots + n) : -1;
-  if (slot >= a.num_slots) {
-    if (ln.o1 == 0 && side == 0 && chunk == 0) atomicAdd(&g_bad_entries, 1u);
-    slot = -1;
-  }
-  const bool mapped = slot >= 0;
-  const bool on = ln.active && mapped;
-  const E* x = static_cast<const E*>(sd.x) + n * sd.xt;
-  E* y;
-  int64_t yh;
-  if (side == 0) {
-    y = static_cast<E*>(a.q_out) + n * sd.H * tb.D;
-    yh = tb.D;
-  } else {
-    const int64_t page = mapped ? slot / a.bs : 0;
-    y = static_cast<E*>(a.cache[side - 1]) + (page * sd.H * a.bs + (mapped ? slot - page * a.bs : 0)) * tb.D;
-    yh = (int64_t)a.bs * tb.D;
-  }
-  float c[8], s[8], w1[8], w2[8];
-  Lane la = ln;
-  la.active = on;
-  if (side < 2) {
-    const int64_t p = on && tb.R > 0 ? (tb.pos_bytes ? read_pos(tb.pos, tb.pos_bytes, n) : n) : 0;
-    load_angles(tb, la, p, &g_bad_entries, c, s);
-    load_weights(sd.w, a.w_dtype, la, w1, w2);
-  }
-  const int h0 = chunk * a.hc, h1 = min(sd.H, h0 + a.hc);
-  constexpr int U = 4;  // heads in flight
-  for (int h = h0; h < h1; h += U) {
-    Raw8<E> p[U], q[U];
-#pragma unroll
-    for (int u = 0; u < U; ++u) {
-      if (on && h + u < h1) {
-        p[u].load(x + (h + u) * sd.xh + ln.o1);
-        q[u].load(x + (h + u) * sd.xh + ln.o2);
-      } else {
-        p[u].zero();
-        q[u].zero();
-      }
-    }
-#pragma unroll
-    for (int u = 0; u < U; ++u) {
-      if (h + u >= h1) break;  // uniform over the warp
-      if (side < 2) norm_rope<E, L>(tb, p[u], q[u], w1, w2, c, s);
-      if (side == 0 && !mapped) p[u].zero(), q[u].zero();  // a padding token's q row is zeros
-      const bool write = side == 0 ? ln.active && n < a.N : on;
-      if (write && SA_DCHECK(h + u < sd.H && ln.o2 + 8 <= tb.D)) {
-        p[u].store(y + (h + u) * yh + ln.o1);
-        q[u].store(y + (h + u) * yh + ln.o2);
-      }
-    }
-  }
-}
-
-static int sm_count() {
-  int dev = 0, n = 148;
-  if (cudaGetDevice(&dev) != cudaSuccess || cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess) {
-    cudaGetLastError();
-    n = 148;
-  }
-  return n;
-}
-
-template <typename E>
-static int launch_append(const AppendArgs& a, const Tables& tb, cudaStream_t st) {
-  const int64_t tasks = a.groups * (a.s[0].chunks + a.s[1].chunks + a.s[2].chunks);
-  const int64_t blocks = (tasks + kWarps - 1) / kWarps;
-  if (blocks > INT32_MAX) return SA_ERR_UNSUPPORTED;
-  switch (lanes_for(tb.D)) {
-    case 1: qk_norm_rope_append<E, 1><<<(unsigned)blocks, kWarps * 32, 0, st>>>(a, tb); break;
-    case 2: qk_norm_rope_append<E, 2><<<(unsigned)blocks, kWarps * 32, 0, st>>>(a, tb); break;
-    case 4: qk_norm_rope_append<E, 4><<<(unsigned)blocks, kWarps * 32, 0, st>>>(a, tb); break;
-    case 8: qk_norm_rope_append<E, 8><<<(unsigned)blocks, kWarps * 32, 0, st>>>(a, tb); break;
-    default: qk_norm_rope_append<E, 16><<<(unsigned)blocks, kWarps * 32, 0, st>>>(a, tb); break;
-  }
-  return sa_record_cuda_error(cudaGetLastError());
+  auto token = [&](int64_t g) { return g * (32 / L) + (threadIdx.x & 31) / L; };
+  auto slot_at = [&](int64_t g) -> int64_t {
+    const int64_t n = token(g);
+    return n < a.N ? __ldg(a.slots + n) : -1;
+  };
+  auto pos_at = [&](int64_t g) -> int64_t {  // 0 for a padding token: its position says nothing
+    const int64_t n = token(g);
+    if (side == 2 || tb.R == 0 || n >= a.N) return kNoPos;
+    const int64_t p = tb.pos_bytes ? read_pos(tb.pos, tb.pos_bytes, n) : n;
+    return slot_at(g) < 0 ? 0 : p;
+  };
+  Angles<decltype(pos_at)> ang(tb, ln, &g_bad_entries, un, pos_at);
+  Cursor slot_ahead(un);  // of next_slot
+  int64_t more_slots = un.count - 1;
+  Map map;
+  E* y = nullptr;  // the row that comes next
+  int64_t yh = 0, next_slot = 0;
+  bool write = false, padding = false;
+  walk_rows<E, 1, kAppendHeads, kAppendRing>(
+      un, ln, ring,
+      [&](int64_t g) {
+        const int64_t n = token(g);
+        return Source<E, 1>{{static_cast<const E*>(sd.x) + (n < a.N ? n : 0) * sd.xt}, {sd.xh}, ln.active && n < a.N};
+      },
+      [&]() {
+        next_slot = slot_at(slot_ahead.group);
+        if (side < 2) ang.begin();
+      },
+      [&](int64_t g, int h) {
+        if (side < 2) {
+          float2 c[4], s[4], w1[4], w2[4];
+          load_weights(sd.w, a.w_dtype, ln, w1, w2);
+          ang.enter(c, s);
+          map.make(c, s, w1, w2);
+        }
+        int64_t slot = next_slot;
+        if (more_slots-- > 0) {
+          slot_ahead.next(un);
+          next_slot = slot_at(slot_ahead.group);
+        }
+        if (slot >= a.num_slots) {
+          if (side == 0 && ln.o1 == 0) atomicAdd(&g_bad_entries, 1u);
+          slot = -1;
+        }
+        const int64_t n = token(g);
+        padding = slot < 0;
+        if (side == 0) {  // a padding token's q row is zeros
+          write = ln.active && n < a.N;
+          y = static_cast<E*>(a.q_out) + n * sd.H * tb.D;
+          yh = tb.D;
+        } else {
+          write = ln.active && !padding;
+          const int64_t page = padding ? 0 : slot <= INT32_MAX ? (int64_t)a.by_bs.div((uint32_t)slot) : slot / a.bs;
+          y = static_cast<E*>(a.cache[side - 1]) + (page * sd.H * a.bs + (padding ? 0 : slot - page * a.bs)) * tb.D;
+          yh = (int64_t)a.bs * tb.D;
+        }
+        y += h * yh + ln.o1;
+      },
+      [&](Raw8<E> (&rows)[2]) {
+        if (side < 2) norm_rope<E, L>(tb, map, rows[0], rows[1]);
+        if (padding) rows[0].zero(), rows[1].zero();
+        if (write && SA_DCHECK(ln.o2 + 8 <= tb.D)) {
+          rows[0].store(y);
+          rows[1].store(y + (ln.o2 - ln.o1));
+        }
+        y += yh;
+      });
 }
 
 // Opt-in to `bytes` of dynamic shared memory (the requests' scans).
 template <typename F> static int opt_in(F* f, size_t bytes) {
   if (bytes <= 48 * 1024) return SA_OK;
   return sa_record_cuda_error(cudaFuncSetAttribute(f, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes));
+}
+
+template <typename E, int L>
+static int launch_append_l(const AppendArgs& a, const Tables& tb, cudaStream_t st) {
+  constexpr int smem = Ring<E, 1, kAppendHeads, kAppendRing>::kBytesPerThread * kWalkThreads;
+  static_assert(smem <= 56 * 1024, "four blocks an SM");
+  const int rc = opt_in(qk_norm_rope_append<E, L>, smem);
+  if (rc != SA_OK) return rc;
+  const unsigned blocks = (unsigned)(a.warps / (kWalkThreads / 32));
+  qk_norm_rope_append<E, L><<<blocks, kWalkThreads, smem, st>>>(a, tb);
+  return sa_record_cuda_error(cudaGetLastError());
+}
+
+template <typename E>
+static int launch_append(const AppendArgs& a, const Tables& tb, cudaStream_t st) {
+  switch (lanes_for(tb.D)) {
+    case 1: return launch_append_l<E, 1>(a, tb, st);
+    case 2: return launch_append_l<E, 2>(a, tb, st);
+    case 4: return launch_append_l<E, 4>(a, tb, st);
+    case 8: return launch_append_l<E, 8>(a, tb, st);
+    default: return launch_append_l<E, 16>(a, tb, st);
+  }
 }
 
 static int check_requests(int64_t B, int64_t max_blocks, int64_t bs, int64_t ld, int64_t num_free) {
@@ -430,26 +444,40 @@ extern "C" int sa_qk_norm_rope_paged_append(const void* q, const void* k, const 
     if (s[2] != 1 || s[0] % 8 != 0 || s[1] % 8 != 0) return SA_ERR_ALIGN;
   AppendArgs a;
   const int per = 32 / sa::qkr::lanes_for(D);
+  const int64_t groups = (N + per - 1) / per;
   a.N = N;
-  a.groups = (N + per - 1) / per;
   a.num_slots = num_blocks * block_size;
   a.w_dtype = w_dtype;
   a.bs = (int)block_size;
-  a.hc = sa::qkr::heads_per_warp(a.groups, Hq + 2 * Hkv, 16ll * sm_count());
+  a.by_bs = sa::qkr::FastDiv((uint32_t)block_size);
   a.q_out = q_out;
   a.cache[0] = k_cache;
   a.cache[1] = v_cache;
   a.slots = reinterpret_cast<const long long*>(slots);
   const void* xs[3] = {q, k, v};
   const void* ws[3] = {q_weight, k_weight, nullptr};
+  const int64_t heads = Hq + 2 * Hkv;
+  const int C = sa::qkr::unit_heads(groups * heads, (int64_t)kAppendBlocks * sa::qkr::sm_count() * (sa::qkr::kWalkThreads / 32),
+                                    kAppendHeads);
+  int64_t units = 0;
   for (int i = 0; i < 3; ++i) {
     a.s[i].x = xs[i];
     a.s[i].w = ws[i];
     a.s[i].xt = st3[i][0];
     a.s[i].xh = st3[i][1];
     a.s[i].H = (int)(i == 0 ? Hq : Hkv);
-    a.s[i].chunks = (a.s[i].H + a.hc - 1) / a.hc;
+    a.s[i].C = C;
+    a.s[i].per = (a.s[i].H + C - 1) / C;
+    a.s[i].units = groups * a.s[i].per;
+    units += a.s[i].units;
   }
+  // warps by each side's share of the rows, at least one where it has any (four warps a block: always enough)
+  a.warps = sa::qkr::walk_blocks(units, kAppendBlocks) * (sa::qkr::kWalkThreads / 32);
+  const int64_t q_warps = (int64_t)((double)a.warps * (double)Hq / (double)heads + 0.5);
+  const int64_t qk_warps = (int64_t)((double)a.warps * (double)(Hq + Hkv) / (double)heads + 0.5);
+  a.s[0].warp0 = 0;
+  a.s[1].warp0 = std::min<int64_t>(a.warps - 2, std::max<int64_t>(Hq > 0, q_warps));
+  a.s[2].warp0 = std::min<int64_t>(a.warps - 1, std::max<int64_t>(a.s[1].warp0 + 1, qk_warps));
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   return dtype == SA_BF16 ? launch_append<__nv_bfloat16>(a, tb, st) : launch_append<__half>(a, tb, st);
 }

@@ -348,7 +348,7 @@ template <typename E, int D>
 static int launch_means(const MeansArgs& a, int64_t B, cudaStream_t st) {
   // enough blocks for 8 an SM, each a contiguous stride of warps; a sequence without new pages leaves at once
   const int64_t most = ((int64_t)a.max_blocks * a.Hkv + 7) / 8;
-  const int64_t x = std::max<int64_t>(1, std::min(most, (148 * 16 + B - 1) / B));
+  const int64_t x = std::max<int64_t>(1, std::min<int64_t>(most, (16ll * qkr::sm_count() + B - 1) / B));
   paged_key_means_kernel<E, D><<<dim3((unsigned)x, (unsigned)B), 256, 0, st>>>(a);
   return sa_record_cuda_error(cudaGetLastError());
 }

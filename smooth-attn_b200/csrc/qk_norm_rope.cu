@@ -14,12 +14,14 @@
 // saves nothing.
 //
 // Bound: HBM.  Forward reads x and writes y; backward reads x and dy and
-// writes dx.  A warp owns 32 / L neighbouring tokens (L lanes a row) and walks
-// over some of their heads, so a token's cos / sin stay in registers for all
-// of them.  dw: every lane keeps fp32 sums of its own 16 channels over the
-// rows it meets, a block adds its warps' sums in a fixed order and writes one
-// row of partial sums, and a second small kernel adds those in a fixed order:
-// no atomics, bitwise the same from run to run.
+// writes dx.  A warp owns a contiguous range of (token group, heads) items of
+// q or of k and streams their rows through shared memory (walk_rows): a
+// token's cos / sin stay in registers for its heads, and all warps' ranges are
+// equally long, so nothing is left over at the end.  dw: every lane keeps fp32
+// sums of its own 16 channels over the rows it meets, a block adds its warps'
+// sums in a fixed order and writes one row of partial sums for each of q and
+// k, and a second small kernel adds those in a fixed order: no atomics,
+// bitwise the same from run to run.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
@@ -37,21 +39,21 @@ namespace qkr {
 
 static __device__ unsigned g_bad_positions;
 
-constexpr int kWarps = 8;
-
 struct Side {
   const void* x;
   void* y;          // forward: y; backward: dx
   const void* dy;   // backward
   const void* w;    // nullable
   int64_t xb, xh, xt, yb, yh, yt, gb, gh, gt;  // element strides
-  int H, hc, chunks;  // heads, heads a warp takes, ceil(H / hc)
+  int64_t units;    // groups * per
+  int H, C, per;    // heads, heads of a unit, units of a token group
 };
 
 struct Shape {
   int64_t N, T;     // B * T tokens
-  int64_t groups;   // of 32 / L tokens
+  int64_t q_warps;  // warps that walk over q; the others walk over k
   int w_dtype;
+  FastDiv by_T;     // where N < 2^31
 };
 
 struct Token {
@@ -64,177 +66,192 @@ __device__ __forceinline__ Token token_of(const Shape& sh, int64_t group) {
   const int64_t n = group * (32 / L) + (threadIdx.x & 31) / L;
   Token k;
   k.valid = n < sh.N;
-  k.b = k.valid ? n / sh.T : 0;
+  k.b = !k.valid ? 0 : sh.N <= INT32_MAX ? (int64_t)sh.by_T.div((uint32_t)n) : n / sh.T;
   k.t = k.valid ? n - k.b * sh.T : 0;
   return k;
 }
 
 __device__ __forceinline__ int64_t pos_of(const Tables& tb, const Token& k) {
+  if (!k.valid || tb.R == 0) return kNoPos;
   return tb.pos_bytes ? read_pos(tb.pos, tb.pos_bytes, k.b * tb.pos_sb + k.t) : k.t;
 }
+
+// A warp's units of q or of k.
+struct Part {
+  bool is_q;
+  Units un;
+};
+__device__ __forceinline__ Part part_of_warp(const Side& q, const Side& k, const Shape& sh) {
+  const int64_t warp = (int64_t)blockIdx.x * (kWalkThreads / 32) + (threadIdx.x >> 5);
+  const int64_t all = (int64_t)gridDim.x * (kWalkThreads / 32);
+  Part p;
+  p.is_q = warp < sh.q_warps;
+  const Side& sd = p.is_q ? q : k;
+  p.un = make_units(p.is_q ? warp : warp - sh.q_warps, p.is_q ? sh.q_warps : all - sh.q_warps, sd.units, sd.H, sd.C,
+                    sd.per);
+  return p;
+}
+
+// Heads an item, depth of the ring and resident blocks an SM: four forward
+// blocks of 49 KB and 128 registers a thread, three backward blocks of at most
+// 65 KB and 168 registers (at 128 the backward spills).
+template <typename E> constexpr int kFwdHeads = sizeof(E) == 4 ? 1 : 2;
+constexpr int kBwdHeads = 1;
+constexpr int kFwdRing = 6;
+template <typename E> constexpr int kBwdRing = sizeof(E) == 4 ? 4 : 6;
+constexpr int kFwdBlocks = 4, kBwdBlocks = 3;
 
 // ---- forward ----------------------------------------------------------------
 
 template <typename E, int L>
-__global__ void __launch_bounds__(kWarps * 32) qk_norm_rope_fwd(Side q, Side k, Tables tb, Shape sh) {
-  const int per = q.chunks + k.chunks;
-  const int64_t task = (int64_t)blockIdx.x * kWarps + (threadIdx.x >> 5);
-  if (task >= sh.groups * per) return;  // the whole warp
-  const int64_t group = task / per;
-  int chunk = (int)(task - group * per);
-  const bool is_q = chunk < q.chunks;
-  const Side& sd = is_q ? q : k;
-  if (!is_q) chunk -= q.chunks;
-
+__global__ void __launch_bounds__(kWalkThreads, kFwdBlocks)
+    qk_norm_rope_fwd(Side q, Side k, Tables tb, Shape sh) {
+  extern __shared__ __align__(16) uint4 ring[];
+  const Part part = part_of_warp(q, k, sh);
+  if (part.un.count == 0) return;
+  const Side& sd = part.is_q ? q : k;
   const Lane ln = lane_of<L>(tb);
-  const Token tk = token_of<L>(sh, group);
-  const bool on = ln.active && tk.valid;
-  float c[8], s[8], w1[8], w2[8];
-  Lane la = ln;
-  la.active = on;
-  load_angles(tb, la, pos_of(tb, tk), &g_bad_positions, c, s);
-  load_weights(sd.w, sh.w_dtype, la, w1, w2);
-  const E* x = static_cast<const E*>(sd.x) + tk.b * sd.xb + tk.t * sd.xt;
-  E* y = static_cast<E*>(sd.y) + tk.b * sd.yb + tk.t * sd.yt;
-  const int h0 = chunk * sd.hc, h1 = min(sd.H, h0 + sd.hc);
-  constexpr int U = 4;  // heads in flight
-  for (int h = h0; h < h1; h += U) {
-    Raw8<E> a[U], b[U];
-#pragma unroll
-    for (int u = 0; u < U; ++u) {
-      if (on && h + u < h1) {
-        a[u].load(x + (h + u) * sd.xh + ln.o1);
-        b[u].load(x + (h + u) * sd.xh + ln.o2);
-      } else {
-        a[u].zero();
-        b[u].zero();
-      }
-    }
-#pragma unroll
-    for (int u = 0; u < U; ++u) {
-      if (h + u >= h1) break;  // uniform over the warp
-      norm_rope<E, L>(tb, a[u], b[u], w1, w2, c, s);
-      if (on && SA_DCHECK(tk.t < sh.T && h + u < sd.H && ln.o2 + 8 <= tb.D)) {
-        a[u].store(y + (h + u) * sd.yh + ln.o1);
-        b[u].store(y + (h + u) * sd.yh + ln.o2);
-      }
-    }
-  }
+  auto pos_at = [&](int64_t g) { return pos_of(tb, token_of<L>(sh, g)); };
+  Angles<decltype(pos_at)> ang(tb, ln, &g_bad_positions, part.un, pos_at);
+  Map map;
+  E* y = nullptr;  // the row that comes next
+  bool on = false;
+  walk_rows<E, 1, kFwdHeads<E>, kFwdRing>(
+      part.un, ln, ring,
+      [&](int64_t g) {
+        const Token tk = token_of<L>(sh, g);
+        return Source<E, 1>{{static_cast<const E*>(sd.x) + tk.b * sd.xb + tk.t * sd.xt}, {sd.xh},
+                            ln.active && tk.valid};
+      },
+      [&]() { ang.begin(); },
+      [&](int64_t g, int h) {
+        float2 c[4], s[4], w1[4], w2[4];
+        load_weights(sd.w, sh.w_dtype, ln, w1, w2);
+        ang.enter(c, s);
+        map.make(c, s, w1, w2);
+        const Token tk = token_of<L>(sh, g);
+        on = ln.active && tk.valid;
+        y = static_cast<E*>(sd.y) + tk.b * sd.yb + tk.t * sd.yt + h * sd.yh + ln.o1;
+      },
+      [&](Raw8<E> (&rows)[2]) {
+        norm_rope<E, L>(tb, map, rows[0], rows[1]);
+        if (on && SA_DCHECK(ln.o2 + 8 <= tb.D)) {
+          rows[0].store(y);
+          rows[1].store(y + (ln.o2 - ln.o1));
+        }
+        y += sd.yh;
+      });
 }
 
 // ---- backward ---------------------------------------------------------------
 
-// Blocks [0, q_blocks) walk over q's tasks, the others over k's, so a lane
-// keeps one set of dw sums.  part: [gridDim.x][D] fp32, or null without dw.
+// part_sums: [2][gridDim.x][D] fp32 (q's rows, then k's), or null without dw.
 template <typename E, int L>
-__global__ void __launch_bounds__(kWarps * 32, 2)
-    qk_norm_rope_bwd(Side q, Side k, Tables tb, Shape sh, float* part, int q_blocks) {
-  extern __shared__ float red[];  // [kWarps][D]
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const bool is_q = (int)blockIdx.x < q_blocks;
-  const Side& sd = is_q ? q : k;
-  const int64_t first = (int64_t)(is_q ? blockIdx.x : blockIdx.x - q_blocks) * kWarps + warp;
-  const int64_t step = (int64_t)(is_q ? q_blocks : gridDim.x - q_blocks) * kWarps;
+__global__ void __launch_bounds__(kWalkThreads, kBwdBlocks)
+    qk_norm_rope_bwd(Side q, Side k, Tables tb, Shape sh, float* part_sums) {
+  extern __shared__ __align__(16) uint4 ring[];
+  const Part part = part_of_warp(q, k, sh);
+  const Side& sd = part.is_q ? q : k;
   const Lane ln = lane_of<L>(tb);
-  float w1[8], w2[8], dw1[8], dw2[8];
+  auto pos_at = [&](int64_t g) { return pos_of(tb, token_of<L>(sh, g)); };
+  Angles<decltype(pos_at)> ang(tb, ln, &g_bad_positions, part.un, pos_at);
+  float2 c[4], s[4], w1[4], w2[4], dw1[4], dw2[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) dw1[i] = dw2[i] = splat(0.f);
   load_weights(sd.w, sh.w_dtype, ln, w1, w2);
+  E* dx = nullptr;  // the row that comes next
+  bool on = false;
+  walk_rows<E, 2, kBwdHeads, kBwdRing<E>>(
+      part.un, ln, ring,
+      [&](int64_t g) {
+        const Token tk = token_of<L>(sh, g);
+        return Source<E, 2>{{static_cast<const E*>(sd.x) + tk.b * sd.xb + tk.t * sd.xt,
+                             static_cast<const E*>(sd.dy) + tk.b * sd.gb + tk.t * sd.gt},
+                            {sd.xh, sd.gh},
+                            ln.active && tk.valid};
+      },
+      [&]() { ang.begin(); },
+      [&](int64_t g, int h) {
+        ang.enter(c, s);
+        const Token tk = token_of<L>(sh, g);
+        on = ln.active && tk.valid;
+        dx = static_cast<E*>(sd.y) + tk.b * sd.yb + tk.t * sd.yt + h * sd.yh + ln.o1;
+      },
+      [&](Raw8<E> (&rows)[4]) {
+        float2 x1[4], x2[4], g1[4], g2[4];  // g becomes dn
+        rows[0].get(x1);
+        rows[1].get(x2);
+        rows[2].get(g1);
+        rows[3].get(g2);
 #pragma unroll
-  for (int i = 0; i < 8; ++i) dw1[i] = dw2[i] = 0.f;
-
-  const int64_t tasks = sh.groups * sd.chunks;
-  for (int64_t task = first; task < tasks; task += step) {
-    const int64_t group = task / sd.chunks;
-    const int chunk = (int)(task - group * sd.chunks);
-    const Token tk = token_of<L>(sh, group);
-    const bool on = ln.active && tk.valid;
-    float c[8], s[8];
-    Lane la = ln;
-    la.active = on;
-    load_angles(tb, la, pos_of(tb, tk), &g_bad_positions, c, s);
-    const E* x = static_cast<const E*>(sd.x) + tk.b * sd.xb + tk.t * sd.xt;
-    const E* dy = static_cast<const E*>(sd.dy) + tk.b * sd.gb + tk.t * sd.gt;
-    E* dx = static_cast<E*>(sd.y) + tk.b * sd.yb + tk.t * sd.yt;
-    const int h0 = chunk * sd.hc, h1 = min(sd.H, h0 + sd.hc);
-    constexpr int U = sizeof(E) == 4 ? 1 : 2;
-    for (int h = h0; h < h1; h += U) {
-      Raw8<E> xa[U], xb[U], ga[U], gb[U];
-#pragma unroll
-      for (int u = 0; u < U; ++u) {
-        if (on && h + u < h1) {
-          xa[u].load(x + (h + u) * sd.xh + ln.o1);
-          xb[u].load(x + (h + u) * sd.xh + ln.o2);
-          ga[u].load(dy + (h + u) * sd.gh + ln.o1);
-          gb[u].load(dy + (h + u) * sd.gh + ln.o2);
-        } else {
-          xa[u].zero(), xb[u].zero(), ga[u].zero(), gb[u].zero();
-        }
-      }
-#pragma unroll
-      for (int u = 0; u < U; ++u) {
-        if (h + u >= h1) break;  // uniform over the warp
-        float x1[8], x2[8], g1[8], g2[8];
-        xa[u].get(x1);
-        xb[u].get(x2);
-        ga[u].get(g1);
-        gb[u].get(g2);
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          const float n1 = g1[i] * c[i] + g2[i] * s[i], n2 = g2[i] * c[i] - g1[i] * s[i];
-          g1[i] = n1, g2[i] = n2;
+        for (int i = 0; i < 4; ++i) {
+          const float2 n1 = ffma2(g1[i], c[i], fmul2(g2[i], s[i]));
+          g2[i] = fsub2(fmul2(g2[i], c[i]), fmul2(g1[i], s[i]));
+          g1[i] = n1;
         }
         if (tb.normalize) {
-          float ss = 0.f, gx = 0.f;
+          float2 ss = fmul2(x1[0], x1[0]), gx = splat(0.f), v1[4], v2[4];  // v: dn w
 #pragma unroll
-          for (int i = 0; i < 8; ++i) {
-            ss = fmaf(x1[i], x1[i], ss);
-            ss = fmaf(x2[i], x2[i], ss);
-            gx = fmaf(g1[i] * w1[i], x1[i], gx);
-            gx = fmaf(g2[i] * w2[i], x2[i], gx);
+          for (int i = 0; i < 4; ++i) {
+            if (i) ss = ffma2(x1[i], x1[i], ss);
+            ss = ffma2(x2[i], x2[i], ss);
+            v1[i] = fmul2(g1[i], w1[i]);
+            v2[i] = fmul2(g2[i], w2[i]);
+            gx = ffma2(v1[i], x1[i], gx);
+            gx = ffma2(v2[i], x2[i], gx);
           }
-          ss = row_sum<L>(ss);
-          gx = row_sum<L>(gx);
-          const float r = rsqrtf(fmaf(ss, tb.inv_d, tb.eps));
-          const float m = gx * tb.inv_d * r * r;
+          const float sum = row_sum<L>(ss.x + ss.y), dot = row_sum<L>(gx.x + gx.y);
+          const float r = rsqrtf(fmaf(sum, tb.inv_d, tb.eps));
+          const float2 r2 = splat(r), m2 = splat(-(dot * tb.inv_d) * r * r * r);
 #pragma unroll
-          for (int i = 0; i < 8; ++i) {
-            dw1[i] = fmaf(g1[i], x1[i] * r, dw1[i]);
-            dw2[i] = fmaf(g2[i], x2[i] * r, dw2[i]);
-            g1[i] = r * (g1[i] * w1[i] - x1[i] * m);
-            g2[i] = r * (g2[i] * w2[i] - x2[i] * m);
+          for (int i = 0; i < 4; ++i) {
+            dw1[i] = ffma2(g1[i], fmul2(x1[i], r2), dw1[i]);
+            dw2[i] = ffma2(g2[i], fmul2(x2[i], r2), dw2[i]);
+            g1[i] = ffma2(x1[i], m2, fmul2(v1[i], r2));
+            g2[i] = ffma2(x2[i], m2, fmul2(v2[i], r2));
           }
         }
-        if (on && SA_DCHECK(tk.t < sh.T && h + u < sd.H && ln.o2 + 8 <= tb.D)) {
-          ga[u].set(g1);
-          gb[u].set(g2);
-          ga[u].store(dx + (h + u) * sd.yh + ln.o1);
-          gb[u].store(dx + (h + u) * sd.yh + ln.o2);
+        if (on && SA_DCHECK(ln.o2 + 8 <= tb.D)) {
+          rows[2].set(g1);
+          rows[3].set(g2);
+          rows[2].store(dx);
+          rows[3].store(dx + (ln.o2 - ln.o1));
         }
-      }
-    }
-  }
-  if (part == nullptr) return;
-  // lanes that hold the same channels (one per token of the warp), then warps
+        dx += sd.yh;
+      });
+  if (part_sums == nullptr) return;
+  // lanes that hold the same channels (one per token of the group), then the block's warps of one side
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
+  for (int i = 0; i < 4; ++i) {
 #pragma unroll
     for (int m = L; m < 32; m <<= 1) {
-      dw1[i] += __shfl_xor_sync(0xffffffffu, dw1[i], m);
-      dw2[i] += __shfl_xor_sync(0xffffffffu, dw2[i], m);
+      dw1[i].x += __shfl_xor_sync(0xffffffffu, dw1[i].x, m);
+      dw1[i].y += __shfl_xor_sync(0xffffffffu, dw1[i].y, m);
+      dw2[i].x += __shfl_xor_sync(0xffffffffu, dw2[i].x, m);
+      dw2[i].y += __shfl_xor_sync(0xffffffffu, dw2[i].y, m);
     }
   }
+  constexpr int W = kWalkThreads / 32;
+  float* red = reinterpret_cast<float*>(ring);  // [W][D]; every warp's copies have landed and been read
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  __syncthreads();
   if (lane < L && ln.active) {
+    float2* to1 = reinterpret_cast<float2*>(red + warp * tb.D + ln.o1);
+    float2* to2 = reinterpret_cast<float2*>(red + warp * tb.D + ln.o2);
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      red[warp * tb.D + ln.o1 + i] = dw1[i];
-      red[warp * tb.D + ln.o2 + i] = dw2[i];
-    }
+    for (int i = 0; i < 4; ++i) to1[i] = dw1[i], to2[i] = dw2[i];
   }
   __syncthreads();
-  for (int d = threadIdx.x; d < tb.D; d += kWarps * 32) {
-    float v = 0.f;
+  const int64_t w0 = (int64_t)blockIdx.x * W;
+  for (int d = threadIdx.x; d < tb.D; d += kWalkThreads) {
+    float vq = 0.f, vk = 0.f;
 #pragma unroll
-    for (int wi = 0; wi < kWarps; ++wi) v += red[wi * tb.D + d];
-    part[(int64_t)blockIdx.x * tb.D + d] = v;
+    for (int w = 0; w < W; ++w) {
+      if (w0 + w < sh.q_warps) vq += red[w * tb.D + d];
+      else vk += red[w * tb.D + d];
+    }
+    part_sums[(int64_t)blockIdx.x * tb.D + d] = vq;
+    part_sums[((int64_t)gridDim.x + blockIdx.x) * tb.D + d] = vk;
   }
 }
 
@@ -249,17 +266,18 @@ __device__ __forceinline__ void store_any(void* p, int at, int dtype, float v) {
 
 // Adds the blocks' partial rows: one block per 32 channels of one side, 32
 // threads along the rows, joined in a fixed order.
-__global__ void __launch_bounds__(1024) qk_dw_sum(const float* part, void* dwq, void* dwk, int w_dtype, int D,
-                                                  int q_blocks, int blocks) {
+__global__ void __launch_bounds__(1024) qk_dw_sum(const float* part_sums, void* dwq, void* dwk, int w_dtype, int D,
+                                                  int blocks) {
   __shared__ float red[32][33];
-  const bool is_q = blockIdx.y == 0;
-  void* out = is_q ? dwq : dwk;
+  void* out = blockIdx.y == 0 ? dwq : dwk;
   if (out == nullptr) return;
+  const float* part = part_sums + (int64_t)blockIdx.y * blocks * D;
   const int col = threadIdx.x & 31, row = threadIdx.x >> 5, d = blockIdx.x * 32 + col;
-  const int lo = is_q ? 0 : q_blocks, hi = is_q ? q_blocks : blocks;
   float v = 0.f;
-  if (d < D)
-    for (int r = lo + row; r < hi; r += 32) v += part[(int64_t)r * D + d];
+  if (d < D) {
+#pragma unroll 8
+    for (int r = row; r < blocks; r += 32) v += __ldg(part + (int64_t)r * D + d);
+  }
   red[row][col] = v;
   __syncthreads();
   // transposed: warp `row` now sums column `row` over its 32 lanes
@@ -271,15 +289,6 @@ __global__ void __launch_bounds__(1024) qk_dw_sum(const float* part, void* dwq, 
 }
 
 // ---- host side ----------------------------------------------------------------
-
-static int sm_count() {
-  int dev = 0, n = 148;
-  if (cudaGetDevice(&dev) != cudaSuccess || cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess) {
-    cudaGetLastError();
-    n = 148;
-  }
-  return n;
-}
 
 static int check_rows(const void* p, const int64_t* s, int esize) {
   if (!p || !s) return SA_ERR_ARG;
@@ -298,67 +307,83 @@ static int check_shape(int64_t B, int64_t Hq, int64_t Hkv, int64_t T, int64_t D,
 }
 
 static Side side_of(const void* x, void* y, const void* dy, const void* w, int64_t H, const int64_t* xs,
-                    const int64_t* ys, const int64_t* gs, int hc) {
-  Side s;
+                    const int64_t* ys, const int64_t* gs, int64_t groups, int C) {
+  Side s{};
   s.x = x, s.y = y, s.dy = dy, s.w = w;
+  s.H = (int)H, s.C = C, s.per = (int)((H + C - 1) / C);
+  s.units = groups * s.per;
+  if (H == 0) return s;
   s.xb = xs[0], s.xh = xs[1], s.xt = xs[2];
   s.yb = ys[0], s.yh = ys[1], s.yt = ys[2];
-  s.gb = gs ? gs[0] : 0, s.gh = gs ? gs[1] : 0, s.gt = gs ? gs[2] : 0;
-  s.H = (int)H, s.hc = hc, s.chunks = (int)((H + hc - 1) / hc);
+  if (gs) s.gb = gs[0], s.gh = gs[1], s.gt = gs[2];
   return s;
 }
 
-static Shape shape_of(int64_t B, int64_t T, int64_t D, int w_dtype) {
-  Shape sh;
-  sh.N = B * T, sh.T = T, sh.w_dtype = w_dtype;
-  const int per = 32 / lanes_for(D);
-  sh.groups = (sh.N + per - 1) / per;
-  return sh;
+static int64_t groups_of(int64_t N, int64_t D) {
+  const int64_t per = 32 / lanes_for(D);
+  return (N + per - 1) / per;
 }
 
-template <typename E>
-static int launch_fwd(const Side& q, const Side& k, const Tables& tb, const Shape& sh, cudaStream_t st) {
-  const int64_t tasks = sh.groups * (q.chunks + k.chunks), blocks = (tasks + kWarps - 1) / kWarps;
-  if (blocks > INT32_MAX) return SA_ERR_UNSUPPORTED;
-  switch (lanes_for(tb.D)) {
-    case 1: qk_norm_rope_fwd<E, 1><<<(unsigned)blocks, kWarps * 32, 0, st>>>(q, k, tb, sh); break;
-    case 2: qk_norm_rope_fwd<E, 2><<<(unsigned)blocks, kWarps * 32, 0, st>>>(q, k, tb, sh); break;
-    case 4: qk_norm_rope_fwd<E, 4><<<(unsigned)blocks, kWarps * 32, 0, st>>>(q, k, tb, sh); break;
-    case 8: qk_norm_rope_fwd<E, 8><<<(unsigned)blocks, kWarps * 32, 0, st>>>(q, k, tb, sh); break;
-    default: qk_norm_rope_fwd<E, 16><<<(unsigned)blocks, kWarps * 32, 0, st>>>(q, k, tb, sh); break;
-  }
+// Blocks, and the warps of q by its share of the rows: at least one for each side that has any.
+static int64_t plan(const Side& q, const Side& k, Shape* sh, int per_sm) {
+  const int64_t blocks = walk_blocks(q.units + k.units, per_sm), warps = blocks * (kWalkThreads / 32);
+  if (blocks == 0) return 0;
+  sh->q_warps = (int64_t)((double)warps * (double)q.H / (double)(q.H + k.H) + 0.5);
+  if (q.units) sh->q_warps = std::max<int64_t>(1, sh->q_warps);
+  if (k.units) sh->q_warps = std::min(sh->q_warps, warps - 1);  // (four warps a block: one is left)
+  return blocks;
+}
+
+template <typename F> static int opt_in(F* f, int bytes) {
+  if (bytes <= 48 * 1024) return SA_OK;
+  return sa_record_cuda_error(cudaFuncSetAttribute(f, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes));
+}
+
+template <typename E, int L>
+static int launch_fwd_l(const Side& q, const Side& k, const Tables& tb, const Shape& sh, int64_t blocks,
+                        cudaStream_t st) {
+  constexpr int smem = Ring<E, 1, kFwdHeads<E>, kFwdRing>::kBytesPerThread * kWalkThreads;
+  static_assert(smem <= 56 * 1024, "four blocks an SM");
+  const int rc = opt_in(qk_norm_rope_fwd<E, L>, smem);
+  if (rc != SA_OK) return rc;
+  qk_norm_rope_fwd<E, L><<<(unsigned)blocks, kWalkThreads, smem, st>>>(q, k, tb, sh);
   return sa_record_cuda_error(cudaGetLastError());
 }
 
-struct BwdPlan {
-  int64_t blocks, q_blocks;
-};
-
-// Two resident blocks an SM, split between q and k by their heads.
-static BwdPlan plan_bwd(int64_t tasks_q, int64_t tasks_k, int64_t Hq, int64_t Hkv) {
-  const int64_t most = 2ll * sm_count();
-  const int64_t need_q = (tasks_q + kWarps - 1) / kWarps, need_k = (tasks_k + kWarps - 1) / kWarps;
-  BwdPlan p;
-  const int64_t share = std::max<int64_t>(1, std::min<int64_t>(most - 1, (most * Hq + (Hq + Hkv) / 2) / std::max<int64_t>(1, Hq + Hkv)));
-  p.q_blocks = std::min(need_q, share);
-  p.blocks = p.q_blocks + std::min(need_k, most - share);
-  return p;
-}
-
 template <typename E>
-static int launch_bwd(const Side& q, const Side& k, const Tables& tb, const Shape& sh, float* part, const BwdPlan& p,
+static int launch_fwd(const Side& q, const Side& k, const Tables& tb, const Shape& sh, int64_t blocks,
                       cudaStream_t st) {
-  const size_t smem = part ? (size_t)kWarps * tb.D * 4 : 0;  // at most 8 KB
-  const unsigned g = (unsigned)p.blocks;
-  const int qb = (int)p.q_blocks;
   switch (lanes_for(tb.D)) {
-    case 1: qk_norm_rope_bwd<E, 1><<<g, kWarps * 32, smem, st>>>(q, k, tb, sh, part, qb); break;
-    case 2: qk_norm_rope_bwd<E, 2><<<g, kWarps * 32, smem, st>>>(q, k, tb, sh, part, qb); break;
-    case 4: qk_norm_rope_bwd<E, 4><<<g, kWarps * 32, smem, st>>>(q, k, tb, sh, part, qb); break;
-    case 8: qk_norm_rope_bwd<E, 8><<<g, kWarps * 32, smem, st>>>(q, k, tb, sh, part, qb); break;
-    default: qk_norm_rope_bwd<E, 16><<<g, kWarps * 32, smem, st>>>(q, k, tb, sh, part, qb); break;
+    case 1: return launch_fwd_l<E, 1>(q, k, tb, sh, blocks, st);
+    case 2: return launch_fwd_l<E, 2>(q, k, tb, sh, blocks, st);
+    case 4: return launch_fwd_l<E, 4>(q, k, tb, sh, blocks, st);
+    case 8: return launch_fwd_l<E, 8>(q, k, tb, sh, blocks, st);
+    default: return launch_fwd_l<E, 16>(q, k, tb, sh, blocks, st);
   }
+}
+
+template <typename E, int L>
+static int launch_bwd_l(const Side& q, const Side& k, const Tables& tb, const Shape& sh, float* part, int64_t blocks,
+                        cudaStream_t st) {
+  constexpr int smem = Ring<E, 2, kBwdHeads, kBwdRing<E>>::kBytesPerThread * kWalkThreads;
+  static_assert(smem >= kWalkThreads / 32 * 256 * 4, "the block's dw sums");
+  static_assert(smem <= 74 * 1024, "three blocks an SM");
+  const int rc = opt_in(qk_norm_rope_bwd<E, L>, smem);
+  if (rc != SA_OK) return rc;
+  qk_norm_rope_bwd<E, L><<<(unsigned)blocks, kWalkThreads, smem, st>>>(q, k, tb, sh, part);
   return sa_record_cuda_error(cudaGetLastError());
+}
+
+template <typename E>
+static int launch_bwd(const Side& q, const Side& k, const Tables& tb, const Shape& sh, float* part, int64_t blocks,
+                      cudaStream_t st) {
+  switch (lanes_for(tb.D)) {
+    case 1: return launch_bwd_l<E, 1>(q, k, tb, sh, part, blocks, st);
+    case 2: return launch_bwd_l<E, 2>(q, k, tb, sh, part, blocks, st);
+    case 4: return launch_bwd_l<E, 4>(q, k, tb, sh, part, blocks, st);
+    case 8: return launch_bwd_l<E, 8>(q, k, tb, sh, part, blocks, st);
+    default: return launch_bwd_l<E, 16>(q, k, tb, sh, part, blocks, st);
+  }
 }
 
 }  // namespace qkr
@@ -393,24 +418,26 @@ extern "C" int sa_qk_norm_rope(const void* q, const void* k, void* q_out, void* 
   if (rc != SA_OK) return rc;
   if (B == 0 || T == 0 || Hq + Hkv == 0) return SA_OK;
   const int es = dtype == SA_F32 ? 4 : 2;
-  const int64_t none[4] = {0, 0, 0, 1};
   if (Hq > 0 && ((rc = check_rows(q, q_strides, es)) != SA_OK || (rc = check_rows(q_out, qo_strides, es)) != SA_OK))
     return rc;
   if (Hkv > 0 && ((rc = check_rows(k, k_strides, es)) != SA_OK || (rc = check_rows(k_out, ko_strides, es)) != SA_OK))
     return rc;
-  const Shape sh = shape_of(B, T, D, w_dtype);
-  const int hc = heads_per_warp(sh.groups, Hq + Hkv, 16ll * sm_count());
-  const Side a = side_of(q, q_out, nullptr, q_weight, Hq, Hq ? q_strides : none, Hq ? qo_strides : none, nullptr, hc);
-  const Side b = side_of(k, k_out, nullptr, k_weight, Hkv, Hkv ? k_strides : none, Hkv ? ko_strides : none, nullptr, hc);
+  const int64_t groups = groups_of(B * T, D);
+  const int uh = unit_heads(groups * (Hq + Hkv), (int64_t)kFwdBlocks * sm_count() * (kWalkThreads / 32),
+                            dtype == SA_F32 ? kFwdHeads<float> : kFwdHeads<__half>);
+  const Side a = side_of(q, q_out, nullptr, q_weight, Hq, q_strides, qo_strides, nullptr, groups, uh);
+  const Side b = side_of(k, k_out, nullptr, k_weight, Hkv, k_strides, ko_strides, nullptr, groups, uh);
+  Shape sh{B * T, T, 0, w_dtype, FastDiv((uint32_t)T)};
+  const int64_t blocks = plan(a, b, &sh, kFwdBlocks);
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  if (dtype == SA_F32) return launch_fwd<float>(a, b, tb, sh, st);
-  if (dtype == SA_BF16) return launch_fwd<__nv_bfloat16>(a, b, tb, sh, st);
-  return launch_fwd<__half>(a, b, tb, sh, st);
+  if (dtype == SA_F32) return launch_fwd<float>(a, b, tb, sh, blocks, st);
+  if (dtype == SA_BF16) return launch_fwd<__nv_bfloat16>(a, b, tb, sh, blocks, st);
+  return launch_fwd<__half>(a, b, tb, sh, blocks, st);
 }
 
 extern "C" int64_t sa_qk_norm_rope_bwd_workspace_size(int64_t D) {
   if (D <= 0 || D > 256) return SA_ERR_UNSUPPORTED;
-  return 2ll * sa::qkr::sm_count() * D * 4;
+  return 2ll * sa::qkr::kBwdBlocks * sa::qkr::sm_count() * D * 4;
 }
 
 extern "C" int sa_qk_norm_rope_bwd(const void* q, const void* k, const void* dq_out, const void* dk_out, void* dq,
@@ -437,7 +464,6 @@ extern "C" int sa_qk_norm_rope_bwd(const void* q, const void* k, const void* dq_
   }
   const int es = dtype == SA_F32 ? 4 : 2;
   const bool work = B > 0 && T > 0;
-  const int64_t none[4] = {0, 0, 0, 1};
   const int64_t hq = work ? Hq : 0, hk = work ? Hkv : 0;
   if (hq > 0 && ((rc = check_rows(q, q_strides, es)) != SA_OK || (rc = check_rows(dq_out, dqo_strides, es)) != SA_OK ||
                  (rc = check_rows(dq, dq_strides, es)) != SA_OK))
@@ -445,24 +471,23 @@ extern "C" int sa_qk_norm_rope_bwd(const void* q, const void* k, const void* dq_
   if (hk > 0 && ((rc = check_rows(k, k_strides, es)) != SA_OK || (rc = check_rows(dk_out, dko_strides, es)) != SA_OK ||
                  (rc = check_rows(dk, dk_strides, es)) != SA_OK))
     return rc;
-  const Shape sh = shape_of(work ? B : 0, work ? T : 1, D, w_dtype);
-  const int hc = heads_per_warp(sh.groups, Hq + Hkv, 16ll * sm_count());
-  const Side a = side_of(q, dq, dq_out, q_weight, hq, hq ? q_strides : none, hq ? dq_strides : none,
-                         hq ? dqo_strides : none, hc);
-  const Side b = side_of(k, dk, dk_out, k_weight, hk, hk ? k_strides : none, hk ? dk_strides : none,
-                         hk ? dko_strides : none, hc);
-  const BwdPlan p = plan_bwd(sh.groups * a.chunks, sh.groups * b.chunks, hq, hk);
+  const int64_t groups = work ? groups_of(B * T, D) : 0;
+  const int uh = unit_heads(groups * (hq + hk), (int64_t)kBwdBlocks * sm_count() * (kWalkThreads / 32), kBwdHeads);
+  const Side a = side_of(q, dq, dq_out, q_weight, hq, q_strides, dq_strides, dqo_strides, groups, uh);
+  const Side b = side_of(k, dk, dk_out, k_weight, hk, k_strides, dk_strides, dko_strides, groups, uh);
+  Shape sh{B * T, work ? T : 1, 0, w_dtype, FastDiv(work ? (uint32_t)T : 1u)};
+  const int64_t blocks = plan(a, b, &sh, kBwdBlocks);
   float* part = dw ? static_cast<float*>(workspace) : nullptr;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  if (p.blocks > 0) {
-    rc = dtype == SA_F32    ? launch_bwd<float>(a, b, tb, sh, part, p, st)
-         : dtype == SA_BF16 ? launch_bwd<__nv_bfloat16>(a, b, tb, sh, part, p, st)
-                            : launch_bwd<__half>(a, b, tb, sh, part, p, st);
+  if (blocks > 0) {
+    rc = dtype == SA_F32    ? launch_bwd<float>(a, b, tb, sh, part, blocks, st)
+         : dtype == SA_BF16 ? launch_bwd<__nv_bfloat16>(a, b, tb, sh, part, blocks, st)
+                            : launch_bwd<__half>(a, b, tb, sh, part, blocks, st);
     if (rc != SA_OK) return rc;
   }
   if (dw) {  // also without rows: zeros
     qk_dw_sum<<<dim3((unsigned)((D + 31) / 32), 2), 1024, 0, st>>>(part, dq_weight, dk_weight, w_dtype, (int)D,
-                                                                   (int)p.q_blocks, (int)p.blocks);
+                                                                   (int)blocks);
     rc = sa_record_cuda_error(cudaGetLastError());
   }
   return rc;

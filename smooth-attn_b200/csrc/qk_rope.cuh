@@ -15,12 +15,16 @@
 
 #include <stdint.h>
 
+#include <atomic>
+
 #include "sa_common.cuh"
 
 namespace sa {
 namespace qkr {
 
-// 8 elements of E as they lie in memory.
+// 8 elements of E as they lie in memory, and as fp32 pairs (the arithmetic runs
+// in packed two-element instructions: with scalar ones the forward was bound by
+// issue slots at 0.75 of HBM's rate).
 template <typename E> struct Raw8 {
   uint4 u[sizeof(E) / 2];
   __device__ __forceinline__ void load(const E* p) {
@@ -32,18 +36,33 @@ template <typename E> struct Raw8 {
     for (int i = 0; i < (int)sizeof(E) / 2; ++i) u[i] = make_uint4(0, 0, 0, 0);
   }
   __device__ __forceinline__ void get(float (&f)[8]) const { unpack<E, 8>(u, f); }
-  __device__ __forceinline__ void set(const float (&f)[8]) {
+  __device__ __forceinline__ void get(float2 (&f)[4]) const {
+    float g[8];
+    unpack<E, 8>(u, g);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) f[i] = make_float2(g[2 * i], g[2 * i + 1]);
+  }
+  __device__ __forceinline__ void set(const float2 (&f)[4]) {
     if constexpr (sizeof(E) == 4) {
 #pragma unroll
       for (int i = 0; i < 2; ++i)
-        u[i] = make_uint4(__float_as_uint(f[4 * i]), __float_as_uint(f[4 * i + 1]), __float_as_uint(f[4 * i + 2]),
-                          __float_as_uint(f[4 * i + 3]));
-    } else {
-      Pack<E, 8> p;
+        u[i] = make_uint4(__float_as_uint(f[2 * i].x), __float_as_uint(f[2 * i].y), __float_as_uint(f[2 * i + 1].x),
+                          __float_as_uint(f[2 * i + 1].y));
+    } else if constexpr (std::is_same<E, __nv_bfloat16>::value) {
+      __nv_bfloat162 h[4];
 #pragma unroll
-      for (int i = 0; i < 8; ++i) p.set(i, f[i]);
-      u[0] = p.u;
+      for (int i = 0; i < 4; ++i) h[i] = __float22bfloat162_rn(f[i]);
+      u[0] = *reinterpret_cast<const uint4*>(h);
+    } else {
+      __half2 h[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) h[i] = __float22half2_rn(f[i]);
+      u[0] = *reinterpret_cast<const uint4*>(h);
     }
+  }
+  __device__ __forceinline__ void set(const float (&f)[8]) {
+    const float2 g[4] = {{f[0], f[1]}, {f[2], f[3]}, {f[4], f[5]}, {f[6], f[7]}};
+    set(g);
   }
   __device__ __forceinline__ void store(E* p) const {
 #pragma unroll
@@ -66,6 +85,13 @@ __device__ __forceinline__ void load8_any(const void* p, int64_t at, int dtype, 
     r.load(static_cast<const __half*>(p) + at);
     r.get(f);
   }
+}
+
+__device__ __forceinline__ void load8_any(const void* p, int64_t at, int dtype, float2 (&f)[4]) {
+  float g[8];
+  load8_any(p, at, dtype, g);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) f[i] = make_float2(g[2 * i], g[2 * i + 1]);
 }
 
 // What a lane owns of every row, and the tables it reads.
@@ -99,23 +125,6 @@ __device__ __forceinline__ Lane lane_of(const Tables& t) {
   return l;
 }
 
-// cos and sin of one token for this lane; a position outside the tables is
-// read as 0 and counted (the caller's counter).
-__device__ __forceinline__ void load_angles(const Tables& t, const Lane& l, int64_t p, unsigned* bad, float (&c)[8],
-                                            float (&s)[8]) {
-  if (l.active && l.rotated) {
-    if (p < 0 || p >= t.num_pos) {
-      if (l.o1 == 0) atomicAdd(bad, 1u);
-      p = 0;
-    }
-    load8_any(t.cosv, p * (t.R / 2) + l.o1, t.cs_dtype, c);
-    load8_any(t.sinv, p * (t.R / 2) + l.o1, t.cs_dtype, s);
-  } else {
-#pragma unroll
-    for (int i = 0; i < 8; ++i) c[i] = 1.f, s[i] = 0.f;
-  }
-}
-
 __device__ __forceinline__ int64_t read_pos(const void* pos, int bytes, int64_t at) {
   return bytes == 8 ? __ldg(static_cast<const long long*>(pos) + at) : (int64_t)__ldg(static_cast<const int*>(pos) + at);
 }
@@ -127,52 +136,318 @@ template <int L> __device__ __forceinline__ float row_sum(float v) {
   return v;
 }
 
-template <int L>
-__device__ __forceinline__ float row_rscale(const Tables& t, const float (&x1)[8], const float (&x2)[8]) {
-  float ss = 0.f;
+__device__ __forceinline__ float2 splat(float v) { return make_float2(v, v); }
+
+// The forward map of a token's rows for one lane's channels, the weights folded
+// into the rotation: y1 = r (x1 a1 - x2 b1), y2 = r (x2 a2 + x1 b2).
+struct Map {
+  float2 a1[4], b1[4], a2[4], b2[4];  // w1 c, -w2 s, w2 c, w1 s
+  __device__ __forceinline__ void make(const float2 (&c)[4], const float2 (&s)[4], const float2 (&w1)[4],
+                                       const float2 (&w2)[4]) {
 #pragma unroll
-  for (int i = 0; i < 8; ++i) ss = fmaf(x1[i], x1[i], ss);
-#pragma unroll
-  for (int i = 0; i < 8; ++i) ss = fmaf(x2[i], x2[i], ss);
-  return rsqrtf(fmaf(row_sum<L>(ss), t.inv_d, t.eps));
-}
+    for (int i = 0; i < 4; ++i) {
+      a1[i] = fmul2(w1[i], c[i]);
+      b1[i] = fmul2(w2[i], make_float2(-s[i].x, -s[i].y));
+      a2[i] = fmul2(w2[i], c[i]);
+      b2[i] = fmul2(w1[i], s[i]);
+    }
+  }
+};
 
 // y of one row from its two raw chunks (zeros in lanes without one).
 template <typename E, int L>
-__device__ __forceinline__ void norm_rope(const Tables& t, Raw8<E>& a, Raw8<E>& b, const float (&w1)[8],
-                                          const float (&w2)[8], const float (&c)[8], const float (&s)[8]) {
-  float x1[8], x2[8];
+__device__ __forceinline__ void norm_rope(const Tables& t, const Map& m, Raw8<E>& a, Raw8<E>& b) {
+  float2 x1[4], x2[4], y1[4], y2[4];
   a.get(x1);
   b.get(x2);
-  if (t.normalize) {
-    const float r = row_rscale<L>(t, x1, x2);
 #pragma unroll
-    for (int i = 0; i < 8; ++i) x1[i] = x1[i] * r * w1[i], x2[i] = x2[i] * r * w2[i];
+  for (int i = 0; i < 4; ++i) {
+    y1[i] = ffma2(x1[i], m.a1[i], fmul2(x2[i], m.b1[i]));
+    y2[i] = ffma2(x2[i], m.a2[i], fmul2(x1[i], m.b2[i]));
   }
-  float y1[8], y2[8];
+  if (t.normalize) {
+    float2 ss = fmul2(x1[0], x1[0]);
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    y1[i] = x1[i] * c[i] - x2[i] * s[i];
-    y2[i] = x2[i] * c[i] + x1[i] * s[i];
+    for (int i = 1; i < 4; ++i) ss = ffma2(x1[i], x1[i], ss);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) ss = ffma2(x2[i], x2[i], ss);
+    const float2 r = splat(rsqrtf(fmaf(row_sum<L>(ss.x + ss.y), t.inv_d, t.eps)));
+#pragma unroll
+    for (int i = 0; i < 4; ++i) y1[i] = fmul2(y1[i], r), y2[i] = fmul2(y2[i], r);
   }
   a.set(y1);
   b.set(y2);
 }
 
-__device__ __forceinline__ void load_weights(const void* w, int w_dtype, const Lane& l, float (&w1)[8],
-                                             float (&w2)[8]) {
+__device__ __forceinline__ void load_weights(const void* w, int w_dtype, const Lane& l, float2 (&w1)[4],
+                                             float2 (&w2)[4]) {
   if (w != nullptr && l.active) {
     load8_any(w, l.o1, w_dtype, w1);
     load8_any(w, l.o2, w_dtype, w2);
   } else {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) w1[i] = w2[i] = 1.f;
+    for (int i = 0; i < 4; ++i) w1[i] = w2[i] = splat(1.f);
   }
 }
+
+// ---- the walk over rows ----------------------------------------------------------
+
+// The rows are cut into units: a token group (32 / L neighbouring tokens, one
+// row per L lanes) and C neighbouring heads.  Warp w of W takes units w, w + W,
+// ..., so what all warps read and write at a time lies close together.  Inside a
+// unit an item is UH heads.  Every lane streams its own 16-byte chunks of the rows
+// through a private ring in shared memory with cp.async, RING - 1 items ahead:
+// the bytes in flight then cost no registers (with plain loads 128 registers a
+// thread held only one item's), and since a lane reads only what it copied
+// itself there is no barrier, only its own wait.
+// (A plain contiguous range per warp ran the backward at 0.77 of HBM's rate, these
+// interleaved units at 0.92: the pages of memory in use at a time are few.)
+struct Units {
+  int64_t step_group;  // step = step_group * per + step_part
+  int64_t group0;      // this warp's first unit
+  int64_t count;       // and how many it has
+  int part0, step_part;
+  int H, C, per;       // heads, heads of a unit, units of a group
+};
+
+__device__ __forceinline__ Units make_units(int64_t first, int64_t step, int64_t all, int H, int C, int per) {
+  Units u;
+  u.count = first < all ? (all - first - 1) / step + 1 : 0;
+  u.group0 = first / per;
+  u.part0 = (int)(first - u.group0 * per);
+  u.step_group = step / per;
+  u.step_part = (int)(step - u.step_group * per);
+  u.H = H, u.C = C, u.per = per;
+  return u;
+}
+
+// A place in a warp's units (no division on the way).
+struct Cursor {
+  int64_t group;
+  int part;
+  __device__ __forceinline__ explicit Cursor(const Units& u) : group(u.group0), part(u.part0) {}
+  __device__ __forceinline__ void next(const Units& u) {
+    group += u.step_group;
+    part += u.step_part;
+    if (part >= u.per) part -= u.per, ++group;
+  }
+};
+
+constexpr int kWalkThreads = 128;
+
+template <typename E, int NSRC> struct Source {
+  const E* base[NSRC];  // the lane's token, head 0
+  int64_t hs[NSRC];     // head strides
+  bool on;              // the lane has a chunk of an existing token
+};
+
+template <typename E, int NSRC, int UH, int RING> struct Ring {
+  static constexpr int kChunk = sizeof(E) / 2;                 // 16-byte pieces of 8 elements
+  static constexpr int kPieces = UH * NSRC * 2 * kChunk;       // pieces a lane copies per item
+  static constexpr int kBytesPerThread = RING * kPieces * 16;
+};
+
+// 16 bytes to shared memory, or zeros (nothing is read) where !valid.
+__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, bool valid) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(valid ? 16 : 0) : "memory");
+}
+
+// ring: the block's shared memory, blockDim.x * kBytesPerThread bytes.
+// source(group) gives a group's Source; begin() is called after the first rows
+// were asked for, enter(group, head) when the walk comes to a unit, use(rows) for
+// each of the unit's heads in order, with the 2 * NSRC raw chunks (zeros where
+// Source.on is false).  All are called by the whole warp.
+template <typename E, int NSRC, int UH, int RING, class FSource, class FBegin, class FEnter, class FUse>
+__device__ __forceinline__ void walk_rows(const Units& un, const Lane& ln, uint4* ring, FSource&& source,
+                                          FBegin&& begin, FEnter&& enter, FUse&& use) {
+  using R = Ring<E, NSRC, UH, RING>;
+  if (un.count <= 0) return;
+  constexpr uint32_t kSlot = kWalkThreads * 16, kStage = R::kPieces * kSlot;
+  const uint32_t mine = smem_u32(ring) + threadIdx.x * 16;
+  Cursor ahead(un);           // unit of the next item to ask for
+  int64_t more = un.count;    // units not yet wholly asked for
+  int pn = 0;                 // heads of `ahead` not yet asked for
+  const E* at[NSRC];
+  int64_t hs[NSRC];
+  bool on = false;
+  const int d12 = ln.o2 - ln.o1;
+  auto open = [&]() {
+    const int h = ahead.part * un.C;
+    const Source<E, NSRC> src = source(ahead.group);
+    on = src.on;
+    pn = min(un.C, un.H - h);
+#pragma unroll
+    for (int k = 0; k < NSRC; ++k) {
+      hs[k] = src.hs[k];
+      at[k] = src.base[k] + h * hs[k] + ln.o1;
+    }
+  };
+  open();
+  uint32_t ask_slot = mine, use_slot = mine;
+  auto ask = [&]() {
+    if (more > 0) {
+#pragma unroll
+      for (int u = 0; u < UH; ++u) {
+        const bool ok = on && (UH == 1 || u < pn);
+#pragma unroll
+        for (int k = 0; k < NSRC; ++k) {
+          const uint32_t to = ask_slot + (u * NSRC + k) * 2 * R::kChunk * kSlot;
+#pragma unroll
+          for (int c = 0; c < R::kChunk; ++c) {
+            cp_async16(to + c * kSlot, at[k] + c * 4, ok);
+            cp_async16(to + (R::kChunk + c) * kSlot, at[k] + d12 + c * 4, ok);
+          }
+          at[k] += hs[k];
+        }
+      }
+      pn -= UH;
+      if (pn <= 0 && --more > 0) {
+        ahead.next(un);
+        open();
+      }
+    }
+    asm volatile("cp.async.commit_group;" ::: "memory");
+    ask_slot = ask_slot == mine + (RING - 1) * kStage ? mine : ask_slot + kStage;
+  };
+#pragma unroll
+  for (int s = 0; s < RING - 1; ++s) ask();
+  begin();
+  Cursor cur(un);
+  for (int64_t j = un.count; j > 0; --j, cur.next(un)) {
+    const int h = cur.part * un.C;
+    enter(cur.group, h);
+    for (int n = min(un.C, un.H - h); n > 0; n -= UH) {
+      asm volatile("cp.async.wait_group %0;" ::"n"(RING - 2) : "memory");
+      Raw8<E> rows[UH][2 * NSRC];
+#pragma unroll
+      for (int u = 0; u < UH; ++u)
+#pragma unroll
+        for (int k = 0; k < 2 * NSRC; ++k)
+#pragma unroll
+          for (int c = 0; c < R::kChunk; ++c) {
+            uint4& v = rows[u][k].u[c];
+            asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];"
+                         : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
+                         : "r"(use_slot + ((u * 2 * NSRC + k) * R::kChunk + c) * kSlot)
+                         : "memory");
+          }
+      use_slot = use_slot == mine + (RING - 1) * kStage ? mine : use_slot + kStage;
+      ask();  // into the slot of the item before this one: its rows were used
+#pragma unroll
+      for (int u = 0; u < UH; ++u)
+        if (UH == 1 || u < n) use(rows[u]);
+    }
+  }
+  asm volatile("cp.async.wait_group 0;" ::: "memory");  // nothing of this walk is left in flight
+}
+
+// cos and sin of a walk's units, asked for one unit ahead (the position two
+// ahead), so that entering a unit waits for neither.  pos_at(group): the lane's
+// position there, -1 (none) where it has no token.
+constexpr int64_t kNoPos = INT64_MIN;
+template <class FPos> struct Angles {
+  const Tables& t;
+  const Lane& l;
+  unsigned* bad;
+  const Units& un;
+  FPos pos_at;
+  Cursor ahead;     // of next_pos
+  int64_t more;     // units behind it
+  int64_t next_pos;
+  uint4 raw[4];
+  bool have;
+
+  __device__ __forceinline__ Angles(const Tables& tb, const Lane& ln, unsigned* b, const Units& u, FPos p)
+      : t(tb), l(ln), bad(b), un(u), pos_at(p), ahead(u), more(u.count - 1), have(false) {}
+  // The first unit's, once the walk has asked for its first rows.
+  __device__ __forceinline__ void begin() {
+    next_pos = pos_at(ahead.group);
+    step();
+  }
+  // Asks for the angles of next_pos, and for the position behind it.
+  __device__ __forceinline__ void step() {
+    int64_t p = next_pos;
+    have = l.active && l.rotated && p != kNoPos;
+    if (more > 0) {
+      ahead.next(un);
+      --more;
+      next_pos = pos_at(ahead.group);
+    } else {
+      next_pos = kNoPos;
+    }
+    if (!have) return;
+    if (p < 0 || p >= t.num_pos) {
+      if (l.o1 == 0) atomicAdd(bad, 1u);
+      p = 0;
+    }
+    const int64_t at = p * (t.R / 2) + l.o1;
+    const int es = t.cs_dtype == SA_F32 ? 4 : 2;
+    const uint4* c = reinterpret_cast<const uint4*>(static_cast<const uint8_t*>(t.cosv) + at * es);
+    const uint4* s = reinterpret_cast<const uint4*>(static_cast<const uint8_t*>(t.sinv) + at * es);
+    raw[0] = __ldg(c);
+    raw[2] = __ldg(s);
+    if (t.cs_dtype == SA_F32) {
+      raw[1] = __ldg(c + 1);
+      raw[3] = __ldg(s + 1);
+    }
+  }
+  template <typename CS> __device__ __forceinline__ void open(float2 (&c)[4], float2 (&s)[4]) {
+    Raw8<CS> a, b;
+#pragma unroll
+    for (int i = 0; i < (int)sizeof(CS) / 2; ++i) a.u[i] = raw[i], b.u[i] = raw[2 + i];
+    a.get(c);
+    b.get(s);
+  }
+  // cos and sin of the unit that the walk enters.
+  __device__ __forceinline__ void enter(float2 (&c)[4], float2 (&s)[4]) {
+    if (!have) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) c[i] = splat(1.f), s[i] = splat(0.f);
+    } else if (t.cs_dtype == SA_F32) {
+      open<float>(c, s);
+    } else if (t.cs_dtype == SA_BF16) {
+      open<__nv_bfloat16>(c, s);
+    } else {
+      open<__half>(c, s);
+    }
+    step();
+  }
+};
+
+// n / d for 0 <= n < 2^31 by a multiplication.
+struct FastDiv {
+  uint32_t d, mul, shift;
+  __host__ FastDiv() : d(1), mul(0), shift(0) {}
+  __host__ explicit FastDiv(uint32_t divisor) : d(divisor), mul(0), shift(0) {
+    if (d <= 1) return;
+    uint32_t bits = 0;
+    while ((1ull << bits) < d) ++bits;  // 2^bits >= d
+    // n mul / 2^(31 + bits) passes n / d by less than n / 2^(31 + bits) < 1 / d: the floors are the same
+    mul = (uint32_t)(((1ull << (31 + bits)) + d - 1) / d);
+    shift = bits - 1;
+  }
+  __device__ __forceinline__ uint32_t div(uint32_t n) const { return mul ? __umulhi(n, mul) >> shift : n; }
+};
 
 // ---- host side ----------------------------------------------------------------
 
 inline bool al16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
+
+// SMs of the current device (asked once per device: the query costs as much as a launch).
+inline int sm_count() {
+  static std::atomic<int> known[64];
+  int dev = 0, n = 0;
+  if (cudaGetDevice(&dev) == cudaSuccess && dev >= 0 && dev < 64) {
+    n = known[dev].load(std::memory_order_relaxed);
+    if (n > 0) return n;
+    if (cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) == cudaSuccess && n > 0) {
+      known[dev].store(n, std::memory_order_relaxed);
+      return n;
+    }
+  }
+  cudaGetLastError();
+  return 148;
+}
 
 // Lanes of a row: the power of two that holds its D / 16 chunk pairs.
 inline int lanes_for(int64_t D) {
@@ -214,12 +489,27 @@ inline int make_tables(Tables* t, const void* cosv, const void* sinv, int cs_dty
   return SA_OK;
 }
 
-// Heads a warp takes per token: 8 (the angles are loaded once for all of them)
-// unless that leaves fewer than `want` warps, then fewer.
-inline int heads_per_warp(int64_t groups, int64_t heads, int64_t want) {
-  int hc = 8;
-  while (hc > 1 && groups * ((heads + hc - 1) / hc) < want) hc /= 2;
-  return hc;
+// Heads of a unit, for `rows` (token group, head) pairs on `warps` warps: the
+// choice among least, ..., 8 with the shortest busiest warp, a unit costing its
+// heads and about one and a half more for its angles and addresses.  Many heads
+// share a token's angles; few keep the shares equal, and a small problem spread out.
+inline int unit_heads(int64_t rows, int64_t warps, int least) {
+  int best = least;
+  double cost = 0;
+  for (int c = least; c <= 8; c *= 2) {
+    const int64_t units = (rows + c - 1) / c, rounds = (units + warps - 1) / warps;
+    const double t = (double)rounds * (c + 1.5);
+    if (c == least || t < cost) best = c, cost = t;
+  }
+  return best;
+}
+
+// Blocks of kWalkThreads for `units`: one resident wave of `per_sm` blocks an
+// SM, fewer when there are not that many units for the warps.
+inline int64_t walk_blocks(int64_t units, int per_sm) {
+  const int64_t need = (units + kWalkThreads / 32 - 1) / (kWalkThreads / 32);
+  const int64_t wave = (int64_t)per_sm * sm_count();
+  return need < wave ? need : wave;
 }
 
 }  // namespace qkr

