@@ -235,7 +235,27 @@ struct AppendArgs {
   FastDiv by_bs;
 };
 
-constexpr int kAppendHeads = 2, kAppendRing = 6, kAppendBlocks = 4;
+constexpr int kAppendRing = 8, kAppendBlocks = 3;  // 33 KB and 168 registers a thread (at 128 it spills: 46 us for 39)
+
+// A token's position; a padding token's (its slot is negative) says nothing and counts as 0.
+template <int L> struct Where {
+  const Tables& tb;
+  const AppendArgs& a;
+  struct Pos {
+    RawInt pos, slot;
+  };
+  __device__ __forceinline__ bool fetch(int64_t group, Pos& p) const {
+    const int64_t n = group * (32 / L) + (threadIdx.x & 31) / L;
+    if (n >= a.N || tb.R == 0) return false;
+    p.slot.load(a.slots, 8, n);
+    if (tb.pos_bytes) p.pos.load(tb.pos, tb.pos_bytes, n);
+    else p.pos.v = make_uint2((uint32_t)n, 0);
+    return true;
+  }
+  __device__ __forceinline__ int64_t get(const Pos& p) const {
+    return p.slot.get(8) < 0 ? 0 : p.pos.get(tb.pos_bytes);
+  }
+};
 
 template <typename E, int L>
 __global__ void __launch_bounds__(kWalkThreads, kAppendBlocks) qk_norm_rope_append(AppendArgs a, Tables tb) {
@@ -248,31 +268,27 @@ __global__ void __launch_bounds__(kWalkThreads, kAppendBlocks) qk_norm_rope_appe
   if (un.count == 0) return;
   const Lane ln = lane_of<L>(tb);
   auto token = [&](int64_t g) { return g * (32 / L) + (threadIdx.x & 31) / L; };
-  auto slot_at = [&](int64_t g) -> int64_t {
-    const int64_t n = token(g);
-    return n < a.N ? __ldg(a.slots + n) : -1;
-  };
-  auto pos_at = [&](int64_t g) -> int64_t {  // 0 for a padding token: its position says nothing
-    const int64_t n = token(g);
-    if (side == 2 || tb.R == 0 || n >= a.N) return kNoPos;
-    const int64_t p = tb.pos_bytes ? read_pos(tb.pos, tb.pos_bytes, n) : n;
-    return slot_at(g) < 0 ? 0 : p;
-  };
-  Angles<decltype(pos_at)> ang(tb, ln, &g_bad_entries, un, pos_at);
-  Cursor slot_ahead(un);  // of next_slot
-  int64_t more_slots = un.count - 1;
+  const Where<L> where{tb, a};
+  Angles<Where<L>> ang(tb, ln, &g_bad_entries, un, where);
   Map map;
   E* y = nullptr;  // the row that comes next
-  int64_t yh = 0, next_slot = 0;
+  int64_t yh = 0;
+  RawInt next_slot;
+  Cursor slot_ahead(un);  // of next_slot
+  int64_t more_slots = un.count - 1;
+  auto ask_slot = [&]() {
+    const int64_t n = token(slot_ahead.group);
+    if (n < a.N) next_slot.load(a.slots, 8, n);
+  };
   bool write = false, padding = false;
-  walk_rows<E, 1, kAppendHeads, kAppendRing>(
+  walk_rows<E, 1, kAppendRing>(
       un, ln, ring,
       [&](int64_t g) {
         const int64_t n = token(g);
         return Source<E, 1>{{static_cast<const E*>(sd.x) + (n < a.N ? n : 0) * sd.xt}, {sd.xh}, ln.active && n < a.N};
       },
       [&]() {
-        next_slot = slot_at(slot_ahead.group);
+        ask_slot();
         if (side < 2) ang.begin();
       },
       [&](int64_t g, int h) {
@@ -282,16 +298,16 @@ __global__ void __launch_bounds__(kWalkThreads, kAppendBlocks) qk_norm_rope_appe
           ang.enter(c, s);
           map.make(c, s, w1, w2);
         }
-        int64_t slot = next_slot;
+        const int64_t n = token(g);
+        int64_t slot = n < a.N ? next_slot.get(8) : -1;
         if (more_slots-- > 0) {
           slot_ahead.next(un);
-          next_slot = slot_at(slot_ahead.group);
+          ask_slot();
         }
         if (slot >= a.num_slots) {
           if (side == 0 && ln.o1 == 0) atomicAdd(&g_bad_entries, 1u);
           slot = -1;
         }
-        const int64_t n = token(g);
         padding = slot < 0;
         if (side == 0) {  // a padding token's q row is zeros
           write = ln.active && n < a.N;
@@ -324,8 +340,8 @@ template <typename F> static int opt_in(F* f, size_t bytes) {
 
 template <typename E, int L>
 static int launch_append_l(const AppendArgs& a, const Tables& tb, cudaStream_t st) {
-  constexpr int smem = Ring<E, 1, kAppendHeads, kAppendRing>::kBytesPerThread * kWalkThreads;
-  static_assert(smem <= 56 * 1024, "four blocks an SM");
+  constexpr int smem = Ring<E, 1, kAppendRing>::kBytesPerThread * kWalkThreads;
+  static_assert(smem <= 56 * 1024, "three blocks an SM");
   const int rc = opt_in(qk_norm_rope_append<E, L>, smem);
   if (rc != SA_OK) return rc;
   const unsigned blocks = (unsigned)(a.warps / (kWalkThreads / 32));
@@ -457,8 +473,7 @@ extern "C" int sa_qk_norm_rope_paged_append(const void* q, const void* k, const 
   const void* xs[3] = {q, k, v};
   const void* ws[3] = {q_weight, k_weight, nullptr};
   const int64_t heads = Hq + 2 * Hkv;
-  const int C = sa::qkr::unit_heads(groups * heads, (int64_t)kAppendBlocks * sa::qkr::sm_count() * (sa::qkr::kWalkThreads / 32),
-                                    kAppendHeads);
+  const int C = sa::qkr::unit_heads(groups * heads, (int64_t)kAppendBlocks * sa::qkr::sm_count() * (sa::qkr::kWalkThreads / 32));
   int64_t units = 0;
   for (int i = 0; i < 3; ++i) {
     a.s[i].x = xs[i];

@@ -71,10 +71,20 @@ __device__ __forceinline__ Token token_of(const Shape& sh, int64_t group) {
   return k;
 }
 
-__device__ __forceinline__ int64_t pos_of(const Tables& tb, const Token& k) {
-  if (!k.valid || tb.R == 0) return kNoPos;
-  return tb.pos_bytes ? read_pos(tb.pos, tb.pos_bytes, k.b * tb.pos_sb + k.t) : k.t;
-}
+// A token's position: its index along T, or what `positions` says.
+template <int L> struct Where {
+  const Tables& tb;
+  const Shape& sh;
+  using Pos = RawInt;
+  __device__ __forceinline__ bool fetch(int64_t group, RawInt& p) const {
+    const Token k = token_of<L>(sh, group);
+    if (!k.valid || tb.R == 0) return false;
+    if (tb.pos_bytes) p.load(tb.pos, tb.pos_bytes, k.b * tb.pos_sb + k.t);
+    else p.v.x = (uint32_t)k.t;
+    return true;
+  }
+  __device__ __forceinline__ int64_t get(const RawInt& p) const { return p.get(tb.pos_bytes); }
+};
 
 // A warp's units of q or of k.
 struct Part {
@@ -92,12 +102,10 @@ __device__ __forceinline__ Part part_of_warp(const Side& q, const Side& k, const
   return p;
 }
 
-// Heads an item, depth of the ring and resident blocks an SM: four forward
-// blocks of 49 KB and 128 registers a thread, three backward blocks of at most
-// 65 KB and 168 registers (at 128 the backward spills).
-template <typename E> constexpr int kFwdHeads = sizeof(E) == 4 ? 1 : 2;
-constexpr int kBwdHeads = 1;
-constexpr int kFwdRing = 6;
+// Depth of the ring and resident blocks an SM: four forward blocks of 41 KB (16-bit)
+// and 128 registers a thread, three backward blocks of at most 65 KB and 168
+// registers (at 128 the backward spills).
+template <typename E> constexpr int kFwdRing = sizeof(E) == 4 ? 6 : 10;
 template <typename E> constexpr int kBwdRing = sizeof(E) == 4 ? 4 : 6;
 constexpr int kFwdBlocks = 4, kBwdBlocks = 3;
 
@@ -111,12 +119,12 @@ __global__ void __launch_bounds__(kWalkThreads, kFwdBlocks)
   if (part.un.count == 0) return;
   const Side& sd = part.is_q ? q : k;
   const Lane ln = lane_of<L>(tb);
-  auto pos_at = [&](int64_t g) { return pos_of(tb, token_of<L>(sh, g)); };
-  Angles<decltype(pos_at)> ang(tb, ln, &g_bad_positions, part.un, pos_at);
+  const Where<L> where{tb, sh};
+  Angles<Where<L>> ang(tb, ln, &g_bad_positions, part.un, where);
   Map map;
   E* y = nullptr;  // the row that comes next
   bool on = false;
-  walk_rows<E, 1, kFwdHeads<E>, kFwdRing>(
+  walk_rows<E, 1, kFwdRing<E>>(
       part.un, ln, ring,
       [&](int64_t g) {
         const Token tk = token_of<L>(sh, g);
@@ -153,15 +161,15 @@ __global__ void __launch_bounds__(kWalkThreads, kBwdBlocks)
   const Part part = part_of_warp(q, k, sh);
   const Side& sd = part.is_q ? q : k;
   const Lane ln = lane_of<L>(tb);
-  auto pos_at = [&](int64_t g) { return pos_of(tb, token_of<L>(sh, g)); };
-  Angles<decltype(pos_at)> ang(tb, ln, &g_bad_positions, part.un, pos_at);
+  const Where<L> where{tb, sh};
+  Angles<Where<L>> ang(tb, ln, &g_bad_positions, part.un, where);
   float2 c[4], s[4], w1[4], w2[4], dw1[4], dw2[4];
 #pragma unroll
   for (int i = 0; i < 4; ++i) dw1[i] = dw2[i] = splat(0.f);
   load_weights(sd.w, sh.w_dtype, ln, w1, w2);
   E* dx = nullptr;  // the row that comes next
   bool on = false;
-  walk_rows<E, 2, kBwdHeads, kBwdRing<E>>(
+  walk_rows<E, 2, kBwdRing<E>>(
       part.un, ln, ring,
       [&](int64_t g) {
         const Token tk = token_of<L>(sh, g);
@@ -342,7 +350,7 @@ template <typename F> static int opt_in(F* f, int bytes) {
 template <typename E, int L>
 static int launch_fwd_l(const Side& q, const Side& k, const Tables& tb, const Shape& sh, int64_t blocks,
                         cudaStream_t st) {
-  constexpr int smem = Ring<E, 1, kFwdHeads<E>, kFwdRing>::kBytesPerThread * kWalkThreads;
+  constexpr int smem = Ring<E, 1, kFwdRing<E>>::kBytesPerThread * kWalkThreads;
   static_assert(smem <= 56 * 1024, "four blocks an SM");
   const int rc = opt_in(qk_norm_rope_fwd<E, L>, smem);
   if (rc != SA_OK) return rc;
@@ -365,7 +373,7 @@ static int launch_fwd(const Side& q, const Side& k, const Tables& tb, const Shap
 template <typename E, int L>
 static int launch_bwd_l(const Side& q, const Side& k, const Tables& tb, const Shape& sh, float* part, int64_t blocks,
                         cudaStream_t st) {
-  constexpr int smem = Ring<E, 2, kBwdHeads, kBwdRing<E>>::kBytesPerThread * kWalkThreads;
+  constexpr int smem = Ring<E, 2, kBwdRing<E>>::kBytesPerThread * kWalkThreads;
   static_assert(smem >= kWalkThreads / 32 * 256 * 4, "the block's dw sums");
   static_assert(smem <= 74 * 1024, "three blocks an SM");
   const int rc = opt_in(qk_norm_rope_bwd<E, L>, smem);
@@ -423,10 +431,9 @@ extern "C" int sa_qk_norm_rope(const void* q, const void* k, void* q_out, void* 
   if (Hkv > 0 && ((rc = check_rows(k, k_strides, es)) != SA_OK || (rc = check_rows(k_out, ko_strides, es)) != SA_OK))
     return rc;
   const int64_t groups = groups_of(B * T, D);
-  const int uh = unit_heads(groups * (Hq + Hkv), (int64_t)kFwdBlocks * sm_count() * (kWalkThreads / 32),
-                            dtype == SA_F32 ? kFwdHeads<float> : kFwdHeads<__half>);
-  const Side a = side_of(q, q_out, nullptr, q_weight, Hq, q_strides, qo_strides, nullptr, groups, uh);
-  const Side b = side_of(k, k_out, nullptr, k_weight, Hkv, k_strides, ko_strides, nullptr, groups, uh);
+  const int C = unit_heads(groups * (Hq + Hkv), (int64_t)kFwdBlocks * sm_count() * (kWalkThreads / 32));
+  const Side a = side_of(q, q_out, nullptr, q_weight, Hq, q_strides, qo_strides, nullptr, groups, C);
+  const Side b = side_of(k, k_out, nullptr, k_weight, Hkv, k_strides, ko_strides, nullptr, groups, C);
   Shape sh{B * T, T, 0, w_dtype, FastDiv((uint32_t)T)};
   const int64_t blocks = plan(a, b, &sh, kFwdBlocks);
   cudaStream_t st = static_cast<cudaStream_t>(stream);
@@ -472,9 +479,9 @@ extern "C" int sa_qk_norm_rope_bwd(const void* q, const void* k, const void* dq_
                  (rc = check_rows(dk, dk_strides, es)) != SA_OK))
     return rc;
   const int64_t groups = work ? groups_of(B * T, D) : 0;
-  const int uh = unit_heads(groups * (hq + hk), (int64_t)kBwdBlocks * sm_count() * (kWalkThreads / 32), kBwdHeads);
-  const Side a = side_of(q, dq, dq_out, q_weight, hq, q_strides, dq_strides, dqo_strides, groups, uh);
-  const Side b = side_of(k, dk, dk_out, k_weight, hk, k_strides, dk_strides, dko_strides, groups, uh);
+  const int C = unit_heads(groups * (hq + hk), (int64_t)kBwdBlocks * sm_count() * (kWalkThreads / 32));
+  const Side a = side_of(q, dq, dq_out, q_weight, hq, q_strides, dq_strides, dqo_strides, groups, C);
+  const Side b = side_of(k, dk, dk_out, k_weight, hk, k_strides, dk_strides, dko_strides, groups, C);
   Shape sh{B * T, work ? T : 1, 0, w_dtype, FastDiv(work ? (uint32_t)T : 1u)};
   const int64_t blocks = plan(a, b, &sh, kBwdBlocks);
   float* part = dw ? static_cast<float*>(workspace) : nullptr;

@@ -125,9 +125,18 @@ __device__ __forceinline__ Lane lane_of(const Tables& t) {
   return l;
 }
 
-__device__ __forceinline__ int64_t read_pos(const void* pos, int bytes, int64_t at) {
-  return bytes == 8 ? __ldg(static_cast<const long long*>(pos) + at) : (int64_t)__ldg(static_cast<const int*>(pos) + at);
-}
+// A 4- or 8-byte integer as loaded, so that a load can be issued long before its
+// value is looked at (a conversion beside the load would wait for it).
+struct RawInt {
+  uint2 v;
+  __device__ __forceinline__ void load(const void* p, int bytes, int64_t at) {
+    if (bytes == 8) v = __ldg(static_cast<const uint2*>(p) + at);
+    else v.x = __ldg(static_cast<const unsigned*>(p) + at);
+  }
+  __device__ __forceinline__ int64_t get(int bytes) const {
+    return bytes == 8 ? (int64_t)(((uint64_t)v.y << 32) | v.x) : (int64_t)(int)v.x;
+  }
+};
 
 // Sum over the L lanes of a row; every lane of the warp takes part.
 template <int L> __device__ __forceinline__ float row_sum(float v) {
@@ -195,7 +204,7 @@ __device__ __forceinline__ void load_weights(const void* w, int w_dtype, const L
 // The rows are cut into units: a token group (32 / L neighbouring tokens, one
 // row per L lanes) and C neighbouring heads.  Warp w of W takes units w, w + W,
 // ..., so what all warps read and write at a time lies close together.  Inside a
-// unit an item is UH heads.  Every lane streams its own 16-byte chunks of the rows
+// unit an item is one head.  Every lane streams its own 16-byte chunks of the rows
 // through a private ring in shared memory with cp.async, RING - 1 items ahead:
 // the bytes in flight then cost no registers (with plain loads 128 registers a
 // thread held only one item's), and since a lane reads only what it copied
@@ -241,9 +250,9 @@ template <typename E, int NSRC> struct Source {
   bool on;              // the lane has a chunk of an existing token
 };
 
-template <typename E, int NSRC, int UH, int RING> struct Ring {
+template <typename E, int NSRC, int RING> struct Ring {
   static constexpr int kChunk = sizeof(E) / 2;                 // 16-byte pieces of 8 elements
-  static constexpr int kPieces = UH * NSRC * 2 * kChunk;       // pieces a lane copies per item
+  static constexpr int kPieces = NSRC * 2 * kChunk;       // pieces a lane copies per item
   static constexpr int kBytesPerThread = RING * kPieces * 16;
 };
 
@@ -257,10 +266,10 @@ __device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, bool v
 // were asked for, enter(group, head) when the walk comes to a unit, use(rows) for
 // each of the unit's heads in order, with the 2 * NSRC raw chunks (zeros where
 // Source.on is false).  All are called by the whole warp.
-template <typename E, int NSRC, int UH, int RING, class FSource, class FBegin, class FEnter, class FUse>
+template <typename E, int NSRC, int RING, class FSource, class FBegin, class FEnter, class FUse>
 __device__ __forceinline__ void walk_rows(const Units& un, const Lane& ln, uint4* ring, FSource&& source,
                                           FBegin&& begin, FEnter&& enter, FUse&& use) {
-  using R = Ring<E, NSRC, UH, RING>;
+  using R = Ring<E, NSRC, RING>;
   if (un.count <= 0) return;
   constexpr uint32_t kSlot = kWalkThreads * 16, kStage = R::kPieces * kSlot;
   const uint32_t mine = smem_u32(ring) + threadIdx.x * 16;
@@ -287,21 +296,16 @@ __device__ __forceinline__ void walk_rows(const Units& un, const Lane& ln, uint4
   auto ask = [&]() {
     if (more > 0) {
 #pragma unroll
-      for (int u = 0; u < UH; ++u) {
-        const bool ok = on && (UH == 1 || u < pn);
+      for (int k = 0; k < NSRC; ++k) {
+        const uint32_t to = ask_slot + k * 2 * R::kChunk * kSlot;
 #pragma unroll
-        for (int k = 0; k < NSRC; ++k) {
-          const uint32_t to = ask_slot + (u * NSRC + k) * 2 * R::kChunk * kSlot;
-#pragma unroll
-          for (int c = 0; c < R::kChunk; ++c) {
-            cp_async16(to + c * kSlot, at[k] + c * 4, ok);
-            cp_async16(to + (R::kChunk + c) * kSlot, at[k] + d12 + c * 4, ok);
-          }
-          at[k] += hs[k];
+        for (int c = 0; c < R::kChunk; ++c) {
+          cp_async16(to + c * kSlot, at[k] + c * 4, on);
+          cp_async16(to + (R::kChunk + c) * kSlot, at[k] + d12 + c * 4, on);
         }
+        at[k] += hs[k];
       }
-      pn -= UH;
-      if (pn <= 0 && --more > 0) {
+      if (--pn == 0 && --more > 0) {
         ahead.next(un);
         open();
       }
@@ -316,66 +320,63 @@ __device__ __forceinline__ void walk_rows(const Units& un, const Lane& ln, uint4
   for (int64_t j = un.count; j > 0; --j, cur.next(un)) {
     const int h = cur.part * un.C;
     enter(cur.group, h);
-    for (int n = min(un.C, un.H - h); n > 0; n -= UH) {
+    for (int n = min(un.C, un.H - h); n > 0; --n) {
       asm volatile("cp.async.wait_group %0;" ::"n"(RING - 2) : "memory");
-      Raw8<E> rows[UH][2 * NSRC];
+      Raw8<E> rows[2 * NSRC];
 #pragma unroll
-      for (int u = 0; u < UH; ++u)
+      for (int k = 0; k < 2 * NSRC; ++k)
 #pragma unroll
-        for (int k = 0; k < 2 * NSRC; ++k)
-#pragma unroll
-          for (int c = 0; c < R::kChunk; ++c) {
-            uint4& v = rows[u][k].u[c];
-            asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];"
-                         : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
-                         : "r"(use_slot + ((u * 2 * NSRC + k) * R::kChunk + c) * kSlot)
-                         : "memory");
-          }
+        for (int c = 0; c < R::kChunk; ++c) {
+          uint4& v = rows[k].u[c];
+          asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];"
+                       : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
+                       : "r"(use_slot + (k * R::kChunk + c) * kSlot)
+                       : "memory");
+        }
       use_slot = use_slot == mine + (RING - 1) * kStage ? mine : use_slot + kStage;
       ask();  // into the slot of the item before this one: its rows were used
-#pragma unroll
-      for (int u = 0; u < UH; ++u)
-        if (UH == 1 || u < n) use(rows[u]);
+      use(rows);
     }
   }
   asm volatile("cp.async.wait_group 0;" ::: "memory");  // nothing of this walk is left in flight
 }
 
 // cos and sin of a walk's units, asked for one unit ahead (the position two
-// ahead), so that entering a unit waits for neither.  pos_at(group): the lane's
-// position there, -1 (none) where it has no token.
-constexpr int64_t kNoPos = INT64_MIN;
-template <class FPos> struct Angles {
+// ahead), so that entering a unit waits for neither.  Where.fetch(group, pos)
+// loads what the lane's position there is made of (false: it has no token);
+// Where.get(pos) is called a unit later.
+template <class Where> struct Angles {
   const Tables& t;
   const Lane& l;
   unsigned* bad;
   const Units& un;
-  FPos pos_at;
-  Cursor ahead;     // of next_pos
+  const Where& where;
+  Cursor ahead;     // of next
   int64_t more;     // units behind it
-  int64_t next_pos;
+  typename Where::Pos next;
+  bool next_on;
   uint4 raw[4];
   bool have;
 
-  __device__ __forceinline__ Angles(const Tables& tb, const Lane& ln, unsigned* b, const Units& u, FPos p)
-      : t(tb), l(ln), bad(b), un(u), pos_at(p), ahead(u), more(u.count - 1), have(false) {}
+  __device__ __forceinline__ Angles(const Tables& tb, const Lane& ln, unsigned* b, const Units& u, const Where& w)
+      : t(tb), l(ln), bad(b), un(u), where(w), ahead(u), more(u.count - 1), next_on(false), have(false) {}
   // The first unit's, once the walk has asked for its first rows.
   __device__ __forceinline__ void begin() {
-    next_pos = pos_at(ahead.group);
+    next_on = where.fetch(ahead.group, next);
     step();
   }
-  // Asks for the angles of next_pos, and for the position behind it.
+  // Asks for the angles of `next`, and for the position behind it.
   __device__ __forceinline__ void step() {
-    int64_t p = next_pos;
-    have = l.active && l.rotated && p != kNoPos;
+    have = next_on && l.active && l.rotated;
+    const int64_t pos = have ? where.get(next) : 0;
+    next_on = false;
     if (more > 0) {
       ahead.next(un);
       --more;
-      next_pos = pos_at(ahead.group);
-    } else {
-      next_pos = kNoPos;
+      next_on = where.fetch(ahead.group, next);
     }
     if (!have) return;
+    int64_t p = pos;
     if (p < 0 || p >= t.num_pos) {
       if (l.o1 == 0) atomicAdd(bad, 1u);
       p = 0;
@@ -490,16 +491,17 @@ inline int make_tables(Tables* t, const void* cosv, const void* sinv, int cs_dty
 }
 
 // Heads of a unit, for `rows` (token group, head) pairs on `warps` warps: the
-// choice among least, ..., 8 with the shortest busiest warp, a unit costing its
-// heads and about one and a half more for its angles and addresses.  Many heads
-// share a token's angles; few keep the shares equal, and a small problem spread out.
-inline int unit_heads(int64_t rows, int64_t warps, int least) {
-  int best = least;
+// choice among 1, 2, 4 and 8 with the shortest busiest warp, a unit costing its heads
+// and about one and a half more for its angles and addresses.  Many rows take 8:
+// a block's four warps then cover 32 neighbouring heads of their tokens (backward
+// of [4, 32 + 8, 4096, 128]: 84 us; 96 us with 4, 98 us with 16).
+inline int unit_heads(int64_t rows, int64_t warps) {
+  int best = 1;
   double cost = 0;
-  for (int c = least; c <= 8; c *= 2) {
+  for (int c = 1; c <= 8; c *= 2) {
     const int64_t units = (rows + c - 1) / c, rounds = (units + warps - 1) / warps;
     const double t = (double)rounds * (c + 1.5);
-    if (c == least || t < cost) best = c, cost = t;
+    if (c == 1 || t < cost) best = c, cost = t;
   }
   return best;
 }

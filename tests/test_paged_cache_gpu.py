@@ -180,6 +180,8 @@ def _append_inputs(N, Hq, Hkv, D, dt, seed):
     (37, 5, 12, 12, 64, 32, 16, torch.bfloat16, True), (129, 1, 9, 3, 80, 80, 5, torch.float16, True),
     (50, 0, 4, 4, 256, 0, 32, torch.bfloat16, True), (77, 3, 8, 2, 128, 64, 64, torch.bfloat16, False),
     (513, 0, 16, 1, 16, 16, 8, torch.float16, False), (3, 3, 2, 2, 64, 64, 16, torch.bfloat16, True),
+    (9001, 700, 32, 8, 64, 64, 16, torch.bfloat16, True),  # whole units of heads: slots and angles read ahead
+    (9001, 7, 24, 8, 128, 64, 16, torch.float16, True),
 ])
 @pytest.mark.parametrize("layout", ["fused", "heads first", "off"])
 def test_append_matches_the_formula(N, pad, Hq, Hkv, D, R, bs, dt, norm, layout):

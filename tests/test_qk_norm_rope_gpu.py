@@ -158,11 +158,16 @@ def test_table_types(cs):
     _check(y, *ref)
 
 
-def test_gradient_of_a_larger_problem_repeats_bitwise():
+@pytest.mark.parametrize("B,Hq,Hkv,T,D,R,dt,ps", [
+    (2, 16, 4, 2100, 128, 128, torch.bfloat16, "batch32"),
+    (3, 32, 8, 3001, 128, 128, torch.bfloat16, "batch64"),  # whole units of heads: angles through shared memory
+    (2, 24, 8, 5003, 64, 32, torch.float16, "none"),
+    (2, 20, 9, 4099, 80, 80, torch.bfloat16, "row32"),  # heads that units do not divide
+    (1, 8, 16, 5001, 128, 64, torch.float32, "row64"),
+])
+def test_gradient_of_a_larger_problem_repeats_bitwise(B, Hq, Hkv, T, D, R, dt, ps):
     """Many blocks, both sides; the weights' sums join in a fixed order."""
-    B, Hq, Hkv, T, D = 2, 16, 4, 2100, 128
-    q, k, dq, dk, wq, wk, cos, sin, pos, full, eps = _make((B, Hq, Hkv, T, D, D, torch.bfloat16, torch.float32, True,
-                                                            "batch32"))
+    q, k, dq, dk, wq, wk, cos, sin, pos, full, eps = _make((B, Hq, Hkv, T, D, R, dt, torch.float32, True, ps))
     res = []
     for _ in range(2):
         ins = [t.detach().requires_grad_(True) for t in (q, k, wq, wk)]
@@ -172,9 +177,13 @@ def test_gradient_of_a_larger_problem_repeats_bitwise():
     for x, w, dx, dw, dy in ((q, wq, res[0][0], res[0][2], dq), (k, wk, res[0][1], res[0][3], dk)):
         ref = _ref64(x, w, cos, sin, full, eps, dy)
         _check(dx, ref[2], ref[3])
-        # a lane's chain: the rows of a block's lane, at most all rows over (70 blocks x 8 warps x 4 tokens), doubled
-        chain = 64 + 2 * (x.numel() // D) // (60 * 8 * 4)
+        # a lane's chain: all rows over the warps of its side (a ninth of 1700 at least) and the tokens of a
+        # warp (2 at least), doubled for uneven shares
+        chain = 64 + 2 * (x.numel() // D) // (190 * 2)
         _check(dw, ref[4], ref[5] * (24 + chain) / 88)
+    y = sa.qk_norm_rope(q, k, cos, sin, q_weight=wq, k_weight=wk, positions=pos)
+    for x, w, o in ((q, wq, y[0]), (k, wk, y[1])):
+        _check(o, *_ref64(x, w, cos, sin, full, eps))
 
 
 def test_gradient_against_differences():
@@ -268,6 +277,14 @@ def test_far_positions_are_read_as_row_zero_and_reported():
     assert lib.sa_device_status(1) == _lib.SA_ERR_ARG
     assert torch.equal(y[0], at([3, 0, 0, 9])[0])
     assert lib.sa_device_status(1) == _lib.SA_OK
+    # the same where a warp's positions are read ahead of their use
+    q, k = randn((1, 32, 9000, 64), 1, torch.bfloat16, CUDA), randn((1, 8, 9000, 64), 2, torch.bfloat16, CUDA)
+    pos = torch.arange(9000, device=CUDA, dtype=torch.int32) % 10
+    good = sa.qk_norm_rope(q, k, cos, sin, positions=pos)
+    assert lib.sa_device_status(1) == _lib.SA_OK
+    pos[::10] = torch.where(torch.arange(900, device=CUDA) % 2 == 0, -7, 2 ** 31 - 1).to(torch.int32)  # row 0 as before
+    assert all(torch.equal(a, b) for a, b in zip(good, sa.qk_norm_rope(q, k, cos, sin, positions=pos)))
+    assert lib.sa_device_status(1) == _lib.SA_ERR_ARG
 
 
 def test_replayed_from_a_graph_and_on_another_stream():
