@@ -55,7 +55,9 @@ struct MeansArgs {
   int Hkv, bs, max_blocks;
 };
 
-// One warp: one page of one key head; LPR lanes a row, 32 / LPR rows at once.
+// One warp: one page of one key head; LPR lanes a row, 32 / LPR rows at once.  A
+// warp takes several pages and asks for the next one's first rows (and the table
+// entry behind it) before it adds this one's up.
 template <typename E, int D>
 __global__ void __launch_bounds__(256) paged_key_means_kernel(MeansArgs a) {
   constexpr int LPR = D / 8, RPW = 32 / LPR, U = 8;
@@ -64,43 +66,64 @@ __global__ void __launch_bounds__(256) paged_key_means_kernel(MeansArgs a) {
   const int ctx = (int)max((int64_t)0, min(cap, (int64_t)a.cl[b]));
   const int from = a.start ? max(0, a.start[b]) / a.bs : 0;
   const int64_t n = (int64_t)max(0, ctx / a.bs - from) * a.Hkv;
-  for (int64_t w = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5); w < n; w += (int64_t)gridDim.x * 8) {
-    const int j = (int)(w / a.Hkv), h = (int)(w - (int64_t)j * a.Hkv);
-    const int64_t page = a.bt[(int64_t)b * a.max_blocks + from + j];
-    if (page < 0 || page >= a.num_blocks) {
-      if (lane == 0 && h == 0) atomicAdd(&g_bad_pages, 1u);
-      continue;
-    }
-    const E* base = static_cast<const E*>(a.kc) + (page * a.Hkv + h) * a.bs * D + (lane % LPR) * 8;
-    float sum[8];
+  const int32_t* bt = a.bt + (int64_t)b * a.max_blocks + from;
+  const int64_t step = (int64_t)gridDim.x * 8;
+  int64_t w = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
+  if (w >= n) return;
+  const float inv = 1.0f / (float)a.bs;
+  const int r0 = lane / LPR;
+  auto page_at = [&](int64_t i) { return i < n ? __ldg(bt + i / a.Hkv) : 0; };
+  auto rows_of = [&](int64_t i, int page) {
+    const bool ok = page >= 0 && page < a.num_blocks;
+    return static_cast<const E*>(a.kc) + ((ok ? (int64_t)page : 0) * a.Hkv + i % a.Hkv) * a.bs * D + (lane % LPR) * 8;
+  };
+  auto load = [&](Raw8<E> (&x)[U], const E* base, int r) {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) sum[i] = 0.f;
-    for (int r0 = lane / LPR; r0 < a.bs; r0 += RPW * U) {
-      Raw8<E> x[U];
+    for (int u = 0; u < U; ++u) {
+      if (r + u * RPW < a.bs) x[u].load(base + (int64_t)(r + u * RPW) * D);
+      else x[u].zero();
+    }
+  };
+  Raw8<E> x[U];
+  int page = page_at(w), next = page_at(w + step);
+  load(x, rows_of(w, page), r0);
+  for (; w < n; w += step) {
+    float2 sum[4] = {{0.f, 0.f}, {0.f, 0.f}, {0.f, 0.f}, {0.f, 0.f}};
+    auto add = [&](const Raw8<E> (&y)[U]) {
 #pragma unroll
       for (int u = 0; u < U; ++u) {
-        if (r0 + u * RPW < a.bs) x[u].load(base + (int64_t)(r0 + u * RPW) * D);
-        else x[u].zero();
+        float2 f[4];
+        y[u].get(f);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) sum[i] = fadd2(sum[i], f[i]);
       }
+    };
+    const E* base = rows_of(w, page);
+    const int mine = page;
+    add(x);
+    page = next;
+    if (w + step < n) load(x, rows_of(w + step, page), r0);
+    next = page_at(w + 2 * step);
+    for (int r = r0 + RPW * U; r - r0 < a.bs; r += RPW * U) {  // pages of more rows than one batch
+      Raw8<E> y[U];
+      load(y, base, r);
+      add(y);
+    }
 #pragma unroll
-      for (int u = 0; u < U; ++u) {
-        float f[8];
-        x[u].get(f);
+    for (int i = 0; i < 4; ++i) {
 #pragma unroll
-        for (int i = 0; i < 8; ++i) sum[i] += f[i];
+      for (int m = LPR; m < 32; m <<= 1) {
+        sum[i].x += __shfl_xor_sync(0xffffffffu, sum[i].x, m);
+        sum[i].y += __shfl_xor_sync(0xffffffffu, sum[i].y, m);
       }
+      sum[i] = fmul2(sum[i], make_float2(inv, inv));
     }
-    const float inv = 1.0f / (float)a.bs;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-#pragma unroll
-      for (int m = LPR; m < 32; m <<= 1) sum[i] += __shfl_xor_sync(0xffffffffu, sum[i], m);
-      sum[i] *= inv;
-    }
-    if (lane < LPR) {
+    if (mine < 0 || mine >= a.num_blocks) {
+      if (lane == 0 && w % a.Hkv == 0) atomicAdd(&g_bad_pages, 1u);
+    } else if (lane < LPR) {
       Raw8<E> o;
       o.set(sum);
-      o.store(static_cast<E*>(a.means) + (page * a.Hkv + h) * D + lane * 8);
+      o.store(static_cast<E*>(a.means) + ((int64_t)mine * a.Hkv + w % a.Hkv) * D + lane * 8);
     }
   }
 }
@@ -133,10 +156,12 @@ __device__ __forceinline__ Seq seq_of(const SelectArgs& a, int b) {
   return s;
 }
 
-// squareplus(a)^2 without the cancellation of negative a, in 64 bits.
+// squareplus(a)^2 in 64 bits.  a + sqrt(a^2 + 4) loses about a^2 roundings for
+// negative a: the quotient that is equal to it takes over where that passes 64.
 __device__ __forceinline__ double weight64(double a) {
-  const double root = sqrt(a * a + 4.0);
-  const double sp = a < 0 ? 2.0 / (root - a) : 0.5 * (a + root);
+  const double root = sqrt(fma(a, a, 4.0));
+  double sp = 0.5 * (a + root);
+  if (a < -8.0) sp = 2.0 / (root - a);
   return sp * sp;
 }
 
@@ -145,147 +170,259 @@ __device__ __forceinline__ unsigned long long key_of(double score) {
   return isnan(score) ? 0x7ff8000000000000ull : (unsigned long long)__double_as_longlong(score);
 }
 
-// One thread: one page; PAGES pages of one key head a block, their mean keys
-// staged through shared memory (16 bytes of padding a row: conflict-free),
-// the group's queries as doubles beside them, GT heads at a time.
-template <typename E, int D, int GT, int PAGES>
-__global__ void __launch_bounds__(PAGES) paged_score_kernel(SelectArgs a) {
-  constexpr int ROW = D * 2 + 16;
-  extern __shared__ __align__(16) uint8_t smem[];
-  double* qs = reinterpret_cast<double*>(smem);  // [D][GT]
-  uint8_t* rows = smem + (size_t)D * GT * 8;
+// D += A B with A [8 pages x 4 channels], B [4 channels x 8 heads] in 64 bits: lane
+// l holds A[l / 4][l % 4], B[l % 4][l / 4] and D[l / 4][2 (l % 4) + {0, 1}].
+__device__ __forceinline__ void mma64(double (&d)[2], double a, double b) {
+  asm volatile("mma.sync.aligned.m8n8k4.row.col.f64.f64.f64.f64 {%0, %1}, {%2}, {%3}, {%0, %1};"
+               : "+d"(d[0]), "+d"(d[1])
+               : "d"(a), "d"(b));
+}
+
+// One block: 64 pages of one key head, 16 a warp (two row blocks of the product
+// above).  Lane l reads every fourth 16-byte piece of rows l / 4 and 8 + l / 4, so
+// four lanes read 64 neighbouring bytes, and the channels of a product step are
+// the same element of four neighbouring pieces; the queries lie in shared memory
+// as each lane's B of every step.  Heads go eight at a time.  (One page a thread
+// with plain fused multiply-adds took 12.5 us instead of ... for 2048 pages of 8
+// key heads: every query value had to be read again for every page.)
+template <typename E, int D>
+__global__ void __launch_bounds__(128, 4) paged_score_kernel(SelectArgs a) {
+  constexpr int P = D / 32;  // 16-byte pieces a lane holds of a row
+  constexpr bool kAhead = P <= 4;  // the next tile's rows are asked for before this one's product (at D = 256 no room)
+  __shared__ double qs[D / 4][32];
   const int u = blockIdx.y, b = u / a.Hkv, h = u - b * a.Hkv;
   const Seq s = seq_of(a, b);
-  const int m = s.n - 1, p0 = blockIdx.x * PAGES;  // candidates: all but the last
-  if (m <= a.K - 1 || p0 >= m) return;             // all of them are taken: nothing to score
-  constexpr int LPR = D / 8;
-  for (int i = threadIdx.x; i < PAGES * LPR; i += PAGES) {
-    const int r = i / LPR, c = i - r * LPR;
-    if (p0 + r >= m) break;
-    int64_t page = a.bt[(int64_t)b * a.max_blocks + p0 + r];
-    if (page < 0 || page >= a.num_blocks) {
-      if (c == 0 && h == 0) atomicAdd(&g_bad_pages, 1u);
-      page = 0;
+  const int m = s.n - 1;                            // candidates: all but the last page
+  if (m <= a.K - 1 || (int)blockIdx.x * 64 >= m) return;  // all of them are taken: nothing to score
+  const int lane = threadIdx.x & 31, c = lane & 3, step = gridDim.x * 64;
+  int p0 = blockIdx.x * 64 + (threadIdx.x >> 5) * 16 + (lane >> 2);
+  const int32_t* bt = a.bt + (int64_t)b * a.max_blocks;
+  auto load = [&](uint4 (&x)[2][P], int at) {
+    int page[2];
+#pragma unroll
+    for (int r = 0; r < 2; ++r) page[r] = at + 8 * r < m ? __ldg(bt + at + 8 * r) : 0;
+#pragma unroll
+    for (int r = 0; r < 2; ++r) {
+      if (page[r] < 0 || page[r] >= a.num_blocks) {
+        if (c == 0 && h == 0) atomicAdd(&g_bad_pages, 1u);
+        page[r] = 0;
+      }
+      const uint4* row =
+          reinterpret_cast<const uint4*>(static_cast<const E*>(a.means) + ((int64_t)page[r] * a.Hkv + h) * D);
+#pragma unroll
+      for (int i = 0; i < P; ++i) x[r][i] = __ldg(row + 4 * i + c);
     }
-    *reinterpret_cast<uint4*>(rows + r * ROW + c * 16) =
-        __ldg(reinterpret_cast<const uint4*>(static_cast<const E*>(a.means) + (page * a.Hkv + h) * D) + c);
-  }
-  double score = 0.0;
-  for (int g0 = 0; g0 < a.G; g0 += GT) {
-    if (g0) __syncthreads();  // the last group's queries have been read
-    const E* q = static_cast<const E*>(a.q) + ((int64_t)u * a.G + g0) * D;
-    for (int i = threadIdx.x; i < D * GT; i += PAGES) qs[(i % D) * GT + i / D] = (double)to_f<E>(q[i]);
-    __syncthreads();
-    double dot[GT];
+  };
+  uint4 x[2][P];
+  load(x, p0);
+  for (int t0 = blockIdx.x * 64; t0 < m; t0 += step, p0 += step) {
+    uint4 y[2][kAhead ? P : 1];
+    if constexpr (kAhead) {
+      if (t0 + step < m) load(y, p0 + step);
+    }
+    double score[2] = {0.0, 0.0};
+    for (int g0 = 0; g0 < a.G; g0 += 8) {
+      const int heads = min(8, a.G - g0);
+      if (a.G > 8 || t0 < step) {  // one group of heads stays in place
+        if (g0 || t0 >= step) __syncthreads();  // the last heads' queries have been read
+        const uint4* q = reinterpret_cast<const uint4*>(static_cast<const E*>(a.q) + ((int64_t)u * a.G + g0) * D);
 #pragma unroll
-    for (int g = 0; g < GT; ++g) dot[g] = 0.0;
-    for (int c = 0; c < LPR; ++c) {
-      float f[8];
-      unpack<E, 8>(rows + threadIdx.x * ROW + c * 16, f);
+        for (int i = threadIdx.x; i < D; i += 128) {  // 8 heads of D / 8 pieces
+          const int g = i / (D / 8), piece = i % (D / 8);
+          float f[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+          if (g < heads) {
+            const uint4 v = __ldg(q + i);
+            unpack<E, 8>(&v, f);
+          }
 #pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        const double x = (double)f[e];
+          for (int e = 0; e < 8; ++e) qs[(piece / 4) * 8 + e][g * 4 + piece % 4] = (double)f[e];
+        }
+        __syncthreads();
+      }
+      double d0[2] = {0.0, 0.0}, d1[2] = {0.0, 0.0}, o0[2] = {0.0, 0.0}, o1[2] = {0.0, 0.0};  // even and odd steps
 #pragma unroll
-        for (int g = 0; g < GT; ++g) dot[g] = fma(x, qs[(c * 8 + e) * GT + g], dot[g]);
+      for (int i = 0; i < P; ++i) {
+        float f0[8], f1[8];
+        unpack<E, 8>(&x[0][i], f0);
+        unpack<E, 8>(&x[1][i], f1);
+#pragma unroll
+        for (int e = 0; e < 8; e += 2) {
+          const double qa = qs[i * 8 + e][lane], qb = qs[i * 8 + e + 1][lane];
+          mma64(d0, (double)f0[e], qa);
+          mma64(d1, (double)f1[e], qa);
+          mma64(o0, (double)f0[e + 1], qb);
+          mma64(o1, (double)f1[e + 1], qb);
+        }
+      }
+      if (heads <= 4) {  // half the lanes have no head: they take the second row block's
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          const double other = __shfl_xor_sync(0xffffffffu, d1[e] + o1[e], 2);
+          const double w = (c < 2 ? 2 * c + e : 2 * c - 4 + e) < heads
+                               ? weight64(fma(a.scale2, c < 2 ? d0[e] + o0[e] : other, -1.0)) : 0.0;
+          score[0] += c < 2 ? w : 0.0;
+          score[1] += c < 2 ? 0.0 : w;
+        }
+      } else {
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          if (2 * c + e < heads) {
+            score[0] += weight64(fma(a.scale2, d0[e] + o0[e], -1.0));
+            score[1] += weight64(fma(a.scale2, d1[e] + o1[e], -1.0));
+          }
+        }
       }
     }
 #pragma unroll
-    for (int g = 0; g < GT; ++g) score += weight64(fma(a.scale2, dot[g], -1.0));
+    for (int r = 0; r < 2; ++r) {
+      score[r] += __shfl_xor_sync(0xffffffffu, score[r], 1);
+      score[r] += __shfl_xor_sync(0xffffffffu, score[r], 2);
+      if (c == r && p0 + 8 * r < m && SA_DCHECK(p0 + 8 * r < a.max_blocks))
+        a.keys[(int64_t)u * a.max_blocks + p0 + 8 * r] = key_of(score[r]);
+    }
+    if constexpr (kAhead) {
+#pragma unroll
+      for (int r = 0; r < 2; ++r)
+#pragma unroll
+        for (int i = 0; i < P; ++i) x[r][i] = y[r][i];
+    } else {
+      if (t0 + step < m) load(x, p0 + step);
+    }
   }
-  const int p = p0 + threadIdx.x;
-  if (p < m && SA_DCHECK(p < a.max_blocks)) a.keys[(int64_t)u * a.max_blocks + p] = key_of(score);
 }
 
 // ---- choice ---------------------------------------------------------------------
 
-constexpr int kSelThreads = 512;
 constexpr int kBins = 2048;
+constexpr int kKeep = 8;    // keys a thread keeps in registers
+constexpr int kShort = 64;  // keys that are ranked by comparing each with each
 
 // One block: one sequence and key head.  The threshold is found by counting
 // keys in kBins equal ranges of [lo, hi], which is narrowed to the range that
-// holds the last chosen key until all of that range is chosen or it is one
-// value; then one ordered pass writes what is chosen.
+// holds the last chosen key until all of that range is chosen, it is one value,
+// or so few keys that they are ranked directly; then an ordered pass writes what
+// is chosen.
+template <int kSelThreads>
 __global__ void __launch_bounds__(kSelThreads) paged_choose_kernel(SelectArgs a) {
+  constexpr int kSelWarps = kSelThreads / 32;
   __shared__ int bins[kBins];
-  __shared__ unsigned long long ends[2][kSelThreads / 32];
-  __shared__ int warp_sums[kSelThreads / 32];
-  __shared__ int found_bin, found_above, found_count;
+  __shared__ unsigned long long ends[2][kSelWarps], few[kShort];
+  __shared__ int warp_sums[kSelWarps], counts[kKeep * kSelWarps];
+  __shared__ int found_bin, found_above, found_count, nfew;
   const int u = blockIdx.x, b = u / a.Hkv, h = u - b * a.Hkv, tid = threadIdx.x;
-  const int lane = tid & 31, warp = tid >> 5, NW = kSelThreads / 32;
+  const int lane = tid & 31, warp = tid >> 5;
   for (int64_t i = (int64_t)u * kSelThreads + tid; i < a.num_tickets; i += (int64_t)gridDim.x * kSelThreads)
     a.tickets[i] = 0;
   const Seq s = seq_of(a, b);
   const int m = s.n - 1, need = min(a.K, s.n) - 1;  // of the m candidates
   const int32_t* bt = a.bt + (int64_t)b * a.max_blocks;
   const unsigned long long* keys = a.keys + (int64_t)u * a.max_blocks;
-  unsigned long long lo = 0, hi = 0;  // keys above hi are chosen; `rest` of those in [lo, hi], lowest pages first
+  // keys above hi are chosen, and `rest` of those in [lo, hi], lowest pages first
+  unsigned long long lo = 0, hi = ~0ull;
   int rest = need;
+  unsigned long long mine[kKeep];
+  const bool kept = m <= kKeep * kSelThreads;
+  auto each_key = [&](auto&& f) {
+    if (kept) {
+#pragma unroll
+      for (int j = 0; j < kKeep; ++j)
+        if (j * kSelThreads + tid < m) f(mine[j]);
+    } else {
+      for (int i = tid; i < m; i += kSelThreads) f(keys[i]);
+    }
+  };
   if (m > need && need > 0) {
+    if (kept) {
+#pragma unroll
+      for (int j = 0; j < kKeep; ++j)
+        if (j * kSelThreads + tid < m) mine[j] = keys[j * kSelThreads + tid];
+    }
     unsigned long long mn = ~0ull, mx = 0;
-    for (int i = tid; i < m; i += kSelThreads) {
-      const unsigned long long k = keys[i];
+    each_key([&](unsigned long long k) {
       mn = min(mn, k);
       mx = max(mx, k);
-    }
+    });
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) {
       mn = min(mn, __shfl_xor_sync(0xffffffffu, mn, o));
       mx = max(mx, __shfl_xor_sync(0xffffffffu, mx, o));
     }
     if (lane == 0) ends[0][warp] = mn, ends[1][warp] = mx;
+    for (int i = tid; i < kBins; i += kSelThreads) bins[i] = 0;
     __syncthreads();
-    lo = ~0ull, hi = 0;
-    for (int w = 0; w < NW; ++w) {
-      lo = min(lo, ends[0][w]);
-      hi = max(hi, ends[1][w]);
+    mn = ends[0][lane % kSelWarps];
+    mx = ends[1][lane % kSelWarps];
+#pragma unroll
+    for (int o = kSelWarps / 2; o > 0; o >>= 1) {
+      mn = min(mn, __shfl_xor_sync(0xffffffffu, mn, o));
+      mx = max(mx, __shfl_xor_sync(0xffffffffu, mx, o));
     }
+    lo = mn, hi = mx;
     while (lo < hi) {  // each round cuts hi - lo by kBins / 2 or more: at most 7
-      const unsigned long long span = hi - lo;
-      int sh = 0;
-      while ((span >> sh) >= kBins) ++sh;
-      for (int i = tid; i < kBins; i += kSelThreads) bins[i] = 0;
-      __syncthreads();
-      for (int i = tid; i < m; i += kSelThreads) {
-        const unsigned long long k = keys[i];
+      const int sh = max(0, 64 - 11 - __clzll((long long)(hi - lo)));  // (hi - lo) >> sh < kBins = 2^11
+      each_key([&](unsigned long long k) {
         if (k >= lo && k <= hi) atomicAdd(&bins[(int)((k - lo) >> sh)], 1);
-      }
+      });
       __syncthreads();
       // from the top: the bin where the count reaches rest
       constexpr int PER = kBins / kSelThreads;
-      int mine = 0;
+      int cnt[PER], sum = 0;
 #pragma unroll
-      for (int j = 0; j < PER; ++j) mine += bins[kBins - 1 - (tid * PER + j)];
-      int inc = mine;
+      for (int j = 0; j < PER; ++j) sum += cnt[j] = bins[kBins - 1 - (tid * PER + j)];
+      int inc = sum;
 #pragma unroll
       for (int o = 1; o < 32; o <<= 1) {
         const int v = __shfl_up_sync(0xffffffffu, inc, o);
         if (lane >= o) inc += v;
       }
       if (lane == 31) warp_sums[warp] = inc;
+      if (tid == 0) nfew = 0;
       __syncthreads();
-      int before = inc - mine;
-      for (int w = 0; w < warp; ++w) before += warp_sums[w];
-      if (before < rest && before + mine >= rest) {
+      int before = inc - sum;
+#pragma unroll
+      for (int w = 0; w < kSelWarps; ++w) before += w < warp ? warp_sums[w] : 0;
+      if (before < rest && before + sum >= rest) {
         int acc = before;
+#pragma unroll
         for (int j = 0; j < PER; ++j) {
-          const int bin = kBins - 1 - (tid * PER + j), c = bins[bin];
-          if (acc + c >= rest) {
-            found_bin = bin;
+          if (acc < rest && acc + cnt[j] >= rest) {
+            found_bin = kBins - 1 - (tid * PER + j);
             found_above = acc;
-            found_count = c;
-            break;
+            found_count = cnt[j];
           }
-          acc += c;
+          acc += cnt[j];
         }
       }
+#pragma unroll
+      for (int j = 0; j < PER; ++j) bins[kBins - 1 - (tid * PER + j)] = 0;  // for the next round
       __syncthreads();
       rest -= found_above;
-      const unsigned long long top = hi;
       lo += (unsigned long long)found_bin << sh;
-      hi = min(top, lo + ((1ull << sh) - 1));
-      const bool whole = found_count == rest;
-      __syncthreads();  // found_* and bins are free again
-      if (whole) break;
+      hi = min(hi, lo + ((1ull << sh) - 1));
+      const int count = found_count;
+      if (count == rest) break;  // the whole range is chosen
+      if (count <= kShort) {
+        each_key([&](unsigned long long k) {
+          if (k >= lo && k <= hi) few[atomicAdd(&nfew, 1)] = k;
+        });
+        __syncthreads();
+        if (tid < count) {
+          int above = 0, same = 0;
+          const unsigned long long k = few[tid];
+          for (int j = 0; j < count; ++j) {
+            above += few[j] > k;
+            same += few[j] == k;
+          }
+          if (above < rest && above + same >= rest) {  // the last chosen value; equal keys write the same
+            ends[0][0] = k;
+            found_above = above;
+          }
+        }
+        __syncthreads();
+        lo = hi = ends[0][0];
+        rest -= found_above;
+        break;
+      }
     }
   }
   // ordered write: pages in ascending order, the last one behind them
@@ -303,33 +440,57 @@ __global__ void __launch_bounds__(kSelThreads) paged_choose_kernel(SelectArgs a)
       tb[at] = (int32_t)(phys * a.Hkv + h);
     }
   };
-  const bool all = m <= need;
-  int base = 0, base_in = 0;  // chosen and in-range keys of earlier pages
-  for (int i0 = 0; i0 < m && need > 0; i0 += kSelThreads) {
-    const int i = i0 + tid;
-    bool above = false, in = false;
-    if (i < m) {
-      const unsigned long long k = all ? 0 : keys[i];
-      above = all || k > hi;
-      in = !all && k >= lo && k <= hi;
+  if (m <= need) {
+    for (int i = tid; i < m; i += kSelThreads) put(i, i);
+  } else if (need > 0) {
+    // a batch of kKeep * kSelThreads pages at a time; a count is in-range keys, and above ones << 16
+    int base = 0, base_in = 0;  // chosen and in-range keys of earlier batches
+    for (int i0 = 0; i0 < m; i0 += kKeep * kSelThreads) {
+      unsigned in_w[kKeep], ab_w[kKeep];
+#pragma unroll
+      for (int j = 0; j < kKeep; ++j) {
+        const int i = i0 + j * kSelThreads + tid;
+        const unsigned long long k = i >= m ? 0 : kept ? mine[j] : keys[i];
+        in_w[j] = __ballot_sync(0xffffffffu, i < m && k >= lo && k <= hi);
+        ab_w[j] = __ballot_sync(0xffffffffu, i < m && k > hi);
+        if (lane == 0) counts[j * kSelWarps + warp] = __popc(in_w[j]) | (__popc(ab_w[j]) << 16);
+      }
+      __syncthreads();
+      if (warp == 0) {  // exclusive scan of the kKeep * kSelWarps counts, in page order
+        constexpr int PER = kKeep * kSelWarps / 32;
+        int c[PER], sum = 0;
+#pragma unroll
+        for (int j = 0; j < PER; ++j) sum += c[j] = counts[lane * PER + j];
+        int inc = sum;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+          const int v = __shfl_up_sync(0xffffffffu, inc, o);
+          if (lane >= o) inc += v;
+        }
+        int at = inc - sum;
+#pragma unroll
+        for (int j = 0; j < PER; ++j) {
+          counts[lane * PER + j] = at;
+          at += c[j];
+        }
+        if (lane == 31) found_count = inc;  // of the whole batch
+      }
+      __syncthreads();
+      const unsigned below = (1u << lane) - 1;
+#pragma unroll
+      for (int j = 0; j < kKeep; ++j) {
+        const int c = counts[j * kSelWarps + warp], i = i0 + j * kSelThreads + tid;
+        const int in_before = base_in + (c & 0xffff) + __popc(in_w[j] & below);
+        const int ab_before = (c >> 16) + __popc(ab_w[j] & below);
+        const bool in = (in_w[j] >> lane) & 1, above = (ab_w[j] >> lane) & 1;
+        // chosen before this page: the above ones, and of the in-range ones the first `rest`
+        if (above || (in && in_before < rest)) put(base + ab_before + min(in_before, rest) - min(base_in, rest), i);
+      }
+      const int c = found_count;
+      base += (c >> 16) + min(base_in + (c & 0xffff), rest) - min(base_in, rest);
+      base_in += c & 0xffff;
+      __syncthreads();  // counts are free again
     }
-    const unsigned in_w = __ballot_sync(0xffffffffu, in), ab_w = __ballot_sync(0xffffffffu, above);
-    const unsigned below = (1u << lane) - 1;
-    if (lane == 0) warp_sums[warp] = __popc(in_w) | (__popc(ab_w) << 16);
-    __syncthreads();
-    int in_before = base_in + __popc(in_w & below), ab_before = __popc(ab_w & below), in_all = 0, ab_all = 0;
-    for (int w = 0; w < NW; ++w) {
-      const int c = warp_sums[w];
-      if (w < warp) in_before += c & 0xffff, ab_before += c >> 16;
-      in_all += c & 0xffff;
-      ab_all += c >> 16;
-    }
-    // chosen before this page: the above ones, and of the in-range ones the first `rest`
-    const int at = base + ab_before + min(in_before, rest) - min(base_in, rest);
-    if (above || (in && in_before < rest)) put(at, i);
-    base += ab_all + min(base_in + in_all, rest) - min(base_in, rest);
-    base_in += in_all;
-    __syncthreads();
   }
   const int chosen = s.n > 0 ? need + 1 : 0;
   if (tid == 0) {
@@ -344,11 +505,19 @@ __global__ void __launch_bounds__(kSelThreads) paged_choose_kernel(SelectArgs a)
 
 // ---- host side --------------------------------------------------------------------
 
+#ifndef CT
+#define CT 256
+#endif
+#ifndef MB
+#define MB 2
+#endif
+constexpr int kMeansBlocks = MB;
+
 template <typename E, int D>
 static int launch_means(const MeansArgs& a, int64_t B, cudaStream_t st) {
-  // enough blocks for 8 an SM, each a contiguous stride of warps; a sequence without new pages leaves at once
+  // one resident wave (kMeansBlocks an SM) over all sequences; one without new pages leaves at once
   const int64_t most = ((int64_t)a.max_blocks * a.Hkv + 7) / 8;
-  const int64_t x = std::max<int64_t>(1, std::min<int64_t>(most, (16ll * qkr::sm_count() + B - 1) / B));
+  const int64_t x = std::max<int64_t>(1, std::min<int64_t>(most, ((int64_t)kMeansBlocks * qkr::sm_count() + B - 1) / B));
   paged_key_means_kernel<E, D><<<dim3((unsigned)x, (unsigned)B), 256, 0, st>>>(a);
   return sa_record_cuda_error(cudaGetLastError());
 }
@@ -363,36 +532,18 @@ static int launch_means_d(const MeansArgs& a, int64_t B, int64_t D, cudaStream_t
   }
 }
 
-template <typename E, int D, int GT>
-static int launch_score(const SelectArgs& a, int64_t units, cudaStream_t st) {
-  constexpr int PAGES = D == 256 ? 64 : 128;
-  constexpr size_t smem = (size_t)D * GT * 8 + (size_t)PAGES * (D * 2 + 16);
-  static_assert(smem <= 64 * 1024, "score kernel's shared memory");
-  auto kfn = paged_score_kernel<E, D, GT, PAGES>;
-  if (smem > 48 * 1024) {
-    const int rc = sa_record_cuda_error(cudaFuncSetAttribute(kfn, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
-    if (rc != SA_OK) return rc;
-  }
-  kfn<<<dim3((unsigned)((a.max_blocks + PAGES - 1) / PAGES), (unsigned)units), PAGES, smem, st>>>(a);
-  return sa_record_cuda_error(cudaGetLastError());
-}
-
-template <typename E, int D>
-static int launch_score_g(const SelectArgs& a, int64_t units, cudaStream_t st) {
-  if (a.G % 8 == 0) return launch_score<E, D, 8>(a, units, st);
-  if (a.G % 4 == 0) return launch_score<E, D, 4>(a, units, st);
-  if (a.G % 2 == 0) return launch_score<E, D, 2>(a, units, st);
-  return launch_score<E, D, 1>(a, units, st);
-}
-
 template <typename E>
-static int launch_score_d(const SelectArgs& a, int64_t units, int64_t D, cudaStream_t st) {
+static int launch_score(const SelectArgs& a, int64_t units, int64_t D, cudaStream_t st) {
+  // tiles of 64 pages, dealt to at most one resident wave of blocks (four an SM)
+  const int64_t tiles = (a.max_blocks + 63) / 64, wave = 4ll * qkr::sm_count();
+  const dim3 grid((unsigned)std::max<int64_t>(1, std::min(tiles, wave / units)), (unsigned)units);
   switch (D) {
-    case 32: return launch_score_g<E, 32>(a, units, st);
-    case 64: return launch_score_g<E, 64>(a, units, st);
-    case 128: return launch_score_g<E, 128>(a, units, st);
-    default: return launch_score_g<E, 256>(a, units, st);
+    case 32: paged_score_kernel<E, 32><<<grid, 128, 0, st>>>(a); break;
+    case 64: paged_score_kernel<E, 64><<<grid, 128, 0, st>>>(a); break;
+    case 128: paged_score_kernel<E, 128><<<grid, 128, 0, st>>>(a); break;
+    default: paged_score_kernel<E, 256><<<grid, 128, 0, st>>>(a); break;
   }
+  return sa_record_cuda_error(cudaGetLastError());
 }
 
 static int check_cache(int64_t B, int64_t Hkv, int64_t num_blocks, int64_t bs, int64_t max_blocks, int64_t D,
@@ -440,11 +591,11 @@ static int run_choice(SelectArgs& a, const void* q, const void* means, const int
   a.Hkv = (int)Hkv, a.G = (int)(Hq / Hkv), a.bs = (int)bs, a.max_blocks = (int)max_blocks, a.K = (int)K;
   const int64_t units = B * Hkv;
   if (max_blocks > K) {  // else every page is taken
-    const int rc = dtype == SA_BF16 ? launch_score_d<__nv_bfloat16>(a, units, D, st)
-                                    : launch_score_d<__half>(a, units, D, st);
+    const int rc = dtype == SA_BF16 ? launch_score<__nv_bfloat16>(a, units, D, st) : launch_score<__half>(a, units, D, st);
     if (rc != SA_OK) return rc;
   }
-  paged_choose_kernel<<<(unsigned)units, kSelThreads, 0, st>>>(a);
+  if (max_blocks <= CT * kKeep) paged_choose_kernel<CT><<<(unsigned)units, CT, 0, st>>>(a);
+  else paged_choose_kernel<1024><<<(unsigned)units, 1024, 0, st>>>(a);
   return sa_record_cuda_error(cudaGetLastError());
 }
 
