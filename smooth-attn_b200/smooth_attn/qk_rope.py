@@ -210,6 +210,8 @@ class _Plan:
         self.fwd = (self.pos_bytes, self.pos_sb, self.rows, *dims, *ins, *out, *flags)
         self.dims, self.ins, self.out, self.flags = dims, ins, out, flags
         self.device = q.get_device()
+        self.bwd = {}  # by the strides of the two incoming gradients: theirs as the C ABI takes them
+        self.ws_bytes = None
 
     def run(self, q, k, cos, sin, q_weight, k_weight, positions):
         """(q_out, k_out), or None where a base is off a 16-byte boundary."""
@@ -225,6 +227,36 @@ class _Plan:
                 return None
             _lib.check(st, "sa_qk_norm_rope")
         return q_out, k_out
+
+
+    def run_bwd(self, q, k, dq_out, dk_out, q_weight, k_weight, cos, sin, positions, need_dw):
+        """_bwd_direct, or None where a gradient needs a copy or a base is off a 16-byte boundary."""
+        key = (dq_out.stride(), dk_out.stride())
+        strides = self.bwd.get(key)
+        if strides is None:
+            if not (_stride_ok(dq_out) and _stride_ok(dk_out)):
+                return None
+            strides = _keep(self.bwd, key, (_strides(dq_out), _strides(dk_out)))
+        dq, dk = torch.empty_like(q), torch.empty_like(k)
+        dwq = torch.empty_like(q_weight) if need_dw and q_weight is not None else None
+        dwk = torch.empty_like(k_weight) if need_dw and k_weight is not None else None
+        ws, nbytes = None, 0
+        if dwq is not None or dwk is not None:
+            nbytes = _bwd_workspace(self.dims[4], self.device)
+            ws = q.new_empty(nbytes, dtype=torch.uint8)
+        st = _lib.load().sa_qk_norm_rope_bwd(
+            q.data_ptr(), k.data_ptr(), dq_out.data_ptr(), dk_out.data_ptr(), dq.data_ptr(), dk.data_ptr(),
+            None if q_weight is None else q_weight.data_ptr(), None if k_weight is None else k_weight.data_ptr(), self.w,
+            None if dwq is None else dwq.data_ptr(), None if dwk is None else dwk.data_ptr(),
+            None if cos is None else cos.data_ptr(), None if sin is None else sin.data_ptr(), self.cs,
+            None if positions is None else positions.data_ptr(), self.pos_bytes, self.pos_sb, self.rows,
+            None if ws is None else ws.data_ptr(), nbytes, *self.dims, *self.ins, *strides, *self.out, *self.flags,
+            torch._C._cuda_getCurrentRawStream(self.device))
+        if st != _lib.SA_OK:
+            if st == _lib.SA_ERR_ALIGN:
+                return None
+            _lib.check(st, "sa_qk_norm_rope_bwd")
+        return dq, dk, dwq, dwk
 
 
 def _plan_of(q, k, cos, sin, q_weight, k_weight, eps, positions):
@@ -274,24 +306,15 @@ def _bwd_workspace(D, device_index):
     return n
 
 
-def _bwd_direct(q, k, dq_out, dk_out, q_weight, k_weight, cos, sin, positions, eps, need_dw, plan=None):
-    """(dq, dk, dq_weight, dk_weight); the last two None without a weight or when not needed.
-    plan: the forward's, for the same tensors (a hook on saved tensors may hand back others)."""
+def _bwd_direct(q, k, dq_out, dk_out, q_weight, k_weight, cos, sin, positions, eps, need_dw):
+    """(dq, dk, dq_weight, dk_weight); the last two None without a weight or when not needed."""
     B, Hq, T, D = q.shape
     Hkv = k.shape[1]
     dq, dk = _like(q), _like(k)
-    dq_out, dk_out = _rows(dq_out), _rows(dk_out)
-    if plan is not None and plan.key == _key_of(q, k, cos, sin, q_weight, k_weight, eps, positions):
-        wq, wk, w_code, cs_code = q_weight, k_weight, plan.w, plan.cs
-        pos, pos_bytes, pos_sb = positions, plan.pos_bytes, plan.pos_sb
-        ins, outs = plan.ins, plan.out
-    else:
-        plan = None
-        q, k = _rows(q), _rows(k)
-        wq, wk, w_code = _weights(q_weight, k_weight)
-        cos, sin, cs_code = _tables(cos, sin)
-        pos, pos_bytes, pos_sb = _positions(positions, T)
-        ins, outs = (_strides(q), _strides(k)), (_strides(dq), _strides(dk))
+    q, k, dq_out, dk_out = (_rows(t) for t in (q, k, dq_out, dk_out))
+    wq, wk, w_code = _weights(q_weight, k_weight)
+    cos, sin, cs_code = _tables(cos, sin)
+    pos, pos_bytes, pos_sb = _positions(positions, T)
     dwq = torch.empty_like(wq) if need_dw and wq is not None else None
     dwk = torch.empty_like(wk) if need_dw and wk is not None else None
     with K._on(q.device):
@@ -303,10 +326,9 @@ def _bwd_direct(q, k, dq_out, dk_out, q_weight, k_weight, cos, sin, positions, e
             K._ptr(q), K._ptr(k), K._ptr(dq_out), K._ptr(dk_out), K._ptr(dq), K._ptr(dk), K._ptr(wq), K._ptr(wk),
             w_code, K._ptr(dwq), K._ptr(dwk), K._ptr(cos), K._ptr(sin), cs_code, K._ptr(pos), pos_bytes, pos_sb,
             0 if cos is None else cos.shape[0], K._ptr(ws), nbytes, B, Hq, Hkv, T, D,
-            0 if cos is None else 2 * cos.shape[1], *ins, _strides(dq_out), _strides(dk_out), *outs,
-            0.0 if eps is None else float(eps), int(eps is not None), K._DTYPE_CODE[q.dtype], K._stream(q))
-    if st == _lib.SA_ERR_ALIGN and plan is not None:
-        return _bwd_direct(q, k, dq_out, dk_out, q_weight, k_weight, cos, sin, positions, eps, need_dw)
+            0 if cos is None else 2 * cos.shape[1], _strides(q), _strides(k), _strides(dq_out), _strides(dk_out),
+            _strides(dq), _strides(dk), 0.0 if eps is None else float(eps), int(eps is not None),
+            K._DTYPE_CODE[q.dtype], K._stream(q))
     _lib.check(st, "sa_qk_norm_rope_bwd")
     if dwq is not None and dwq.dtype != q_weight.dtype:
         dwq = dwq.to(q_weight.dtype)
@@ -338,8 +360,13 @@ class _QkNormRopeFn(torch.autograd.Function):
             dq, dk, dwq, dwk = K._ops().qk_norm_rope_bwd(q, k, dq_out, dk_out, wq, wk, cos, sin, positions, ctx.eps,
                                                          need_dw)
         else:
-            dq, dk, dwq, dwk = _bwd_direct(q, k, dq_out, dk_out, wq, wk, cos, sin, positions, ctx.eps, need_dw,
-                                           ctx.plan)
+            res, plan = None, ctx.plan
+            # (a hook on saved tensors may hand back others than the forward's)
+            if (plan is not None and plan.device == torch.cuda.current_device()
+                    and plan.key == _key_of(q, k, cos, sin, wq, wk, ctx.eps, positions)):
+                res = plan.run_bwd(q, k, dq_out, dk_out, wq, wk, cos, sin, positions, need_dw)
+            dq, dk, dwq, dwk = res if res is not None else _bwd_direct(q, k, dq_out, dk_out, wq, wk, cos, sin,
+                                                                      positions, ctx.eps, need_dw)
         return (dq, dk, dwq if need[2] else None, dwk if need[3] else None, None, None, None, None, None)
 
 
