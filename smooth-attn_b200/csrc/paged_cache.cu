@@ -39,11 +39,13 @@ namespace pgc {
 static __device__ unsigned g_bad_entries;  // slots past the cache, positions past the tables, a pool given too much back
 
 constexpr int kThreads = 512;
-constexpr int kMaxRequests = 16384;
+constexpr int kMaxRequests = 16384;  // 12 bytes each of shared memory
 
-// Exclusive scan of one int64 per thread over the block; returns the sum before this thread, total in *all.
+// Exclusive scan of one int64 per thread over the block; returns the sum before
+// this thread, the total in *all.  warp_sums: used by no other scan of the block.
 __device__ __forceinline__ int64_t block_scan(int64_t v, int64_t* all, int64_t* warp_sums) {
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, nw = blockDim.x >> 5;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  constexpr int NW = kThreads / 32;
   int64_t inc = v;
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
@@ -52,20 +54,15 @@ __device__ __forceinline__ int64_t block_scan(int64_t v, int64_t* all, int64_t* 
   }
   if (lane == 31) warp_sums[warp] = inc;
   __syncthreads();
-  if (warp == 0) {
-    int64_t s = lane < nw ? warp_sums[lane] : 0;
+  int64_t s = lane < NW ? warp_sums[lane] : 0;  // every warp scans the warps' sums for itself
 #pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const int64_t u = __shfl_up_sync(0xffffffffu, s, o);
-      if (lane >= o) s += u;
-    }
-    if (lane < nw) warp_sums[lane] = s;
+  for (int o = 1; o < NW; o <<= 1) {
+    const int64_t u = __shfl_up_sync(0xffffffffu, s, o);
+    if (lane >= o) s += u;
   }
-  __syncthreads();
-  const int64_t before = warp ? warp_sums[warp - 1] : 0;
-  *all = warp_sums[nw - 1];
-  __syncthreads();
-  return before + inc - v;
+  const int64_t before = __shfl_sync(0xffffffffu, s, warp ? warp - 1 : 0);
+  *all = __shfl_sync(0xffffffffu, s, NW - 1);
+  return (warp ? before : 0) + inc - v;
 }
 
 struct AssignArgs {
@@ -82,81 +79,118 @@ struct AssignArgs {
   int32_t* head_out;
   int64_t num_free;
   int B, N, max_blocks, bs;
+  qkr::FastDiv by_bs;
 };
 
-__global__ void __launch_bounds__(kThreads) paged_assign_kernel(AssignArgs a) {
+// V neighbouring tokens a thread: 4 share one search and are stored 16 bytes at a
+// time; 1 where there are so few tokens that each should have a thread of its own
+// (64 tokens of 64 requests: 4.3 us, 5.9 us with 4; a million tokens: see paged_assign).
+template <int V>
+__global__ void __launch_bounds__(kThreads, 2) paged_assign_kernel(AssignArgs a) {
   extern __shared__ int32_t sm[];  // cu[B + 1], at[B], fits[B]
-  __shared__ int64_t warp_sums[32];
+  __shared__ int64_t warp_sums[2][kThreads / 32];
   int32_t* cu = sm;
   int32_t* at = cu + a.B + 1;
   int32_t* fits = at + a.B;
-  const int64_t cap = (int64_t)a.max_blocks * a.bs;
+  const int64_t cap = (int64_t)a.max_blocks * a.bs;  // at most 2^30
   const int per = (a.B + kThreads - 1) / kThreads;
   const int b0 = min(a.B, (int)threadIdx.x * per), b1 = min(a.B, b0 + per);
-  auto held_tokens = [&](int b) { return max((int64_t)0, min(cap, (int64_t)a.ctx[b])); };
+  auto ctx_of = [&](int b) { return (int)max((int64_t)0, min(cap, (int64_t)__ldg(a.ctx + b))); };
+  auto pages = [&](int64_t tokens) { return (int64_t)a.by_bs.div((uint32_t)(tokens + a.bs - 1)); };
 
+  const int64_t head = max((int64_t)0, min(a.num_free, (int64_t)__ldg(a.head)));
   int64_t sum = 0, all;
-  for (int b = b0; b < b1; ++b) sum += max(0, a.fresh[b]);
-  int64_t run = block_scan(sum, &all, warp_sums);
+  for (int b = b0; b < b1; ++b) {
+    const int n = max(0, __ldg(a.fresh + b));
+    at[b] = n;
+    sum += n;
+  }
+  int64_t run = block_scan(sum, &all, warp_sums[0]);
   sum = 0;
   for (int b = b0; b < b1; ++b) {
-    const int64_t lo = min((int64_t)a.N, run);
-    run += max(0, a.fresh[b]);
-    const int64_t ctx = held_tokens(b);
+    const int64_t lo = min((int64_t)a.N, run), ctx = ctx_of(b);
+    run += at[b];
     const int64_t want = min(min((int64_t)a.N, run) - lo, cap - ctx);
     cu[b] = (int32_t)lo;
     fits[b] = (int32_t)want;
-    sum += (ctx + want + a.bs - 1) / a.bs - (ctx + a.bs - 1) / a.bs;
+    sum += pages(ctx + want) - pages(ctx);
   }
   if (threadIdx.x == 0) cu[a.B] = (int32_t)min((int64_t)a.N, all);
-  const int64_t head = max((int64_t)0, min(a.num_free, (int64_t)*a.head));
-  run = head + block_scan(sum, &all, warp_sums);
+  run = head + block_scan(sum, &all, warp_sums[1]);
   for (int b = b0; b < b1; ++b) {
-    const int64_t ctx = held_tokens(b), held = (ctx + a.bs - 1) / a.bs;
-    const int64_t need = (ctx + fits[b] + a.bs - 1) / a.bs - held;
+    const int64_t ctx = ctx_of(b), held = pages(ctx), need = pages(ctx + fits[b]) - held;
     const int64_t have = max((int64_t)0, min(need, a.num_free - run));
     fits[b] = (int32_t)min((int64_t)fits[b], (held + have) * a.bs - ctx);
-    at[b] = (int32_t)min(run, a.num_free);
+    at[b] = (int32_t)(min(run, a.num_free) - held);  // the list's entry for page 0, were it in it
     run += need;
   }
   __syncthreads();
   if (blockIdx.x == 0) {
     for (int b = threadIdx.x; b <= a.B; b += kThreads) {
       a.cu[b] = cu[b];
-      if (b < a.B) a.ctx_out[b] = (int32_t)(held_tokens(b) + fits[b]);
+      if (b < a.B) a.ctx_out[b] = ctx_of(b) + fits[b];
     }
     if (threadIdx.x == 0) *a.head_out = (int32_t)min(head + all, a.num_free);
   }
 
-  for (int64_t i = (int64_t)blockIdx.x * kThreads + threadIdx.x; i < a.N; i += (int64_t)gridDim.x * kThreads) {
-    int64_t slot = -1;
-    int pos = 0;
-    if (i < cu[a.B]) {
-      int lo = 0, hi = a.B;  // the last b with cu[b] <= i: the one that holds token i (empty ones lie before it)
-      while (hi - lo > 1) {
-        const int mid = (lo + hi) >> 1;
-        if (cu[mid] <= i) lo = mid;
-        else hi = mid;
-      }
-      const int off = (int)i - cu[lo];
-      if (off < fits[lo]) {
-        const int ctx = (int)held_tokens(lo);
-        const int held = (ctx + a.bs - 1) / a.bs;
-        pos = ctx + off;
-        const int pi = pos / a.bs;
-        int page;
-        if (!SA_DCHECK(pi < a.max_blocks)) continue;
-        if (pi < held) {
-          page = a.table[lo * a.ld + pi];
-        } else {
-          page = a.pool[at[lo] + pi - held];
-          if (pos == pi * a.bs) a.table[lo * a.ld + pi] = page;
+  const int total = cu[a.B];
+  for (int64_t i0 = ((int64_t)blockIdx.x * kThreads + threadIdx.x) * V; i0 < a.N;
+       i0 += (int64_t)gridDim.x * kThreads * V) {
+    long long slot[V];
+    int pos[V];
+    int b = 0, end = 0, ctx = 0, seen = -1, page = 0;  // the request, where it ends, the last page looked up
+    bool found = false;
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+      const int i = (int)i0 + j;
+      slot[j] = -1;
+      pos[j] = 0;
+      if (i >= total) continue;
+      if (!found || i >= end) {  // the last b with cu[b] <= i: the one that holds token i (empty ones lie before it)
+        int lo = found ? b : 0, hi = a.B;
+        while (hi - lo > 1) {
+          const int mid = (lo + hi) >> 1;
+          if (cu[mid] <= i) lo = mid;
+          else hi = mid;
         }
-        slot = page < 0 ? -1 : (int64_t)page * a.bs + (pos - pi * a.bs);
+        b = lo;
+        end = cu[b + 1];
+        ctx = ctx_of(b);
+        found = true;
+        seen = -1;
+      }
+      const int off = i - cu[b];
+      if (off >= fits[b]) continue;
+      const int p = ctx + off, pi = (int)a.by_bs.div((uint32_t)p);
+      if (!SA_DCHECK(pi < a.max_blocks)) continue;
+      if (pi != seen) {
+        int32_t* entry = a.table + b * a.ld + pi;
+        if (pi * a.bs < ctx) {  // a page that the request held already
+          page = *entry;
+        } else {
+          page = __ldg(a.pool + at[b] + pi);
+          if (p == pi * a.bs) *entry = page;
+        }
+        seen = pi;
+      }
+      pos[j] = p;
+      if (page >= 0) slot[j] = (long long)page * a.bs + (p - pi * a.bs);
+    }
+    if constexpr (V == 4) {
+      if (i0 + 4 <= a.N) {  // (both buffers start on 16 bytes)
+        *reinterpret_cast<int4*>(a.positions + i0) = make_int4(pos[0], pos[1], pos[2], pos[3]);
+        *reinterpret_cast<longlong2*>(a.slots + i0) = make_longlong2(slot[0], slot[1]);
+        *reinterpret_cast<longlong2*>(a.slots + i0 + 2) = make_longlong2(slot[2], slot[3]);
+        continue;
       }
     }
-    a.slots[i] = slot;
-    a.positions[i] = pos;
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+      if (i0 + j < a.N) {
+        a.positions[i0 + j] = pos[j];
+        a.slots[i0 + j] = slot[j];
+      }
+    }
   }
 }
 
@@ -177,7 +211,7 @@ struct ReleaseArgs {
 // request's pages to the list's entries in front of its head.
 __global__ void __launch_bounds__(kThreads) paged_release_kernel(ReleaseArgs a) {
   extern __shared__ int64_t off[];  // [B]
-  __shared__ int64_t warp_sums[32];
+  __shared__ int64_t warp_sums[kThreads / 32];
   const int64_t cap = (int64_t)a.max_blocks * a.bs;
   const int per = (a.B + kThreads - 1) / kThreads;
   const int b0 = min(a.B, (int)threadIdx.x * per), b1 = min(a.B, b0 + per);
@@ -399,14 +433,23 @@ extern "C" int sa_paged_assign_slots(int32_t* block_table, int64_t table_stride,
   if (B > 0 && (!block_table || !context_lens || !new_lens || !context_lens_out)) return SA_ERR_ARG;
   if (num_free > 0 && !free_pages) return SA_ERR_ARG;
   if (num_tokens > 0 && (!slots || !positions)) return SA_ERR_ARG;
+  if (!sa::qkr::al16(slots) || !sa::qkr::al16(positions)) return SA_ERR_ALIGN;
   AssignArgs a{block_table, table_stride, context_lens, new_lens, free_pages, free_head,
                reinterpret_cast<long long*>(slots), positions, cu_seqlens, context_lens_out, free_head_out, num_free,
-               (int)B, (int)num_tokens, (int)max_blocks, (int)block_size};
+               (int)B, (int)num_tokens, (int)max_blocks, (int)block_size,
+               sa::qkr::FastDiv((uint32_t)block_size)};
   const size_t smem = (3 * (size_t)B + 1) * 4;
-  const int orc = opt_in(paged_assign_kernel, smem);
+  // one token a thread where half a wave (two blocks an SM) holds them, else four in equal rounds
+  const int64_t wave = 2ll * sm_count();
+  const bool few = num_tokens <= wave * kThreads / 2;
+  const int64_t each = few ? kThreads : 4 * kThreads;
+  const int64_t tiles = std::max<int64_t>(1, (num_tokens + each - 1) / each), rounds = (tiles + wave - 1) / wave;
+  const unsigned blocks = (unsigned)((tiles + rounds - 1) / rounds);
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  const int orc = few ? opt_in(paged_assign_kernel<1>, smem) : opt_in(paged_assign_kernel<4>, smem);
   if (orc != SA_OK) return orc;
-  const int64_t blocks = std::max<int64_t>(1, std::min<int64_t>((num_tokens + 4 * kThreads - 1) / (4 * kThreads), 2ll * sm_count()));
-  paged_assign_kernel<<<(unsigned)blocks, kThreads, smem, static_cast<cudaStream_t>(stream)>>>(a);
+  if (few) paged_assign_kernel<1><<<blocks, kThreads, smem, st>>>(a);
+  else paged_assign_kernel<4><<<blocks, kThreads, smem, st>>>(a);
   return sa_record_cuda_error(cudaGetLastError());
 }
 

@@ -44,14 +44,13 @@ class PagedSlots(NamedTuple):
 _PLANS: dict = {}
 
 
-def _key(what, tensors, *rest):
-    """A call's signature, or None where an argument is no tensor or not hashable (the checks then say so)."""
+def _plan(what, rest, tensors):
+    """(key, plan) of a call; (None, None) where an argument is no tensor (the checks then say so)."""
     try:
-        key = (what, *rest, *[None if t is None else (t.shape, t.stride(), t.dtype, t.get_device()) for t in tensors])
-        hash(key)
+        key = (what, rest, *[None if t is None else (t.shape, t.stride(), t.dtype, t.get_device()) for t in tensors])
+        return key, _PLANS.get(key)
     except (AttributeError, TypeError):
-        return None
-    return key
+        return None, None
 
 
 def _same_device(like, **tensors):
@@ -115,11 +114,10 @@ def paged_assign_slots(block_table, context_lens, new_lens, free_pages, free_hea
     context_lens, new_lens: [B], at most 16384 requests.  One launch, no host synchronisation.
     """
     num_tokens, block_size = int(num_tokens), int(block_size)
-    traced = K._tracing(block_table)
+    traced = R._traced(block_table)
     key = None
     if not traced:
-        key = _key("slots", (block_table, context_lens, new_lens, free_pages, free_head), num_tokens, block_size)
-        plan = _PLANS.get(key)
+        key, plan = _plan("slots", (num_tokens, block_size), (block_table, context_lens, new_lens, free_pages, free_head))
         if plan is not None and plan[0] == torch.cuda.current_device():
             return _assign_call(plan, block_table, context_lens, new_lens, free_pages, free_head)
     given = (context_lens, new_lens, free_pages, free_head)
@@ -178,11 +176,10 @@ def paged_release_pages(block_table, context_lens, done, free_pages, free_head, 
     is reported by ``sa_device_status``.  done: bool [B].
     """
     block_size = int(block_size)
-    traced = K._tracing(block_table)
+    traced = R._traced(block_table)
     key = None
     if not traced:
-        key = _key("release", (block_table, context_lens, done, free_pages, free_head), block_size)
-        plan = _PLANS.get(key)
+        key, plan = _plan("release", block_size, (block_table, context_lens, done, free_pages, free_head))
         if plan is not None and plan[0] == torch.cuda.current_device():
             return _release_call(plan, block_table, context_lens, done, free_pages, free_head)
     given = (context_lens, done, free_head)
@@ -254,11 +251,10 @@ def qk_norm_rope_paged_append(q, k, v, k_cache, v_cache, slot_mapping, cos=None,
     takes for one token of each of N sequences.  Forward only.
     """
     eps = None if eps is None else float(eps)
-    traced = K._tracing(q, k, k_cache)
+    traced = R._traced(q)
     key = plan = None
     if not traced:
-        key = _key("append", (q, k, v, k_cache, v_cache, slot_mapping, cos, sin, positions, q_weight, k_weight), eps)
-        plan = _PLANS.get(key)
+        key, plan = _plan("append", eps, (q, k, v, k_cache, v_cache, slot_mapping, cos, sin, positions, q_weight, k_weight))
     if plan is None:
         _check_append(q, k, v, k_cache, v_cache, slot_mapping, cos, sin, positions, q_weight, k_weight, eps)
     if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):
@@ -383,11 +379,10 @@ def paged_key_means(key_means, k_cache, block_table, context_lens, *, start_lens
     are left as they are.  A block_table entry outside the cache is skipped and reported by
     ``sa_device_status``.  Returns key_means.
     """
-    traced = K._tracing(k_cache, key_means)
+    traced = R._traced(k_cache)
     key = None
     if not traced:
-        key = _key("means", (key_means, k_cache, block_table, context_lens, start_lens))
-        plan = _PLANS.get(key)
+        key, plan = _plan("means", None, (key_means, k_cache, block_table, context_lens, start_lens))
         if plan is not None and plan[0] == torch.cuda.current_device():
             return _means_call(plan, key_means, k_cache, block_table, context_lens, start_lens)
     given = (block_table, context_lens, start_lens)
@@ -470,7 +465,7 @@ def sp2norm_paged_select(q, key_means, block_table, context_lens, num_pages, *, 
     num_pages, block_size = int(num_pages), int(block_size)
     block_table, context_lens, n = _check_query(q, key_means, block_table, context_lens, num_pages, block_size)
     scale = 1.0 / math.sqrt(q.shape[3]) if scale is None else float(scale)
-    if K._tracing(q, key_means):
+    if R._traced(q):
         return K._ops().paged_select(q, key_means, block_table, context_lens, n, scale, block_size)
     return _select_direct(q, key_means, block_table, context_lens, n, scale, block_size)
 
@@ -510,13 +505,12 @@ def sp2norm_sparse_paged_attention(q, k_cache, v_cache, key_means, block_table, 
     (int32 [B, H_kv, min(num_pages, max_blocks)], as ``sp2norm_paged_select``).
     """
     num_pages, block_size, scale = int(num_pages), int(block_size), None if scale is None else float(scale)
-    traced = K._tracing(q, k_cache)
+    traced = R._traced(q)
     key = None
     if not traced:
         # (the decode kernel, and so the workspace, is chosen by this variable too)
-        key = _key("sparse", (q, k_cache, v_cache, key_means, block_table, context_lens), num_pages, block_size, scale,
-                   os.environ.get("SA_PAGED_DECODE_KERNEL"))
-        plan = _PLANS.get(key)
+        key, plan = _plan("sparse", (num_pages, block_size, scale, os.environ.get("SA_PAGED_DECODE_KERNEL")),
+                          (q, k_cache, v_cache, key_means, block_table, context_lens))
         if plan is not None and plan[0] == torch.cuda.current_device():
             out, pages = _sparse_call(plan, q, k_cache, v_cache, key_means, block_table, context_lens, return_pages)
             return (out, pages) if return_pages else out

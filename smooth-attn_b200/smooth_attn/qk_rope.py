@@ -23,6 +23,11 @@ QK_MAX_HEAD_DIM = 256  # the rows are split over at most 16 lanes of 16 channels
 _POS_BYTES = {torch.int32: 4, torch.int64: 8}
 
 
+def _traced(t):
+    """Whether a call runs under a tracer (``K._tracing`` of its first tensor, without a generator per call)."""
+    return (torch.compiler.is_compiling() or K._get_proxy_mode() is not None or isinstance(t, K._TRACED_TYPES))
+
+
 def _check_weight(w, name, D, like):
     if w is None:
         return
@@ -346,7 +351,7 @@ class _QkNormRopeFn(torch.autograd.Function):
         ctx.plan = plan if res is not None else None
         if res is not None:
             return res
-        if K._tracing(q, k):
+        if _traced(q):
             return K._ops().qk_norm_rope(q, k, q_weight, k_weight, cos, sin, positions, eps)
         return _fwd_direct(q, k, q_weight, k_weight, cos, sin, positions, eps)
 
@@ -356,7 +361,7 @@ class _QkNormRopeFn(torch.autograd.Function):
         q, k, wq, wk, cos, sin, positions = ctx.saved_tensors
         need = ctx.needs_input_grad
         need_dw = need[2] or need[3]
-        if K._tracing(q, k, dq_out, dk_out):
+        if _traced(dq_out):
             dq, dk, dwq, dwk = K._ops().qk_norm_rope_bwd(q, k, dq_out, dk_out, wq, wk, cos, sin, positions, ctx.eps,
                                                          need_dw)
         else:
@@ -389,7 +394,7 @@ def qk_norm_rope(q, k, cos=None, sin=None, *, q_weight=None, k_weight=None, eps=
     summed in fp32 in a fixed order, bitwise the same from run to run.  No gradient for cos / sin.
     """
     eps = None if eps is None else float(eps)
-    traced = K._tracing(q, k)
+    traced = _traced(q)
     if traced:
         _check_qk(q, k, cos, sin, q_weight, k_weight, eps, positions)
         plan = None
