@@ -356,8 +356,14 @@ class _QkNormRopeFn(torch.autograd.Function):
         return _fwd_direct(q, k, q_weight, k_weight, cos, sin, positions, eps)
 
     @staticmethod
-    @once_differentiable
     def backward(ctx, dq_out, dk_out):
+        # (the wrapper costs microseconds and matters only where a graph of the gradient is being built)
+        if torch.is_grad_enabled():
+            return _grads_once(ctx, dq_out, dk_out)
+        return _QkNormRopeFn._grads(ctx, dq_out, dk_out)
+
+    @staticmethod
+    def _grads(ctx, dq_out, dk_out):
         q, k, wq, wk, cos, sin, positions = ctx.saved_tensors
         need = ctx.needs_input_grad
         need_dw = need[2] or need[3]
@@ -373,6 +379,9 @@ class _QkNormRopeFn(torch.autograd.Function):
             dq, dk, dwq, dwk = res if res is not None else _bwd_direct(q, k, dq_out, dk_out, wq, wk, cos, sin,
                                                                       positions, ctx.eps, need_dw)
         return (dq, dk, dwq if need[2] else None, dwk if need[3] else None, None, None, None, None, None)
+
+
+_grads_once = once_differentiable(_QkNormRopeFn._grads)
 
 
 def qk_norm_rope(q, k, cos=None, sin=None, *, q_weight=None, k_weight=None, eps=1e-6, positions=None):

@@ -186,6 +186,82 @@ def test_gradient_of_a_larger_problem_repeats_bitwise(B, Hq, Hkv, T, D, R, dt, p
         _check(o, *_ref64(x, w, cos, sin, full, eps))
 
 
+def test_offsets_past_32_bits():
+    """2.4 billion elements of q: rows at both ends against the formula."""
+    T, D = 590_001, 128
+    q = torch.zeros(1, T, 32, D, device=CUDA, dtype=torch.bfloat16).transpose(1, 2)
+    k = torch.zeros(1, 1, T, D, device=CUDA, dtype=torch.bfloat16)
+    ends = torch.tensor([0, 1, T // 2, T - 2, T - 1], device=CUDA)
+    q[:, :, ends] = randn((1, 32, 5, D), 1, torch.bfloat16, CUDA)
+    k[:, :, ends] = randn((1, 1, 5, D), 2, torch.bfloat16, CUDA)
+    cos, sin = _angles(T, D, torch.bfloat16)
+    q.requires_grad_(True)
+    yq, yk = sa.qk_norm_rope(q, k, cos, sin)
+    qe, ke = q.detach()[:, :, ends], k[:, :, ends]
+    _check(yq.detach()[:, :, ends], *_ref64(qe, None, cos.float(), sin.float(), ends[None], 1e-6))
+    _check(yk[:, :, ends], *_ref64(ke, None, cos.float(), sin.float(), ends[None], 1e-6))
+    assert yq.count_nonzero() == yq[:, :, ends].count_nonzero()
+    (dq,) = torch.autograd.grad(yq, q, torch.ones_like(yq))
+    ref = _ref64(qe, None, cos.float(), sin.float(), ends[None], 1e-6, torch.ones_like(qe))
+    _check(dq[:, :, ends], ref[2], ref[3])
+
+
+def test_bases_off_a_boundary_and_mixed_weight_types():
+    """Contiguous views that start off 16 bytes; weights of two types, each with its own gradient type."""
+    def off(t):
+        b = torch.empty(t.numel() + 1, device=CUDA, dtype=t.dtype)
+        return b[1:].view(t.shape).copy_(t)
+
+    q, k, dq, dk, wq, wk, cos, sin, pos, full, eps = _make((2, 4, 2, 9, 64, 64, torch.bfloat16, torch.bfloat16, True,
+                                                            "batch64"))
+    want = [t.clone() for t in (q, k, wq, wk)]
+    for base, mixed in ((True, False), (False, True), (True, True)):
+        ins = [off(t) if base else t.clone() for t in want]
+        if mixed:
+            ins[2] = off(want[2].float())
+        ins = [t.detach().requires_grad_(True) for t in ins]
+        c, s = (off(cos), off(sin)) if base else (cos, sin)
+        y = sa.qk_norm_rope(ins[0], ins[1], c, s, q_weight=ins[2], k_weight=ins[3], positions=off(pos) if base else pos)
+        g = torch.autograd.grad(y, ins, (off(dq), off(dk)) if base else (dq, dk))
+        assert g[2].dtype == ins[2].dtype and g[3].dtype == torch.bfloat16
+        for x, w, o, dx, dw, dy in ((q, wq, y[0], g[0], g[2], dq), (k, wk, y[1], g[1], g[3], dk)):
+            ref = _ref64(x, w, cos, sin, full, eps, dy)
+            _check(o.detach(), ref[0], ref[1])
+            _check(dx, ref[2], ref[3])
+            # (bf16 weights beside fp32 ones are taken as fp32: one more rounding to their gradient's type)
+            _check(dw, ref[4], ref[5] + 4 * U * ref[4].abs())
+
+
+def test_hooks_on_saved_tensors():
+    """Saved tensors that come back in another layout (an offload) give the same gradients."""
+    q, k, dq, dk, wq, wk, cos, sin, pos, full, eps = _make((2, 8, 2, 33, 64, 64, torch.bfloat16, torch.float32, True,
+                                                            "batch32"))
+    q = q.transpose(1, 2).contiguous().transpose(1, 2)
+
+    def grads(hooked):
+        ins = [t.detach().clone().requires_grad_(True) for t in (q, k, wq, wk)]
+        pack = torch.autograd.graph.saved_tensors_hooks(lambda t: t.contiguous().cpu(), lambda t: t.to(CUDA))
+        if hooked:
+            with pack:
+                y = sa.qk_norm_rope(ins[0], ins[1], cos, sin, q_weight=ins[2], k_weight=ins[3], positions=pos)
+        else:
+            y = sa.qk_norm_rope(ins[0], ins[1], cos, sin, q_weight=ins[2], k_weight=ins[3], positions=pos)
+        return torch.autograd.grad(y, ins, (dq, dk))
+
+    assert all(torch.equal(a, b) for a, b in zip(grads(False), grads(True)))
+
+
+def test_a_changed_input_is_noticed():
+    """The backward reads the forward's inputs: changing one in between is an error, as for torch's own operators."""
+    q, k, *_ = _make(CASES[1])
+    x = q.clone().requires_grad_(True)
+    held = x * 1
+    y, _ = sa.qk_norm_rope(held, k)
+    held.add_(1)
+    with pytest.raises(RuntimeError, match="modified by an inplace"):
+        y.sum().backward()
+
+
 def test_gradient_against_differences():
     """fp32: the gradient along a direction against a central difference of the kernel's own forward."""
     case = (1, 2, 1, 9, 64, 32, torch.float32, torch.float32, True, "none")
