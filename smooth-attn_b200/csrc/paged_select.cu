@@ -191,18 +191,33 @@ __global__ void __launch_bounds__(128, 4) paged_score_kernel(SelectArgs a) {
   constexpr bool kAhead = P <= 4;  // the next tile's rows are asked for before this one's product (at D = 256 no room)
   __shared__ double qs[D / 4][32];
   const int u = blockIdx.y, b = u / a.Hkv, h = u - b * a.Hkv;
-  const Seq s = seq_of(a, b);
-  const int m = s.n - 1;                            // candidates: all but the last page
-  if (m <= a.K - 1 || (int)blockIdx.x * 64 >= m) return;  // all of them are taken: nothing to score
   const int lane = threadIdx.x & 31, c = lane & 3, step = gridDim.x * 64;
   int p0 = blockIdx.x * 64 + (threadIdx.x >> 5) * 16 + (lane >> 2);
   const int32_t* bt = a.bt + (int64_t)b * a.max_blocks;
-  auto load = [&](uint4 (&x)[2][P], int at) {
-    int page[2];
+  // the first tile's ids and the queries are asked for beside the length, not after it
+  int page[2];
+  auto ids = [&](int at, int end) {
 #pragma unroll
-    for (int r = 0; r < 2; ++r) page[r] = at + 8 * r < m ? __ldg(bt + at + 8 * r) : 0;
+    for (int r = 0; r < 2; ++r) page[r] = at + 8 * r < end ? __ldg(bt + at + 8 * r) : 0;
+  };
+  auto load_q = [&](int g0, uint4 (&v)[(D + 127) / 128]) {
+    const uint4* q = reinterpret_cast<const uint4*>(static_cast<const E*>(a.q) + ((int64_t)u * a.G + g0) * D);
+#pragma unroll
+    for (int j = 0; j < (D + 127) / 128; ++j) {  // 8 heads of D / 8 pieces
+      const int i = threadIdx.x + j * 128;
+      v[j] = i < D && i / (D / 8) < a.G - g0 ? __ldg(q + i) : make_uint4(0, 0, 0, 0);
+    }
+  };
+  uint4 qv[(D + 127) / 128];
+  ids(p0, a.max_blocks);
+  load_q(0, qv);
+  const Seq s = seq_of(a, b);
+  const int m = s.n - 1;                            // candidates: all but the last page
+  if (m <= a.K - 1 || (int)blockIdx.x * 64 >= m) return;  // all of them are taken: nothing to score
+  auto load = [&](uint4 (&x)[2][P], int at) {
 #pragma unroll
     for (int r = 0; r < 2; ++r) {
+      if (at + 8 * r >= m) page[r] = 0;  // (an entry behind the context says nothing)
       if (page[r] < 0 || page[r] >= a.num_blocks) {
         if (c == 0 && h == 0) atomicAdd(&g_bad_pages, 1u);
         page[r] = 0;
@@ -215,25 +230,27 @@ __global__ void __launch_bounds__(128, 4) paged_score_kernel(SelectArgs a) {
   };
   uint4 x[2][P];
   load(x, p0);
+  ids(p0 + step, m);
   for (int t0 = blockIdx.x * 64; t0 < m; t0 += step, p0 += step) {
     uint4 y[2][kAhead ? P : 1];
     if constexpr (kAhead) {
-      if (t0 + step < m) load(y, p0 + step);
+      if (t0 + step < m) {
+        load(y, p0 + step);
+        ids(p0 + 2 * step, m);
+      }
     }
     double score[2] = {0.0, 0.0};
     for (int g0 = 0; g0 < a.G; g0 += 8) {
       const int heads = min(8, a.G - g0);
       if (a.G > 8 || t0 < step) {  // one group of heads stays in place
         if (g0 || t0 >= step) __syncthreads();  // the last heads' queries have been read
-        const uint4* q = reinterpret_cast<const uint4*>(static_cast<const E*>(a.q) + ((int64_t)u * a.G + g0) * D);
+        if (g0 || t0 >= step) load_q(g0, qv);
 #pragma unroll
-        for (int i = threadIdx.x; i < D; i += 128) {  // 8 heads of D / 8 pieces
-          const int g = i / (D / 8), piece = i % (D / 8);
-          float f[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-          if (g < heads) {
-            const uint4 v = __ldg(q + i);
-            unpack<E, 8>(&v, f);
-          }
+        for (int j = 0; j < (D + 127) / 128; ++j) {
+          const int i = threadIdx.x + j * 128, g = i / (D / 8), piece = i % (D / 8);
+          if (i >= D) break;
+          float f[8];
+          unpack<E, 8>(&qv[j], f);
 #pragma unroll
           for (int e = 0; e < 8; ++e) qs[(piece / 4) * 8 + e][g * 4 + piece % 4] = (double)f[e];
         }
@@ -286,7 +303,10 @@ __global__ void __launch_bounds__(128, 4) paged_score_kernel(SelectArgs a) {
 #pragma unroll
         for (int i = 0; i < P; ++i) x[r][i] = y[r][i];
     } else {
-      if (t0 + step < m) load(x, p0 + step);
+      if (t0 + step < m) {
+        load(x, p0 + step);
+        ids(p0 + 2 * step, m);
+      }
     }
   }
 }
@@ -313,14 +333,20 @@ __global__ void __launch_bounds__(kSelThreads) paged_choose_kernel(SelectArgs a)
   const int lane = tid & 31, warp = tid >> 5;
   for (int64_t i = (int64_t)u * kSelThreads + tid; i < a.num_tickets; i += (int64_t)gridDim.x * kSelThreads)
     a.tickets[i] = 0;
-  const Seq s = seq_of(a, b);
-  const int m = s.n - 1, need = min(a.K, s.n) - 1;  // of the m candidates
   const int32_t* bt = a.bt + (int64_t)b * a.max_blocks;
   const unsigned long long* keys = a.keys + (int64_t)u * a.max_blocks;
+  // read beside the length, not after it: what lies behind the candidates is not looked at
+  unsigned long long mine[kKeep];
+#pragma unroll
+  for (int j = 0; j < kKeep; ++j) {
+    const int i = j * kSelThreads + tid;
+    mine[j] = i < a.max_blocks && a.max_blocks > a.K ? keys[i] : 0;
+  }
+  const Seq s = seq_of(a, b);
+  const int m = s.n - 1, need = min(a.K, s.n) - 1;  // of the m candidates
   // keys above hi are chosen, and `rest` of those in [lo, hi], lowest pages first
   unsigned long long lo = 0, hi = ~0ull;
   int rest = need;
-  unsigned long long mine[kKeep];
   const bool kept = m <= kKeep * kSelThreads;
   auto each_key = [&](auto&& f) {
     if (kept) {
@@ -332,11 +358,6 @@ __global__ void __launch_bounds__(kSelThreads) paged_choose_kernel(SelectArgs a)
     }
   };
   if (m > need && need > 0) {
-    if (kept) {
-#pragma unroll
-      for (int j = 0; j < kKeep; ++j)
-        if (j * kSelThreads + tid < m) mine[j] = keys[j * kSelThreads + tid];
-    }
     unsigned long long mn = ~0ull, mx = 0;
     each_key([&](unsigned long long k) {
       mn = min(mn, k);
@@ -409,6 +430,7 @@ __global__ void __launch_bounds__(kSelThreads) paged_choose_kernel(SelectArgs a)
         if (tid < count) {
           int above = 0, same = 0;
           const unsigned long long k = few[tid];
+#pragma unroll 8
           for (int j = 0; j < count; ++j) {
             above += few[j] > k;
             same += few[j] == k;

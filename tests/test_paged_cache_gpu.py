@@ -414,6 +414,36 @@ def test_choice_of_ties_and_odd_values():
     _attend(out, q, kc, vc, bt, ctx, want, scale)
 
 
+@pytest.mark.parametrize("mb,K", [(500, 40), (3000, 200)])  # scores kept in registers, and read again
+def test_choice_among_pages_that_32_bits_cannot_tell_apart(mb, K):
+    """Mean keys that differ in single last bits of single channels: many real scores inside one fp32 rounding."""
+    q, kc, vc, means, bt = _cache(1, 8, 2, 128, mb, 16, torch.bfloat16, 21)
+    g = torch.Generator().manual_seed(3)
+    for share in (0.05, 0.3, 1.0):  # of the pages: a handful at the border, then all of them
+        near = means.clone()
+        alike = torch.randperm(mb - 1, generator=g)[:max(2, int(share * (mb - 1)))].to(CUDA)
+        score = choose64(q, means, bt, [mb * 16], K, 128 ** -0.5, 16)[0][0][K // 2]  # a page in the middle of the chosen
+        near[bt[0, alike].long()] = means[bt[0, score].long()]
+        for p in alike.tolist()[::2]:
+            c = int(torch.randint(0, 128, (1,), generator=g))
+            bits = near[bt[0, p].long(), :, c].view(torch.int16)
+            near[bt[0, p].long(), :, c] = (bits ^ 1).view(torch.bfloat16)
+        want = choose64(q, near, bt, [mb * 16], K, 128 ** -0.5, 16)
+        pages, _ = sa.sp2norm_paged_select(q, near, bt, _i32([mb * 16]), K)
+        assert pages[0].tolist() == want[0]
+
+
+@pytest.mark.parametrize("scale", [1e-30, 1e-4, 1.0, 1e4, 1e20, 1e30, -0.3])
+def test_choice_at_odd_scales(scale):
+    """Scores that are all alike, far negative, or past fp32: the choice is the 64-bit one."""
+    for dt in (torch.bfloat16, torch.float16):
+        q, kc, vc, means, bt = _cache(2, 6, 2, 64, 700, 16, dt, 22)
+        ctx = [700 * 16 - 5, 3000]
+        want = choose64(q, means, bt, ctx, 33, scale, 16)
+        pages, _ = sa.sp2norm_paged_select(q, means, bt, _i32(ctx), 33, scale=scale)
+        assert pages.tolist() == [[r + [-1] * (33 - len(r)) for r in row] for row in want]
+
+
 def test_choice_of_a_long_context():
     """65536 pages, more than one staging of everything; far negative scores too."""
     q, kc, vc, means, bt = _cache(1, 4, 1, 128, 65536, 16, torch.bfloat16, 5, spread=3.0)
