@@ -376,7 +376,7 @@ template <typename E, int L>
 static int launch_append_l(const AppendArgs& a, const Tables& tb, cudaStream_t st) {
   constexpr int smem = Ring<E, 1, kAppendRing>::kBytesPerThread * kWalkThreads;
   static_assert(smem <= 56 * 1024, "three blocks an SM");
-  const int rc = opt_in(qk_norm_rope_append<E, L>, smem);
+  const int rc = sa_record_cuda_error(opt_in_once<&qk_norm_rope_append<E, L>, smem>());
   if (rc != SA_OK) return rc;
   const unsigned blocks = (unsigned)(a.warps / (kWalkThreads / 32));
   qk_norm_rope_append<E, L><<<blocks, kWalkThreads, smem, st>>>(a, tb);

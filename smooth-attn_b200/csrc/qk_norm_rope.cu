@@ -342,17 +342,12 @@ static int64_t plan(const Side& q, const Side& k, Shape* sh, int per_sm) {
   return blocks;
 }
 
-template <typename F> static int opt_in(F* f, int bytes) {
-  if (bytes <= 48 * 1024) return SA_OK;
-  return sa_record_cuda_error(cudaFuncSetAttribute(f, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes));
-}
-
 template <typename E, int L>
 static int launch_fwd_l(const Side& q, const Side& k, const Tables& tb, const Shape& sh, int64_t blocks,
                         cudaStream_t st) {
   constexpr int smem = Ring<E, 1, kFwdRing<E>>::kBytesPerThread * kWalkThreads;
   static_assert(smem <= 56 * 1024, "four blocks an SM");
-  const int rc = opt_in(qk_norm_rope_fwd<E, L>, smem);
+  const int rc = sa_record_cuda_error(opt_in_once<&qk_norm_rope_fwd<E, L>, smem>());
   if (rc != SA_OK) return rc;
   qk_norm_rope_fwd<E, L><<<(unsigned)blocks, kWalkThreads, smem, st>>>(q, k, tb, sh);
   return sa_record_cuda_error(cudaGetLastError());
@@ -376,7 +371,7 @@ static int launch_bwd_l(const Side& q, const Side& k, const Tables& tb, const Sh
   constexpr int smem = Ring<E, 2, kBwdRing<E>>::kBytesPerThread * kWalkThreads;
   static_assert(smem >= kWalkThreads / 32 * 256 * 4, "the block's dw sums");
   static_assert(smem <= 74 * 1024, "three blocks an SM");
-  const int rc = opt_in(qk_norm_rope_bwd<E, L>, smem);
+  const int rc = sa_record_cuda_error(opt_in_once<&qk_norm_rope_bwd<E, L>, smem>());
   if (rc != SA_OK) return rc;
   qk_norm_rope_bwd<E, L><<<(unsigned)blocks, kWalkThreads, smem, st>>>(q, k, tb, sh, part);
   return sa_record_cuda_error(cudaGetLastError());

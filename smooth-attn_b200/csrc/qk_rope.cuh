@@ -450,6 +450,23 @@ inline int sm_count() {
   return 148;
 }
 
+// Opt-in of a kernel to a fixed `kBytes` of dynamic shared memory on the current
+// device, once per kernel and device (the call costs as much as a third of a launch).
+template <auto kKernel, int kBytes> inline cudaError_t opt_in_once() {
+  if constexpr (kBytes > 48 * 1024) {
+    static std::atomic<uint64_t> done{0};  // bit d: on device d
+    int dev = 0;
+    const cudaError_t g = cudaGetDevice(&dev);
+    if (g != cudaSuccess) return g;
+    const uint64_t bit = dev < 64 ? 1ull << dev : 0;
+    if (done.load(std::memory_order_acquire) & bit) return cudaSuccess;
+    const cudaError_t e = cudaFuncSetAttribute(kKernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kBytes);
+    if (e != cudaSuccess) return e;
+    done.fetch_or(bit, std::memory_order_release);
+  }
+  return cudaSuccess;
+}
+
 // Lanes of a row: the power of two that holds its D / 16 chunk pairs.
 inline int lanes_for(int64_t D) {
   int l = 1;

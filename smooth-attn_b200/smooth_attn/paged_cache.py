@@ -118,7 +118,7 @@ def paged_assign_slots(block_table, context_lens, new_lens, free_pages, free_hea
     key = None
     if not traced:
         key, plan = _plan("slots", (num_tokens, block_size), (block_table, context_lens, new_lens, free_pages, free_head))
-        if plan is not None and plan[0] == torch.cuda.current_device():
+        if plan is not None and plan[0] == torch._C._cuda_getDevice():
             return _assign_call(plan, block_table, context_lens, new_lens, free_pages, free_head)
     given = (context_lens, new_lens, free_pages, free_head)
     B, max_blocks = _table_of(block_table, block_size)
@@ -162,7 +162,7 @@ def _assign_call(plan, block_table, context_lens, new_lens, free_pages, free_hea
         free_head.data_ptr(), slots.data_ptr(), p, p + 4 * N, p + 4 * (N + B + 1), p + 4 * (N + 2 * B + 1), *dims,
         torch._C._cuda_getCurrentRawStream(device))
     _lib.check(st, "sa_paged_assign_slots")
-    return PagedSlots(slots, *i32.split_with_sizes(parts))
+    return PagedSlots(slots, *torch.unsafe_split_with_sizes(i32, parts))
 
 
 def paged_release_pages(block_table, context_lens, done, free_pages, free_head, *, block_size=16):
@@ -180,7 +180,7 @@ def paged_release_pages(block_table, context_lens, done, free_pages, free_head, 
     key = None
     if not traced:
         key, plan = _plan("release", block_size, (block_table, context_lens, done, free_pages, free_head))
-        if plan is not None and plan[0] == torch.cuda.current_device():
+        if plan is not None and plan[0] == torch._C._cuda_getDevice():
             return _release_call(plan, block_table, context_lens, done, free_pages, free_head)
     given = (context_lens, done, free_head)
     B, _ = _table_of(block_table, block_size)
@@ -265,7 +265,7 @@ def qk_norm_rope_paged_append(q, k, v, k_cache, v_cache, slot_mapping, cos=None,
     if plan is None and key is not None and q.shape[0] > 0 and slot_mapping.is_contiguous() and all(
             R._stride_ok(t) for t in (q, k, v)) and R._plain(cos, sin, q_weight, k_weight, positions):
         plan = R._keep(_PLANS, key, _AppendPlan(q, k, v, k_cache, cos, q_weight, k_weight, positions, eps))
-    if plan is not None and plan.device == torch.cuda.current_device():
+    if plan is not None and plan.device == torch._C._cuda_getDevice():
         out = plan.run(q, k, v, k_cache, v_cache, slot_mapping, cos, sin, positions, q_weight, k_weight)
         if out is not None:
             return out
@@ -383,7 +383,7 @@ def paged_key_means(key_means, k_cache, block_table, context_lens, *, start_lens
     key = None
     if not traced:
         key, plan = _plan("means", None, (key_means, k_cache, block_table, context_lens, start_lens))
-        if plan is not None and plan[0] == torch.cuda.current_device():
+        if plan is not None and plan[0] == torch._C._cuda_getDevice():
             return _means_call(plan, key_means, k_cache, block_table, context_lens, start_lens)
     given = (block_table, context_lens, start_lens)
     K._validate_cuda_tensor(k_cache, name="k_cache")
@@ -511,7 +511,7 @@ def sp2norm_sparse_paged_attention(q, k_cache, v_cache, key_means, block_table, 
         # (the decode kernel, and so the workspace, is chosen by this variable too)
         key, plan = _plan("sparse", (num_pages, block_size, scale, os.environ.get("SA_PAGED_DECODE_KERNEL")),
                           (q, k_cache, v_cache, key_means, block_table, context_lens))
-        if plan is not None and plan[0] == torch.cuda.current_device():
+        if plan is not None and plan[0] == torch._C._cuda_getDevice():
             out, pages = _sparse_call(plan, q, k_cache, v_cache, key_means, block_table, context_lens, return_pages)
             return (out, pages) if return_pages else out
     given = (block_table, context_lens)

@@ -278,7 +278,7 @@ def _plan_of(q, k, cos, sin, q_weight, k_weight, eps, positions):
                 or not _plain(cos, sin, q_weight, k_weight, positions)):
             return None
         plan = _keep(_PLANS, key, _Plan(key, q, k, cos, sin, q_weight, k_weight, eps, positions))
-    return plan if plan.device == torch.cuda.current_device() else None
+    return plan if plan.device == torch._C._cuda_getDevice() else None
 
 
 def _fwd_direct(q, k, q_weight, k_weight, cos, sin, positions, eps):
@@ -373,7 +373,7 @@ class _QkNormRopeFn(torch.autograd.Function):
         else:
             res, plan = None, ctx.plan
             # (a hook on saved tensors may hand back others than the forward's)
-            if (plan is not None and plan.device == torch.cuda.current_device()
+            if (plan is not None and plan.device == torch._C._cuda_getDevice()
                     and plan.key == _key_of(q, k, cos, sin, wq, wk, ctx.eps, positions)):
                 res = plan.run_bwd(q, k, dq_out, dk_out, wq, wk, cos, sin, positions, need_dw)
             dq, dk, dwq, dwk = res if res is not None else _bwd_direct(q, k, dq_out, dk_out, wq, wk, cos, sin,
