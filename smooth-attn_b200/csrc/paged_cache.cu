@@ -515,8 +515,7 @@ extern "C" int sa_qk_norm_rope_paged_append(const void* q, const void* k, const 
   a.slots = reinterpret_cast<const long long*>(slots);
   const void* xs[3] = {q, k, v};
   const void* ws[3] = {q_weight, k_weight, nullptr};
-  const int64_t heads = Hq + 2 * Hkv;
-  const int C = sa::qkr::unit_heads(groups * heads, (int64_t)kAppendBlocks * sa::qkr::sm_count() * (sa::qkr::kWalkThreads / 32));
+  const int C = sa::qkr::unit_heads(groups * (Hq + 2 * Hkv), (int64_t)kAppendBlocks * sa::qkr::sm_count() * (sa::qkr::kWalkThreads / 32));
   int64_t units = 0;
   for (int i = 0; i < 3; ++i) {
     a.s[i].x = xs[i];
@@ -529,10 +528,11 @@ extern "C" int sa_qk_norm_rope_paged_append(const void* q, const void* k, const 
     a.s[i].units = groups * a.s[i].per;
     units += a.s[i].units;
   }
-  // warps by each side's share of the rows, at least one where it has any (four warps a block: always enough)
+  // warps by each side's share of the work, at least one where it has any (four warps a block: always enough)
   a.warps = sa::qkr::walk_blocks(units, kAppendBlocks) * (sa::qkr::kWalkThreads / 32);
-  const int64_t q_warps = (int64_t)((double)a.warps * (double)Hq / (double)heads + 0.5);
-  const int64_t qk_warps = (int64_t)((double)a.warps * (double)(Hq + Hkv) / (double)heads + 0.5);
+  const double cq = sa::qkr::walk_cost(groups * Hq, a.s[0].units), ck = sa::qkr::walk_cost(groups * Hkv, a.s[1].units);
+  const int64_t q_warps = (int64_t)((double)a.warps * cq / (cq + 2 * ck) + 0.5);
+  const int64_t qk_warps = (int64_t)((double)a.warps * (cq + ck) / (cq + 2 * ck) + 0.5);
   a.s[0].warp0 = 0;
   a.s[1].warp0 = std::min<int64_t>(a.warps - 2, std::max<int64_t>(Hq > 0, q_warps));
   a.s[2].warp0 = std::min<int64_t>(a.warps - 1, std::max<int64_t>(a.s[1].warp0 + 1, qk_warps));

@@ -165,6 +165,11 @@ __device__ __forceinline__ double weight64(double a) {
   return sp * sp;
 }
 
+// Zeros in the decode's tickets: its next launch finds a workspace of undefined contents.
+__device__ __forceinline__ void clear_tickets(const SelectArgs& a, int64_t first, int64_t step) {
+  for (int64_t i = first; i < a.num_tickets; i += step) a.tickets[i] = 0;
+}
+
 __device__ __forceinline__ unsigned long long key_of(double score) {
   // scores are not negative, so their bits order as they do; NaN above all
   return isnan(score) ? 0x7ff8000000000000ull : (unsigned long long)__double_as_longlong(score);
@@ -178,141 +183,9 @@ __device__ __forceinline__ void mma64(double (&d)[2], double a, double b) {
                : "d"(a), "d"(b));
 }
 
-// One block: 64 pages of one key head, 16 a warp (two row blocks of the product
-// above).  Lane l reads every fourth 16-byte piece of rows l / 4 and 8 + l / 4, so
-// four lanes read 64 neighbouring bytes, and the channels of a product step are
-// the same element of four neighbouring pieces; the queries lie in shared memory
-// as each lane's B of every step.  Heads go eight at a time.  (One page a thread
-// with plain fused multiply-adds took 12.5 us instead of ... for 2048 pages of 8
-// key heads: every query value had to be read again for every page.)
-template <typename E, int D>
-__global__ void __launch_bounds__(128, 4) paged_score_kernel(SelectArgs a) {
-  constexpr int P = D / 32;  // 16-byte pieces a lane holds of a row
-  constexpr bool kAhead = P <= 4;  // the next tile's rows are asked for before this one's product (at D = 256 no room)
-  __shared__ double qs[D / 4][32];
-  const int u = blockIdx.y, b = u / a.Hkv, h = u - b * a.Hkv;
-  const int lane = threadIdx.x & 31, c = lane & 3, step = gridDim.x * 64;
-  int p0 = blockIdx.x * 64 + (threadIdx.x >> 5) * 16 + (lane >> 2);
-  const int32_t* bt = a.bt + (int64_t)b * a.max_blocks;
-  // the first tile's ids and the queries are asked for beside the length, not after it
-  int page[2];
-  auto ids = [&](int at, int end) {
-#pragma unroll
-    for (int r = 0; r < 2; ++r) page[r] = at + 8 * r < end ? __ldg(bt + at + 8 * r) : 0;
-  };
-  auto load_q = [&](int g0, uint4 (&v)[(D + 127) / 128]) {
-    const uint4* q = reinterpret_cast<const uint4*>(static_cast<const E*>(a.q) + ((int64_t)u * a.G + g0) * D);
-#pragma unroll
-    for (int j = 0; j < (D + 127) / 128; ++j) {  // 8 heads of D / 8 pieces
-      const int i = threadIdx.x + j * 128;
-      v[j] = i < D && i / (D / 8) < a.G - g0 ? __ldg(q + i) : make_uint4(0, 0, 0, 0);
-    }
-  };
-  uint4 qv[(D + 127) / 128];
-  ids(p0, a.max_blocks);
-  load_q(0, qv);
-  const Seq s = seq_of(a, b);
-  const int m = s.n - 1;                            // candidates: all but the last page
-  if (m <= a.K - 1 || (int)blockIdx.x * 64 >= m) return;  // all of them are taken: nothing to score
-  auto load = [&](uint4 (&x)[2][P], int at) {
-#pragma unroll
-    for (int r = 0; r < 2; ++r) {
-      if (at + 8 * r >= m) page[r] = 0;  // (an entry behind the context says nothing)
-      if (page[r] < 0 || page[r] >= a.num_blocks) {
-        if (c == 0 && h == 0) atomicAdd(&g_bad_pages, 1u);
-        page[r] = 0;
-      }
-      const uint4* row =
-          reinterpret_cast<const uint4*>(static_cast<const E*>(a.means) + ((int64_t)page[r] * a.Hkv + h) * D);
-#pragma unroll
-      for (int i = 0; i < P; ++i) x[r][i] = __ldg(row + 4 * i + c);
-    }
-  };
-  uint4 x[2][P];
-  load(x, p0);
-  ids(p0 + step, m);
-  for (int t0 = blockIdx.x * 64; t0 < m; t0 += step, p0 += step) {
-    uint4 y[2][kAhead ? P : 1];
-    if constexpr (kAhead) {
-      if (t0 + step < m) {
-        load(y, p0 + step);
-        ids(p0 + 2 * step, m);
-      }
-    }
-    double score[2] = {0.0, 0.0};
-    for (int g0 = 0; g0 < a.G; g0 += 8) {
-      const int heads = min(8, a.G - g0);
-      if (a.G > 8 || t0 < step) {  // one group of heads stays in place
-        if (g0 || t0 >= step) __syncthreads();  // the last heads' queries have been read
-        if (g0 || t0 >= step) load_q(g0, qv);
-#pragma unroll
-        for (int j = 0; j < (D + 127) / 128; ++j) {
-          const int i = threadIdx.x + j * 128, g = i / (D / 8), piece = i % (D / 8);
-          if (i >= D) break;
-          float f[8];
-          unpack<E, 8>(&qv[j], f);
-#pragma unroll
-          for (int e = 0; e < 8; ++e) qs[(piece / 4) * 8 + e][g * 4 + piece % 4] = (double)f[e];
-        }
-        __syncthreads();
-      }
-      double d0[2] = {0.0, 0.0}, d1[2] = {0.0, 0.0}, o0[2] = {0.0, 0.0}, o1[2] = {0.0, 0.0};  // even and odd steps
-#pragma unroll
-      for (int i = 0; i < P; ++i) {
-        float f0[8], f1[8];
-        unpack<E, 8>(&x[0][i], f0);
-        unpack<E, 8>(&x[1][i], f1);
-#pragma unroll
-        for (int e = 0; e < 8; e += 2) {
-          const double qa = qs[i * 8 + e][lane], qb = qs[i * 8 + e + 1][lane];
-          mma64(d0, (double)f0[e], qa);
-          mma64(d1, (double)f1[e], qa);
-          mma64(o0, (double)f0[e + 1], qb);
-          mma64(o1, (double)f1[e + 1], qb);
-        }
-      }
-      if (heads <= 4) {  // half the lanes have no head: they take the second row block's
-#pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          const double other = __shfl_xor_sync(0xffffffffu, d1[e] + o1[e], 2);
-          const double w = (c < 2 ? 2 * c + e : 2 * c - 4 + e) < heads
-                               ? weight64(fma(a.scale2, c < 2 ? d0[e] + o0[e] : other, -1.0)) : 0.0;
-          score[0] += c < 2 ? w : 0.0;
-          score[1] += c < 2 ? 0.0 : w;
-        }
-      } else {
-#pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          if (2 * c + e < heads) {
-            score[0] += weight64(fma(a.scale2, d0[e] + o0[e], -1.0));
-            score[1] += weight64(fma(a.scale2, d1[e] + o1[e], -1.0));
-          }
-        }
-      }
-    }
-#pragma unroll
-    for (int r = 0; r < 2; ++r) {
-      score[r] += __shfl_xor_sync(0xffffffffu, score[r], 1);
-      score[r] += __shfl_xor_sync(0xffffffffu, score[r], 2);
-      if (c == r && p0 + 8 * r < m && SA_DCHECK(p0 + 8 * r < a.max_blocks))
-        a.keys[(int64_t)u * a.max_blocks + p0 + 8 * r] = key_of(score[r]);
-    }
-    if constexpr (kAhead) {
-#pragma unroll
-      for (int r = 0; r < 2; ++r)
-#pragma unroll
-        for (int i = 0; i < P; ++i) x[r][i] = y[r][i];
-    } else {
-      if (t0 + step < m) {
-        load(x, p0 + step);
-        ids(p0 + 2 * step, m);
-      }
-    }
-  }
-}
-
 // ---- choice ---------------------------------------------------------------------
 
+constexpr int kScoreThreads = 256;
 constexpr int kBins = 2048;
 constexpr int kKeep = 8;    // keys a thread keeps in registers
 constexpr int kShort = 64;  // keys that are ranked by comparing each with each
@@ -322,17 +195,24 @@ constexpr int kShort = 64;  // keys that are ranked by comparing each with each
 // holds the last chosen key until all of that range is chosen, it is one value,
 // or so few keys that they are ranked directly; then an ordered pass writes what
 // is chosen.
+template <int kSelThreads> struct ChooseShared {
+  int bins[kBins];
+  unsigned long long ends[2][kSelThreads / 32], few[kShort];
+  int warp_sums[kSelThreads / 32], counts[kKeep * (kSelThreads / 32)];
+  int found_bin, found_above, found_count, nfew;
+};
+
 template <int kSelThreads>
-__global__ void __launch_bounds__(kSelThreads) paged_choose_kernel(SelectArgs a) {
+__device__ __forceinline__ void choose_pages(const SelectArgs& a, int u, ChooseShared<kSelThreads>& sh) {
   constexpr int kSelWarps = kSelThreads / 32;
-  __shared__ int bins[kBins];
-  __shared__ unsigned long long ends[2][kSelWarps], few[kShort];
-  __shared__ int warp_sums[kSelWarps], counts[kKeep * kSelWarps];
-  __shared__ int found_bin, found_above, found_count, nfew;
-  const int u = blockIdx.x, b = u / a.Hkv, h = u - b * a.Hkv, tid = threadIdx.x;
+  auto& bins = sh.bins;
+  auto& ends = sh.ends;
+  auto& few = sh.few;
+  auto& warp_sums = sh.warp_sums;
+  auto& counts = sh.counts;
+  int &found_bin = sh.found_bin, &found_above = sh.found_above, &found_count = sh.found_count, &nfew = sh.nfew;
+  const int b = u / a.Hkv, h = u - b * a.Hkv, tid = threadIdx.x;
   const int lane = tid & 31, warp = tid >> 5;
-  for (int64_t i = (int64_t)u * kSelThreads + tid; i < a.num_tickets; i += (int64_t)gridDim.x * kSelThreads)
-    a.tickets[i] = 0;
   const int32_t* bt = a.bt + (int64_t)b * a.max_blocks;
   const unsigned long long* keys = a.keys + (int64_t)u * a.max_blocks;
   // read beside the length, not after it: what lies behind the candidates is not looked at
@@ -340,7 +220,7 @@ __global__ void __launch_bounds__(kSelThreads) paged_choose_kernel(SelectArgs a)
 #pragma unroll
   for (int j = 0; j < kKeep; ++j) {
     const int i = j * kSelThreads + tid;
-    mine[j] = i < a.max_blocks && a.max_blocks > a.K ? keys[i] : 0;
+    mine[j] = i < a.max_blocks && a.max_blocks > a.K ? __ldcg(keys + i) : 0;  // (other SMs' writes)
   }
   const Seq s = seq_of(a, b);
   const int m = s.n - 1, need = min(a.K, s.n) - 1;  // of the m candidates
@@ -354,7 +234,7 @@ __global__ void __launch_bounds__(kSelThreads) paged_choose_kernel(SelectArgs a)
       for (int j = 0; j < kKeep; ++j)
         if (j * kSelThreads + tid < m) f(mine[j]);
     } else {
-      for (int i = tid; i < m; i += kSelThreads) f(keys[i]);
+      for (int i = tid; i < m; i += kSelThreads) f(__ldcg(keys + i));
     }
   };
   if (m > need && need > 0) {
@@ -472,7 +352,7 @@ __global__ void __launch_bounds__(kSelThreads) paged_choose_kernel(SelectArgs a)
 #pragma unroll
       for (int j = 0; j < kKeep; ++j) {
         const int i = i0 + j * kSelThreads + tid;
-        const unsigned long long k = i >= m ? 0 : kept ? mine[j] : keys[i];
+        const unsigned long long k = i >= m ? 0 : kept ? mine[j] : __ldcg(keys + i);
         in_w[j] = __ballot_sync(0xffffffffu, i < m && k >= lo && k <= hi);
         ab_w[j] = __ballot_sync(0xffffffffu, i < m && k > hi);
         if (lane == 0) counts[j * kSelWarps + warp] = __popc(in_w[j]) | (__popc(ab_w[j]) << 16);
@@ -525,15 +405,168 @@ __global__ void __launch_bounds__(kSelThreads) paged_choose_kernel(SelectArgs a)
   }
 }
 
+// ---- scores, and the choice behind them ---------------------------------------------
+
+// One block: 64 pages of one key head, 16 a warp (two row blocks of the product
+// above).  Lane l reads every fourth 16-byte piece of rows l / 4 and 8 + l / 4, so
+// four lanes read 64 neighbouring bytes, and the channels of a product step are
+// the same element of four neighbouring pieces; the queries lie in shared memory
+// as each lane's B of every step.  Heads go eight at a time.  (One page a thread
+// with plain fused multiply-adds took 12.5 us instead of ... for 2048 pages of 8
+// key heads: every query value had to be read again for every page.)
+template <typename E, int D>
+__global__ void __launch_bounds__(kScoreThreads, 2) paged_score_kernel(SelectArgs a, int choose) {
+  constexpr int P = D / 32;  // 16-byte pieces a lane holds of a row
+  constexpr bool kAhead = P <= 4;  // the next tile's rows are asked for before this one's product (at D = 256 no room)
+  constexpr int TILE = kScoreThreads / 2;  // pages of a block: 16 a warp
+  constexpr int NQ = (D + kScoreThreads - 1) / kScoreThreads;
+  __shared__ double qs[D / 4][32];
+  __shared__ ChooseShared<kScoreThreads> sh;
+  const int u = blockIdx.y, b = u / a.Hkv, h = u - b * a.Hkv;
+  clear_tickets(a, ((int64_t)u * gridDim.x + blockIdx.x) * kScoreThreads + threadIdx.x,
+                (int64_t)gridDim.x * gridDim.y * kScoreThreads);
+  const int lane = threadIdx.x & 31, c = lane & 3, step = gridDim.x * TILE;
+  int p0 = blockIdx.x * TILE + (threadIdx.x >> 5) * 16 + (lane >> 2);
+  const int32_t* bt = a.bt + (int64_t)b * a.max_blocks;
+  // the first tile's ids and the queries are asked for beside the length, not after it
+  int page[2];
+  auto ids = [&](int at, int end) {
+#pragma unroll
+    for (int r = 0; r < 2; ++r) page[r] = at + 8 * r < end ? __ldg(bt + at + 8 * r) : 0;
+  };
+  auto load_q = [&](int g0, uint4 (&v)[NQ]) {
+    const uint4* q = reinterpret_cast<const uint4*>(static_cast<const E*>(a.q) + ((int64_t)u * a.G + g0) * D);
+#pragma unroll
+    for (int j = 0; j < NQ; ++j) {  // 8 heads of D / 8 pieces
+      const int i = threadIdx.x + j * kScoreThreads;
+      v[j] = i < D && i / (D / 8) < a.G - g0 ? __ldg(q + i) : make_uint4(0, 0, 0, 0);
+    }
+  };
+  uint4 qv[NQ];
+  ids(p0, a.max_blocks);
+  load_q(0, qv);
+  const Seq s = seq_of(a, b);
+  const int m = s.n - 1;                            // candidates: all but the last page
+  const bool score_any = m > a.K - 1 && (int)blockIdx.x * TILE < m;  // else all are taken, or none is this block's
+  auto load = [&](uint4 (&x)[2][P], int at) {
+#pragma unroll
+    for (int r = 0; r < 2; ++r) {
+      if (at + 8 * r >= m) page[r] = 0;  // (an entry behind the context says nothing)
+      if (page[r] < 0 || page[r] >= a.num_blocks) {
+        if (c == 0 && h == 0) atomicAdd(&g_bad_pages, 1u);
+        page[r] = 0;
+      }
+      const uint4* row =
+          reinterpret_cast<const uint4*>(static_cast<const E*>(a.means) + ((int64_t)page[r] * a.Hkv + h) * D);
+#pragma unroll
+      for (int i = 0; i < P; ++i) x[r][i] = __ldg(row + 4 * i + c);
+    }
+  };
+  uint4 x[2][P];
+  if (score_any) {
+    load(x, p0);
+    ids(p0 + step, m);
+  }
+  for (int t0 = blockIdx.x * TILE; score_any && t0 < m; t0 += step, p0 += step) {
+    uint4 y[2][kAhead ? P : 1];
+    if constexpr (kAhead) {
+      if (t0 + step < m) {
+        load(y, p0 + step);
+        ids(p0 + 2 * step, m);
+      }
+    }
+    double score[2] = {0.0, 0.0};
+    for (int g0 = 0; g0 < a.G; g0 += 8) {
+      const int heads = min(8, a.G - g0);
+      if (a.G > 8 || t0 < step) {  // one group of heads stays in place
+        if (g0 || t0 >= step) __syncthreads();  // the last heads' queries have been read
+        if (g0 || t0 >= step) load_q(g0, qv);
+#pragma unroll
+        for (int j = 0; j < NQ; ++j) {
+          const int i = threadIdx.x + j * kScoreThreads, g = i / (D / 8), piece = i % (D / 8);
+          if (i >= D) break;
+          float f[8];
+          unpack<E, 8>(&qv[j], f);
+#pragma unroll
+          for (int e = 0; e < 8; ++e) qs[(piece / 4) * 8 + e][g * 4 + piece % 4] = (double)f[e];
+        }
+        __syncthreads();
+      }
+      double d0[2] = {0.0, 0.0}, d1[2] = {0.0, 0.0}, o0[2] = {0.0, 0.0}, o1[2] = {0.0, 0.0};  // even and odd steps
+#pragma unroll
+      for (int i = 0; i < P; ++i) {
+        float f0[8], f1[8];
+        unpack<E, 8>(&x[0][i], f0);
+        unpack<E, 8>(&x[1][i], f1);
+#pragma unroll
+        for (int e = 0; e < 8; e += 2) {
+          const double qa = qs[i * 8 + e][lane], qb = qs[i * 8 + e + 1][lane];
+          mma64(d0, (double)f0[e], qa);
+          mma64(d1, (double)f1[e], qa);
+          mma64(o0, (double)f0[e + 1], qb);
+          mma64(o1, (double)f1[e + 1], qb);
+        }
+      }
+      if (heads <= 4) {  // half the lanes have no head: they take the second row block's
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          const double other = __shfl_xor_sync(0xffffffffu, d1[e] + o1[e], 2);
+          const double w = (c < 2 ? 2 * c + e : 2 * c - 4 + e) < heads
+                               ? weight64(fma(a.scale2, c < 2 ? d0[e] + o0[e] : other, -1.0)) : 0.0;
+          score[0] += c < 2 ? w : 0.0;
+          score[1] += c < 2 ? 0.0 : w;
+        }
+      } else {
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          if (2 * c + e < heads) {
+            score[0] += weight64(fma(a.scale2, d0[e] + o0[e], -1.0));
+            score[1] += weight64(fma(a.scale2, d1[e] + o1[e], -1.0));
+          }
+        }
+      }
+    }
+#pragma unroll
+    for (int r = 0; r < 2; ++r) {
+      score[r] += __shfl_xor_sync(0xffffffffu, score[r], 1);
+      score[r] += __shfl_xor_sync(0xffffffffu, score[r], 2);
+      if (c == r && p0 + 8 * r < m && SA_DCHECK(p0 + 8 * r < a.max_blocks))
+        a.keys[(int64_t)u * a.max_blocks + p0 + 8 * r] = key_of(score[r]);
+    }
+    if constexpr (kAhead) {
+#pragma unroll
+      for (int r = 0; r < 2; ++r)
+#pragma unroll
+        for (int i = 0; i < P; ++i) x[r][i] = y[r][i];
+    } else {
+      if (t0 + step < m) {
+        load(x, p0 + step);
+        ids(p0 + 2 * step, m);
+      }
+    }
+  }
+  if (!choose) return;
+  // the cluster's blocks have scored the sequence's pages; its first one chooses
+  if (gridDim.x > 1) {
+    asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+    if (blockIdx.x != 0) return;
+    asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+  } else {
+    __syncthreads();
+  }
+  choose_pages<kScoreThreads>(a, u, sh);
+}
+
+// The choice by itself: long tables, after their scores, and tables whose every page is taken.
+template <int NT> __global__ void __launch_bounds__(NT) paged_choose_kernel(SelectArgs a) {
+  __shared__ ChooseShared<NT> sh;
+  clear_tickets(a, (int64_t)blockIdx.x * NT + threadIdx.x, (int64_t)gridDim.x * NT);
+  choose_pages<NT>(a, blockIdx.x, sh);
+}
+
 // ---- host side --------------------------------------------------------------------
 
-#ifndef CT
-#define CT 256
-#endif
-#ifndef MB
-#define MB 2
-#endif
-constexpr int kMeansBlocks = MB;
+constexpr int kMeansBlocks = 2;
 
 template <typename E, int D>
 static int launch_means(const MeansArgs& a, int64_t B, cudaStream_t st) {
@@ -554,18 +587,39 @@ static int launch_means_d(const MeansArgs& a, int64_t B, int64_t D, cudaStream_t
   }
 }
 
-template <typename E>
-static int launch_score(const SelectArgs& a, int64_t units, int64_t D, cudaStream_t st) {
-  // tiles of 64 pages, dealt to at most one resident wave of blocks (four an SM)
-  const int64_t tiles = (a.max_blocks + 63) / 64, wave = 4ll * qkr::sm_count();
-  const dim3 grid((unsigned)std::max<int64_t>(1, std::min(tiles, wave / units)), (unsigned)units);
-  switch (D) {
-    case 32: paged_score_kernel<E, 32><<<grid, 128, 0, st>>>(a); break;
-    case 64: paged_score_kernel<E, 64><<<grid, 128, 0, st>>>(a); break;
-    case 128: paged_score_kernel<E, 128><<<grid, 128, 0, st>>>(a); break;
-    default: paged_score_kernel<E, 256><<<grid, 128, 0, st>>>(a); break;
+// Scores, and with `choose` the choice, in one launch: the blocks of one sequence
+// and key head are a cluster, as many as one resident wave (two an SM) has for it,
+// at most 8 (16 measured the same), tiles of 128 pages dealt to them.
+template <typename E, int D>
+static int launch_score_d(const SelectArgs& a, int64_t units, int choose, cudaStream_t st) {
+  auto kfn = paged_score_kernel<E, D>;
+  const int64_t tiles = (a.max_blocks + kScoreThreads / 2 - 1) / (kScoreThreads / 2), wave = 2ll * qkr::sm_count();
+  int64_t x = std::max<int64_t>(1, std::min(tiles, wave / units));
+  if (choose) x = std::min<int64_t>(x, 8);
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)x, (unsigned)units);
+  cfg.blockDim = dim3(kScoreThreads);
+  cfg.stream = st;
+  cudaLaunchAttribute attr;
+  if (choose && x > 1) {
+    attr.id = cudaLaunchAttributeClusterDimension;
+    attr.val.clusterDim.x = (unsigned)x;
+    attr.val.clusterDim.y = 1;
+    attr.val.clusterDim.z = 1;
+    cfg.attrs = &attr;
+    cfg.numAttrs = 1;
   }
-  return sa_record_cuda_error(cudaGetLastError());
+  return sa_record_cuda_error(cudaLaunchKernelEx(&cfg, kfn, a, choose));
+}
+
+template <typename E>
+static int launch_score(const SelectArgs& a, int64_t units, int64_t D, int choose, cudaStream_t st) {
+  switch (D) {
+    case 32: return launch_score_d<E, 32>(a, units, choose, st);
+    case 64: return launch_score_d<E, 64>(a, units, choose, st);
+    case 128: return launch_score_d<E, 128>(a, units, choose, st);
+    default: return launch_score_d<E, 256>(a, units, choose, st);
+  }
 }
 
 static int check_cache(int64_t B, int64_t Hkv, int64_t num_blocks, int64_t bs, int64_t max_blocks, int64_t D,
@@ -612,11 +666,15 @@ static int run_choice(SelectArgs& a, const void* q, const void* means, const int
   a.scale2 = 2.0 * scale;
   a.Hkv = (int)Hkv, a.G = (int)(Hq / Hkv), a.bs = (int)bs, a.max_blocks = (int)max_blocks, a.K = (int)K;
   const int64_t units = B * Hkv;
-  if (max_blocks > K) {  // else every page is taken
-    const int rc = dtype == SA_BF16 ? launch_score<__nv_bfloat16>(a, units, D, st) : launch_score<__half>(a, units, D, st);
-    if (rc != SA_OK) return rc;
+  // a block of 256 threads holds the keys of up to 2048 pages in registers and chooses right behind the scores;
+  // longer tables take a launch of 1024 threads for it
+  const bool at_once = max_blocks <= kKeep * kScoreThreads;
+  if (max_blocks > K) {
+    const int rc = dtype == SA_BF16 ? launch_score<__nv_bfloat16>(a, units, D, at_once, st)
+                                    : launch_score<__half>(a, units, D, at_once, st);
+    if (rc != SA_OK || at_once) return rc;
   }
-  if (max_blocks <= CT * kKeep) paged_choose_kernel<CT><<<(unsigned)units, CT, 0, st>>>(a);
+  if (at_once) paged_choose_kernel<256><<<(unsigned)units, 256, 0, st>>>(a);
   else paged_choose_kernel<1024><<<(unsigned)units, 1024, 0, st>>>(a);
   return sa_record_cuda_error(cudaGetLastError());
 }

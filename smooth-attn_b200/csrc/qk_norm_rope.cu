@@ -332,11 +332,13 @@ static int64_t groups_of(int64_t N, int64_t D) {
   return (N + per - 1) / per;
 }
 
-// Blocks, and the warps of q by its share of the rows: at least one for each side that has any.
+// Blocks, and the warps of q by its share of the work: at least one for each side that has any.
 static int64_t plan(const Side& q, const Side& k, Shape* sh, int per_sm) {
   const int64_t blocks = walk_blocks(q.units + k.units, per_sm), warps = blocks * (kWalkThreads / 32);
   if (blocks == 0) return 0;
-  sh->q_warps = (int64_t)((double)warps * (double)q.H / (double)(q.H + k.H) + 0.5);
+  const double cq = walk_cost(q.per ? q.units / q.per * q.H : 0, q.units);
+  const double ck = walk_cost(k.per ? k.units / k.per * k.H : 0, k.units);
+  sh->q_warps = (int64_t)((double)warps * cq / (cq + ck) + 0.5);
   if (q.units) sh->q_warps = std::max<int64_t>(1, sh->q_warps);
   if (k.units) sh->q_warps = std::min(sh->q_warps, warps - 1);  // (four warps a block: one is left)
   return blocks;

@@ -507,6 +507,10 @@ inline int make_tables(Tables* t, const void* cosv, const void* sinv, int cs_dty
   return SA_OK;
 }
 
+// What `units` units of in all `rows` heads' groups cost a warp, in rows.
+constexpr double kUnitCost = 1.5;
+inline double walk_cost(int64_t rows, int64_t units) { return (double)rows + kUnitCost * (double)units; }
+
 // Heads of a unit, for `rows` (token group, head) pairs on `warps` warps: the
 // choice among 1, 2, 4 and 8 with the shortest busiest warp, a unit costing its heads
 // and about one and a half more for its angles and addresses.  Many rows take 8:
@@ -517,7 +521,7 @@ inline int unit_heads(int64_t rows, int64_t warps) {
   double cost = 0;
   for (int c = 1; c <= 8; c *= 2) {
     const int64_t units = (rows + c - 1) / c, rounds = (units + warps - 1) / warps;
-    const double t = (double)rounds * (c + 1.5);
+    const double t = (double)rounds * (c + kUnitCost);
     if (c == 1 || t < cost) best = c, cost = t;
   }
   return best;
