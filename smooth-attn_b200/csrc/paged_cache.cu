@@ -300,10 +300,10 @@ __global__ void __launch_bounds__(kWalkThreads, kAppendBlocks) qk_norm_rope_appe
   const int64_t warps = (side == 2 ? a.warps : a.s[side + 1].warp0) - sd.warp0;
   const Units un = make_units(warp - sd.warp0, warps, sd.units, sd.H, sd.C, sd.per);
   if (un.count == 0) return;
-  const Lane ln = lane_of<L>(tb);
+  const Lane ln = lane_of<E, L>(tb);
   auto token = [&](int64_t g) { return g * (32 / L) + (threadIdx.x & 31) / L; };
   const Where<L> where{tb, a};
-  Angles<Where<L>> ang(tb, ln, &g_bad_entries, un, where);
+  Angles<E, Where<L>> ang(tb, ln, &g_bad_entries, un, where);
   Map map;
   E* y = nullptr;  // the row that comes next
   int64_t yh = 0;
@@ -328,7 +328,7 @@ __global__ void __launch_bounds__(kWalkThreads, kAppendBlocks) qk_norm_rope_appe
       [&](int64_t g, int h) {
         if (side < 2) {
           float2 c[4], s[4], w1[4], w2[4];
-          load_weights(sd.w, a.w_dtype, ln, w1, w2);
+          load_weights<E>(sd.w, a.w_dtype, ln, w1, w2);
           ang.enter(c, s);
           map.make(c, s, w1, w2);
         }
@@ -358,9 +358,9 @@ __global__ void __launch_bounds__(kWalkThreads, kAppendBlocks) qk_norm_rope_appe
       [&](Raw8<E> (&rows)[2]) {
         if (side < 2) norm_rope<E, L>(tb, map, rows[0], rows[1]);
         if (padding) rows[0].zero(), rows[1].zero();
-        if (write && SA_DCHECK(ln.o2 + 8 <= tb.D)) {
-          rows[0].store(y);
-          rows[1].store(y + (ln.o2 - ln.o1));
+        if (write && SA_DCHECK(ln.o2 + ln.ps + 4 <= tb.D)) {
+          rows[0].store(y, ln.ps);
+          rows[1].store(y + (ln.o2 - ln.o1), ln.ps);
         }
         y += yh;
       });

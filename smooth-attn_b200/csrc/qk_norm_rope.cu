@@ -103,24 +103,25 @@ __device__ __forceinline__ Part part_of_warp(const Side& q, const Side& k, const
 }
 
 // Depth of the ring and resident blocks an SM: four forward blocks of 41 KB (16-bit)
-// and 128 registers a thread, three backward blocks of at most 65 KB and 168
+// and 128 registers a thread (three of 49 KB for fp32), three backward blocks of at most 65 KB and 168
 // registers (at 128 the backward spills).
 template <typename E> constexpr int kFwdRing = sizeof(E) == 4 ? 6 : 10;
 template <typename E> constexpr int kBwdRing = sizeof(E) == 4 ? 4 : 6;
-constexpr int kFwdBlocks = 4, kBwdBlocks = 3;
+template <typename E> constexpr int kFwdBlocks = sizeof(E) == 4 ? 3 : 4;
+constexpr int kBwdBlocks = 3;
 
 // ---- forward ----------------------------------------------------------------
 
 template <typename E, int L>
-__global__ void __launch_bounds__(kWalkThreads, kFwdBlocks)
+__global__ void __launch_bounds__(kWalkThreads, kFwdBlocks<E>)
     qk_norm_rope_fwd(Side q, Side k, Tables tb, Shape sh) {
   extern __shared__ __align__(16) uint4 ring[];
   const Part part = part_of_warp(q, k, sh);
   if (part.un.count == 0) return;
   const Side& sd = part.is_q ? q : k;
-  const Lane ln = lane_of<L>(tb);
+  const Lane ln = lane_of<E, L>(tb);
   const Where<L> where{tb, sh};
-  Angles<Where<L>> ang(tb, ln, &g_bad_positions, part.un, where);
+  Angles<E, Where<L>> ang(tb, ln, &g_bad_positions, part.un, where);
   Map map;
   E* y = nullptr;  // the row that comes next
   bool on = false;
@@ -134,7 +135,7 @@ __global__ void __launch_bounds__(kWalkThreads, kFwdBlocks)
       [&]() { ang.begin(); },
       [&](int64_t g, int h) {
         float2 c[4], s[4], w1[4], w2[4];
-        load_weights(sd.w, sh.w_dtype, ln, w1, w2);
+        load_weights<E>(sd.w, sh.w_dtype, ln, w1, w2);
         ang.enter(c, s);
         map.make(c, s, w1, w2);
         const Token tk = token_of<L>(sh, g);
@@ -143,9 +144,9 @@ __global__ void __launch_bounds__(kWalkThreads, kFwdBlocks)
       },
       [&](Raw8<E> (&rows)[2]) {
         norm_rope<E, L>(tb, map, rows[0], rows[1]);
-        if (on && SA_DCHECK(ln.o2 + 8 <= tb.D)) {
-          rows[0].store(y);
-          rows[1].store(y + (ln.o2 - ln.o1));
+        if (on && SA_DCHECK(ln.o2 + ln.ps + 4 <= tb.D)) {
+          rows[0].store(y, ln.ps);
+          rows[1].store(y + (ln.o2 - ln.o1), ln.ps);
         }
         y += sd.yh;
       });
@@ -160,13 +161,13 @@ __global__ void __launch_bounds__(kWalkThreads, kBwdBlocks)
   extern __shared__ __align__(16) uint4 ring[];
   const Part part = part_of_warp(q, k, sh);
   const Side& sd = part.is_q ? q : k;
-  const Lane ln = lane_of<L>(tb);
+  const Lane ln = lane_of<E, L>(tb);
   const Where<L> where{tb, sh};
-  Angles<Where<L>> ang(tb, ln, &g_bad_positions, part.un, where);
+  Angles<E, Where<L>> ang(tb, ln, &g_bad_positions, part.un, where);
   float2 c[4], s[4], w1[4], w2[4], dw1[4], dw2[4];
 #pragma unroll
   for (int i = 0; i < 4; ++i) dw1[i] = dw2[i] = splat(0.f);
-  load_weights(sd.w, sh.w_dtype, ln, w1, w2);
+  load_weights<E>(sd.w, sh.w_dtype, ln, w1, w2);
   E* dx = nullptr;  // the row that comes next
   bool on = false;
   walk_rows<E, 2, kBwdRing<E>>(
@@ -219,11 +220,11 @@ __global__ void __launch_bounds__(kWalkThreads, kBwdBlocks)
             g2[i] = ffma2(x2[i], m2, fmul2(v2[i], r2));
           }
         }
-        if (on && SA_DCHECK(ln.o2 + 8 <= tb.D)) {
+        if (on && SA_DCHECK(ln.o2 + ln.ps + 4 <= tb.D)) {
           rows[2].set(g1);
           rows[3].set(g2);
-          rows[2].store(dx);
-          rows[3].store(dx + (ln.o2 - ln.o1));
+          rows[2].store(dx, ln.ps);
+          rows[3].store(dx + (ln.o2 - ln.o1), ln.ps);
         }
         dx += sd.yh;
       });
@@ -244,10 +245,13 @@ __global__ void __launch_bounds__(kWalkThreads, kBwdBlocks)
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   __syncthreads();
   if (lane < L && ln.active) {
-    float2* to1 = reinterpret_cast<float2*>(red + warp * tb.D + ln.o1);
-    float2* to2 = reinterpret_cast<float2*>(red + warp * tb.D + ln.o2);
+    float* to = red + warp * tb.D;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) to1[i] = dw1[i], to2[i] = dw2[i];
+    for (int i = 0; i < 4; ++i) {
+      const int d = i / 2 * ln.ps + i % 2 * 2;
+      *reinterpret_cast<float2*>(to + ln.o1 + d) = dw1[i];
+      *reinterpret_cast<float2*>(to + ln.o2 + d) = dw2[i];
+    }
   }
   __syncthreads();
   const int64_t w0 = (int64_t)blockIdx.x * W;
@@ -428,11 +432,12 @@ extern "C" int sa_qk_norm_rope(const void* q, const void* k, void* q_out, void* 
   if (Hkv > 0 && ((rc = check_rows(k, k_strides, es)) != SA_OK || (rc = check_rows(k_out, ko_strides, es)) != SA_OK))
     return rc;
   const int64_t groups = groups_of(B * T, D);
-  const int C = unit_heads(groups * (Hq + Hkv), (int64_t)kFwdBlocks * sm_count() * (kWalkThreads / 32));
+  const int per_sm = dtype == SA_F32 ? kFwdBlocks<float> : kFwdBlocks<__half>;
+  const int C = unit_heads(groups * (Hq + Hkv), (int64_t)per_sm * sm_count() * (kWalkThreads / 32));
   const Side a = side_of(q, q_out, nullptr, q_weight, Hq, q_strides, qo_strides, nullptr, groups, C);
   const Side b = side_of(k, k_out, nullptr, k_weight, Hkv, k_strides, ko_strides, nullptr, groups, C);
   Shape sh{B * T, T, 0, w_dtype, FastDiv((uint32_t)T)};
-  const int64_t blocks = plan(a, b, &sh, kFwdBlocks);
+  const int64_t blocks = plan(a, b, &sh, per_sm);
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   if (dtype == SA_F32) return launch_fwd<float>(a, b, tb, sh, blocks, st);
   if (dtype == SA_BF16) return launch_fwd<__nv_bfloat16>(a, b, tb, sh, blocks, st);

@@ -8,7 +8,7 @@
 //   y[j]       = n[j]                             R <= j < D
 //
 // A row belongs to L = 1, 2, 4, 8 or 16 neighbouring lanes of a warp, each
-// with two 8-element chunks that the rotation pairs (x[8g..], x[R/2 + 8g..]),
+// with two 8-element chunks that the rotation pairs (16-bit: x[8g..], x[R/2 + 8g..]),
 // so the rotation needs no exchange and the norm's sum log2(L) shuffles.
 // Everything between the loads and the one rounding of y is fp32.
 #pragma once
@@ -68,30 +68,43 @@ template <typename E> struct Raw8 {
 #pragma unroll
     for (int i = 0; i < (int)sizeof(E) / 2; ++i) reinterpret_cast<uint4*>(p)[i] = u[i];
   }
+  // fp32: the second 4 elements ps behind the first (16-bit: all 8 together, ps is 4)
+  __device__ __forceinline__ void store(E* p, int ps) const {
+    *reinterpret_cast<uint4*>(p) = u[0];
+    if constexpr (sizeof(E) == 4) *reinterpret_cast<uint4*>(p + ps) = u[1];
+  }
 };
 
-// 8 elements of a table or weight of a type known at run time (one uniform branch).
-__device__ __forceinline__ void load8_any(const void* p, int64_t at, int dtype, float (&f)[8]) {
+// The 8 elements of a table or weight that go with a lane's chunk, of a type known
+// at run time (one uniform branch): 4 at `at` and 4 at `at + ps`, neighbours but for
+// fp32 rows (see Lane).
+template <typename E>
+__device__ __forceinline__ void raw8_any(const void* p, int64_t at, int ps, int dtype, uint4& lo, uint4& hi) {
+  if (dtype == SA_F32) {
+    lo = __ldg(reinterpret_cast<const uint4*>(static_cast<const float*>(p) + at));
+    hi = __ldg(reinterpret_cast<const uint4*>(static_cast<const float*>(p) + at + ps));
+  } else if constexpr (sizeof(E) == 4) {
+    const uint2 a = __ldg(reinterpret_cast<const uint2*>(static_cast<const uint16_t*>(p) + at));
+    const uint2 b = __ldg(reinterpret_cast<const uint2*>(static_cast<const uint16_t*>(p) + at + ps));
+    lo = make_uint4(a.x, a.y, b.x, b.y);
+  } else {
+    lo = __ldg(reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(p) + at));
+  }
+}
+__device__ __forceinline__ void open8_any(const uint4& lo, const uint4& hi, int dtype, float2 (&f)[4]) {
   if (dtype == SA_F32) {
     Raw8<float> r;
-    r.load(static_cast<const float*>(p) + at);
+    r.u[0] = lo, r.u[1] = hi;
     r.get(f);
   } else if (dtype == SA_BF16) {
     Raw8<__nv_bfloat16> r;
-    r.load(static_cast<const __nv_bfloat16*>(p) + at);
+    r.u[0] = lo;
     r.get(f);
   } else {
     Raw8<__half> r;
-    r.load(static_cast<const __half*>(p) + at);
+    r.u[0] = lo;
     r.get(f);
   }
-}
-
-__device__ __forceinline__ void load8_any(const void* p, int64_t at, int dtype, float2 (&f)[4]) {
-  float g[8];
-  load8_any(p, at, dtype, g);
-#pragma unroll
-  for (int i = 0; i < 4; ++i) f[i] = make_float2(g[2 * i], g[2 * i + 1]);
 }
 
 // What a lane owns of every row, and the tables it reads.
@@ -108,20 +121,26 @@ struct Tables {
   float eps, inv_d;
 };
 
+// A chunk is two groups of 4 elements: neighbours in 16-bit rows (16 bytes in
+// all); in fp32 rows, 16 bytes each, a group's lanes apart, so that one
+// instruction's lanes read whole 32-byte sectors.
 struct Lane {
   int o1, o2;     // offsets of the lane's two chunks in the row
+  int ps;         // from a chunk's first group to its second
   bool active;    // the lane has a chunk at all (D / 16 need not be a power of two)
   bool rotated;   // its chunks are a rotated pair
 };
 
-template <int L>
+template <typename E, int L>
 __device__ __forceinline__ Lane lane_of(const Tables& t) {
+  constexpr int kStep = sizeof(E) == 4 ? 4 : 8;
   const int g = (threadIdx.x & 31) % L, nr = t.R / 16;
   Lane l;
   l.active = g < t.D / 16;
   l.rotated = g < nr;
-  l.o1 = l.rotated ? 8 * g : t.R + 8 * (g - nr);
-  l.o2 = l.rotated ? t.R / 2 + 8 * g : t.R + (t.D - t.R) / 2 + 8 * (g - nr);
+  l.o1 = l.rotated ? kStep * g : t.R + kStep * (g - nr);
+  l.o2 = l.o1 + (l.rotated ? t.R : t.D - t.R) / 2;
+  l.ps = sizeof(E) == 4 ? (l.rotated ? t.R : t.D - t.R) / 4 : 4;
   return l;
 }
 
@@ -188,11 +207,15 @@ __device__ __forceinline__ void norm_rope(const Tables& t, const Map& m, Raw8<E>
   b.set(y2);
 }
 
+template <typename E>
 __device__ __forceinline__ void load_weights(const void* w, int w_dtype, const Lane& l, float2 (&w1)[4],
                                              float2 (&w2)[4]) {
   if (w != nullptr && l.active) {
-    load8_any(w, l.o1, w_dtype, w1);
-    load8_any(w, l.o2, w_dtype, w2);
+    uint4 a, b, c, d;
+    raw8_any<E>(w, l.o1, l.ps, w_dtype, a, b);
+    raw8_any<E>(w, l.o2, l.ps, w_dtype, c, d);
+    open8_any(a, b, w_dtype, w1);
+    open8_any(c, d, w_dtype, w2);
   } else {
 #pragma unroll
     for (int i = 0; i < 4; ++i) w1[i] = w2[i] = splat(1.f);
@@ -300,8 +323,8 @@ __device__ __forceinline__ void walk_rows(const Units& un, const Lane& ln, uint4
         const uint32_t to = ask_slot + k * 2 * R::kChunk * kSlot;
 #pragma unroll
         for (int c = 0; c < R::kChunk; ++c) {
-          cp_async16(to + c * kSlot, at[k] + c * 4, on);
-          cp_async16(to + (R::kChunk + c) * kSlot, at[k] + d12 + c * 4, on);
+          cp_async16(to + c * kSlot, at[k] + c * ln.ps, on);
+          cp_async16(to + (R::kChunk + c) * kSlot, at[k] + d12 + c * ln.ps, on);
         }
         at[k] += hs[k];
       }
@@ -345,7 +368,7 @@ __device__ __forceinline__ void walk_rows(const Units& un, const Lane& ln, uint4
 // ahead), so that entering a unit waits for neither.  Where.fetch(group, pos)
 // loads what the lane's position there is made of (false: it has no token);
 // Where.get(pos) is called a unit later.
-template <class Where> struct Angles {
+template <typename E, class Where> struct Angles {
   const Tables& t;
   const Lane& l;
   unsigned* bad;
@@ -382,34 +405,17 @@ template <class Where> struct Angles {
       p = 0;
     }
     const int64_t at = p * (t.R / 2) + l.o1;
-    const int es = t.cs_dtype == SA_F32 ? 4 : 2;
-    const uint4* c = reinterpret_cast<const uint4*>(static_cast<const uint8_t*>(t.cosv) + at * es);
-    const uint4* s = reinterpret_cast<const uint4*>(static_cast<const uint8_t*>(t.sinv) + at * es);
-    raw[0] = __ldg(c);
-    raw[2] = __ldg(s);
-    if (t.cs_dtype == SA_F32) {
-      raw[1] = __ldg(c + 1);
-      raw[3] = __ldg(s + 1);
-    }
-  }
-  template <typename CS> __device__ __forceinline__ void open(float2 (&c)[4], float2 (&s)[4]) {
-    Raw8<CS> a, b;
-#pragma unroll
-    for (int i = 0; i < (int)sizeof(CS) / 2; ++i) a.u[i] = raw[i], b.u[i] = raw[2 + i];
-    a.get(c);
-    b.get(s);
+    raw8_any<E>(t.cosv, at, l.ps, t.cs_dtype, raw[0], raw[1]);
+    raw8_any<E>(t.sinv, at, l.ps, t.cs_dtype, raw[2], raw[3]);
   }
   // cos and sin of the unit that the walk enters.
   __device__ __forceinline__ void enter(float2 (&c)[4], float2 (&s)[4]) {
     if (!have) {
 #pragma unroll
       for (int i = 0; i < 4; ++i) c[i] = splat(1.f), s[i] = splat(0.f);
-    } else if (t.cs_dtype == SA_F32) {
-      open<float>(c, s);
-    } else if (t.cs_dtype == SA_BF16) {
-      open<__nv_bfloat16>(c, s);
     } else {
-      open<__half>(c, s);
+      open8_any(raw[0], raw[1], t.cs_dtype, c);
+      open8_any(raw[2], raw[3], t.cs_dtype, s);
     }
     step();
   }
