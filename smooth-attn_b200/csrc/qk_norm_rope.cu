@@ -13,14 +13,13 @@
 // r is formed again from x, which the backward reads anyhow, so the forward
 // saves nothing.
 //
-// Bound: HBM.  Forward reads x and writes y; backward reads x and dy and
-// writes dx.  A warp owns a contiguous range of (token group, heads) items of
-// q or of k and streams their rows through shared memory (walk_rows): a
-// token's cos / sin stay in registers for its heads, and all warps' ranges are
-// equally long, so nothing is left over at the end.  dw: every lane keeps fp32
-// sums of its own 16 channels over the rows it meets, a block adds its warps'
-// sums in a fixed order and writes one row of partial sums for each of q and
-// k, and a second small kernel adds those in a fixed order: no atomics,
+// Bound: HBM.  Forward reads x and writes y (2 x 168 MB at [4, 32 + 8, 4096, 128]
+// bf16: 58 us, 0.90 of the measured copy rate), backward reads x and dy and writes
+// dx (85 us, 0.92).  The rows go through the walk of qk_rope.cuh, q's and k's warps
+// side by side in one launch, shared out by the work of each.  dw: every lane keeps
+// fp32 sums of its own 16 channels over the rows it meets, a block adds its warps'
+// sums in a fixed order and writes one row of partial sums for each of q and k,
+// and a second small kernel (4 us) adds those in a fixed order: no atomics,
 // bitwise the same from run to run.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>

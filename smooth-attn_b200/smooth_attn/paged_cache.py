@@ -173,7 +173,8 @@ def paged_release_pages(block_table, context_lens, done, free_pages, free_head, 
     the next to be taken.  Returns (context_lens with 0 for those requests, the new free_head); the
     arguments themselves are not changed.  block_table keeps its entries.  Giving back more pages than
     were taken (a request released twice from stale lengths) leaves those out that have no entry and
-    is reported by ``sa_device_status``.  done: bool [B].
+    is reported by ``sa_device_status``.  A page belongs to one request: pages that requests share
+    would be given back once for each.  done: bool [B].
     """
     block_size = int(block_size)
     traced = R._traced(block_table)
@@ -377,7 +378,7 @@ def paged_key_means(key_means, k_cache, block_table, context_lens, *, start_lens
     pages that context_lens[b] tokens fill are set, with start_lens only those that start_lens[b]
     tokens did not fill yet: after a step, pass the lengths before and after it.  Other pages' rows
     are left as they are.  A block_table entry outside the cache is skipped and reported by
-    ``sa_device_status``.  Returns key_means.
+    ``sa_device_status``.  At most 65535 sequences times key heads.  Returns key_means.
     """
     traced = R._traced(k_cache)
     key = None
@@ -460,7 +461,9 @@ def sp2norm_paged_select(q, key_means, block_table, context_lens, num_pages, *, 
     (the weight the attention would give the page's mean token, in 64 bits; ties go to the lowest
     page, NaN counts as the highest).  pages: int32 [B, H_kv, min(num_pages, max_blocks)], indices
     into the sequence's row of block_table, ascending, then -1; lens: int32 [B, H_kv], the tokens in
-    them.
+    them.  Lengths outside [0, max_blocks * block_size] are clamped; block_table entries outside the
+    cache are read as page 0 and reported by ``sa_device_status``.  At most 65535 sequences times key
+    heads.
     """
     num_pages, block_size = int(num_pages), int(block_size)
     block_table, context_lens, n = _check_query(q, key_means, block_table, context_lens, num_pages, block_size)

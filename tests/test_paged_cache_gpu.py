@@ -474,6 +474,17 @@ def test_rows_past_the_context_do_not_matter():
     assert _status() == _lib.SA_OK
 
 
+def test_lengths_outside_the_table_are_clamped():
+    q, kc, vc, means, bt = _cache(3, 4, 2, 128, 6, 16, torch.bfloat16, 12)
+    far, cut = _i32([1000, -5, 2 ** 31 - 1]), _i32([96, 0, 96])
+    a, b = (sa.sp2norm_sparse_paged_attention(q, kc, vc, means, bt, c, 3, return_pages=True) for c in (far, cut))
+    assert torch.equal(a[0], b[0]) and torch.equal(a[1], b[1]) and (a[0][1] == 0).all() and (a[1][1] == -1).all()
+    m0, m1 = torch.zeros_like(means), torch.zeros_like(means)
+    sa.paged_key_means(m0, kc, bt, far, start_lens=_i32([-9, -9, 2 ** 31 - 1]))
+    sa.paged_key_means(m1, kc, bt, _i32([96, 0, 0]))
+    assert torch.equal(m0, m1)
+
+
 def test_bad_pages_are_read_as_page_zero_and_reported():
     q, kc, vc, means, bt = _cache(1, 4, 2, 128, 8, 16, torch.bfloat16, 9)
     good = bt.clone()
