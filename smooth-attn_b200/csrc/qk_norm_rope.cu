@@ -103,11 +103,11 @@ __device__ __forceinline__ Part part_of_warp(const Side& q, const Side& k, const
 
 // Depth of the ring and resident blocks an SM: four forward blocks of 41 KB (16-bit)
 // and 128 registers a thread (three of 49 KB for fp32), three backward blocks of at most 65 KB and 168
-// registers (at 128 the backward spills).
+// registers (at 128 the backward spills), or two with a deeper ring: see bwd_blocks().
 template <typename E> constexpr int kFwdRing = sizeof(E) == 4 ? 6 : 10;
-template <typename E> constexpr int kBwdRing = sizeof(E) == 4 ? 4 : 6;
+template <typename E, int Blocks> constexpr int kBwdRing = sizeof(E) == 4 ? 4 : Blocks == 2 ? 9 : 6;
 template <typename E> constexpr int kFwdBlocks = sizeof(E) == 4 ? 3 : 4;
-constexpr int kBwdBlocks = 3;
+constexpr int kBwdBlocks = 3;  // at most
 
 // ---- forward ----------------------------------------------------------------
 
@@ -154,8 +154,8 @@ __global__ void __launch_bounds__(kWalkThreads, kFwdBlocks<E>)
 // ---- backward ---------------------------------------------------------------
 
 // part_sums: [2][gridDim.x][D] fp32 (q's rows, then k's), or null without dw.
-template <typename E, int L>
-__global__ void __launch_bounds__(kWalkThreads, kBwdBlocks)
+template <typename E, int L, int Blocks>
+__global__ void __launch_bounds__(kWalkThreads, Blocks)
     qk_norm_rope_bwd(Side q, Side k, Tables tb, Shape sh, float* part_sums) {
   extern __shared__ __align__(16) uint4 ring[];
   const Part part = part_of_warp(q, k, sh);
@@ -169,7 +169,7 @@ __global__ void __launch_bounds__(kWalkThreads, kBwdBlocks)
   load_weights<E>(sd.w, sh.w_dtype, ln, w1, w2);
   E* dx = nullptr;  // the row that comes next
   bool on = false;
-  walk_rows<E, 2, kBwdRing<E>>(
+  walk_rows<E, 2, kBwdRing<E, Blocks>>(
       part.un, ln, ring,
       [&](int64_t g) {
         const Token tk = token_of<L>(sh, g);
@@ -370,27 +370,50 @@ static int launch_fwd(const Side& q, const Side& k, const Tables& tb, const Shap
   }
 }
 
+// Blocks an SM of the backward pass.  Many whole 16-bit rows in full units are bound by
+// DRAM, and fewer warps that ask further ahead serve it better: [4, 32 + 8, 4096, 128] in
+// bf16 takes 84 us with two blocks of nine stages, 88-91 with three of six;
+// [4, 64 + 16, 4096, 64] 83-86 and 88-94; 16 + 16 heads of 128 70 and 72; 32 + 4 81 and 82.
+// Where instructions or the last round bind it, the third block's warps count: D = 80
+// (five lanes of eight) 79 with two and 72 with three; units of 6 heads (6 + 6 heads) 58 and
+// 53; 7 + 1 heads 49 and 46; 4 units a warp ([4, 32 + 8, 1024, 128]) 26 and 24 (8 units:
+// equal); D = 256 90 and 87.  D = 32 and fp32 rows: equal.
+static int bwd_blocks(const Side& q, const Side& k, int64_t D, int dtype) {
+  const int64_t warps = 2 * (int64_t)sm_count() * (kWalkThreads / 32);
+  const bool full = q.H + k.H >= 7 * (q.per + k.per), many = q.units + k.units >= 8 * warps;
+  return dtype != SA_F32 && (D == 64 || D == 128) && full && many ? 2 : kBwdBlocks;
+}
+
+template <typename E, int L, int Blocks>
+static int launch_bwd_lb(const Side& q, const Side& k, const Tables& tb, const Shape& sh, float* part, int64_t blocks,
+                         cudaStream_t st) {
+  constexpr int smem = Ring<E, 2, kBwdRing<E, Blocks>>::kBytesPerThread * kWalkThreads;
+  static_assert(smem >= kWalkThreads / 32 * 256 * 4, "the block's dw sums");
+  static_assert(Blocks * (smem + 1024) <= 227 * 1024, "the blocks of an SM");
+  const int rc = sa_record_cuda_error(opt_in_once<&qk_norm_rope_bwd<E, L, Blocks>, smem>());
+  if (rc != SA_OK) return rc;
+  qk_norm_rope_bwd<E, L, Blocks><<<(unsigned)blocks, kWalkThreads, smem, st>>>(q, k, tb, sh, part);
+  return sa_record_cuda_error(cudaGetLastError());
+}
+
 template <typename E, int L>
 static int launch_bwd_l(const Side& q, const Side& k, const Tables& tb, const Shape& sh, float* part, int64_t blocks,
-                        cudaStream_t st) {
-  constexpr int smem = Ring<E, 2, kBwdRing<E>>::kBytesPerThread * kWalkThreads;
-  static_assert(smem >= kWalkThreads / 32 * 256 * 4, "the block's dw sums");
-  static_assert(smem <= 74 * 1024, "three blocks an SM");
-  const int rc = sa_record_cuda_error(opt_in_once<&qk_norm_rope_bwd<E, L>, smem>());
-  if (rc != SA_OK) return rc;
-  qk_norm_rope_bwd<E, L><<<(unsigned)blocks, kWalkThreads, smem, st>>>(q, k, tb, sh, part);
-  return sa_record_cuda_error(cudaGetLastError());
+                        int per_sm, cudaStream_t st) {
+  if constexpr (sizeof(E) == 2 && (L == 4 || L == 8)) {
+    if (per_sm == 2) return launch_bwd_lb<E, L, 2>(q, k, tb, sh, part, blocks, st);
+  }
+  return launch_bwd_lb<E, L, kBwdBlocks>(q, k, tb, sh, part, blocks, st);
 }
 
 template <typename E>
 static int launch_bwd(const Side& q, const Side& k, const Tables& tb, const Shape& sh, float* part, int64_t blocks,
-                      cudaStream_t st) {
+                      int per_sm, cudaStream_t st) {
   switch (lanes_for(tb.D)) {
-    case 1: return launch_bwd_l<E, 1>(q, k, tb, sh, part, blocks, st);
-    case 2: return launch_bwd_l<E, 2>(q, k, tb, sh, part, blocks, st);
-    case 4: return launch_bwd_l<E, 4>(q, k, tb, sh, part, blocks, st);
-    case 8: return launch_bwd_l<E, 8>(q, k, tb, sh, part, blocks, st);
-    default: return launch_bwd_l<E, 16>(q, k, tb, sh, part, blocks, st);
+    case 1: return launch_bwd_l<E, 1>(q, k, tb, sh, part, blocks, per_sm, st);
+    case 2: return launch_bwd_l<E, 2>(q, k, tb, sh, part, blocks, per_sm, st);
+    case 4: return launch_bwd_l<E, 4>(q, k, tb, sh, part, blocks, per_sm, st);
+    case 8: return launch_bwd_l<E, 8>(q, k, tb, sh, part, blocks, per_sm, st);
+    default: return launch_bwd_l<E, 16>(q, k, tb, sh, part, blocks, per_sm, st);
   }
 }
 
@@ -484,13 +507,14 @@ extern "C" int sa_qk_norm_rope_bwd(const void* q, const void* k, const void* dq_
   const Side a = side_of(q, dq, dq_out, q_weight, hq, q_strides, dq_strides, dqo_strides, groups, C);
   const Side b = side_of(k, dk, dk_out, k_weight, hk, k_strides, dk_strides, dko_strides, groups, C);
   Shape sh{B * T, work ? T : 1, 0, w_dtype, FastDiv(work ? (uint32_t)T : 1u)};
-  const int64_t blocks = plan(a, b, &sh, kBwdBlocks);
+  const int per_sm = bwd_blocks(a, b, D, dtype);
+  const int64_t blocks = plan(a, b, &sh, per_sm);
   float* part = dw ? static_cast<float*>(workspace) : nullptr;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   if (blocks > 0) {
-    rc = dtype == SA_F32    ? launch_bwd<float>(a, b, tb, sh, part, blocks, st)
-         : dtype == SA_BF16 ? launch_bwd<__nv_bfloat16>(a, b, tb, sh, part, blocks, st)
-                            : launch_bwd<__half>(a, b, tb, sh, part, blocks, st);
+    rc = dtype == SA_F32    ? launch_bwd<float>(a, b, tb, sh, part, blocks, per_sm, st)
+         : dtype == SA_BF16 ? launch_bwd<__nv_bfloat16>(a, b, tb, sh, part, blocks, per_sm, st)
+                            : launch_bwd<__half>(a, b, tb, sh, part, blocks, per_sm, st);
     if (rc != SA_OK) return rc;
   }
   if (dw) {  // also without rows: zeros

@@ -160,7 +160,8 @@ def test_table_types(cs):
 
 @pytest.mark.parametrize("B,Hq,Hkv,T,D,R,dt,ps", [
     (2, 16, 4, 2100, 128, 128, torch.bfloat16, "batch32"),
-    (3, 32, 8, 3001, 128, 128, torch.bfloat16, "batch64"),  # whole units of heads: angles through shared memory
+    (3, 32, 8, 3001, 128, 128, torch.bfloat16, "batch64"),  # many whole rows in full units: fewer, deeper warps
+    (2, 64, 16, 3801, 64, 32, torch.float16, "row32"),
     (2, 24, 8, 5003, 64, 32, torch.float16, "none"),
     (2, 20, 9, 4099, 80, 80, torch.bfloat16, "row32"),  # heads that units do not divide
     (1, 8, 16, 5001, 128, 64, torch.float32, "row64"),
