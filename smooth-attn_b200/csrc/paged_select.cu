@@ -23,13 +23,15 @@
 //
 // Bound.  32 sequences of 5000 to 8192 tokens, 64 pages of each and 8 key heads
 // (27 MB of mean keys, 134 MB of chosen pages: 25 us at the measured copy rate):
-// scores and choice 24 us, the decode 35 us.  The scores are bound by the 64-bit
-// pipes: half of a product's eight columns are empty for groups of four heads, and
-// 17 cycles a product make 9 us.  (fp32 scores with proven bounds and 64 bits
-// where those overlap were built too: 164 instructions for two rows, a second
-// order statistic, and the rare 64-bit path in some block of every launch: 34 us
-// against 26.)  One sequence of 32768 tokens, 128 pages: 12 us + 10 us, launches
-// and the chain of dependent reads.
+// scores and choice 24 us (21 with the means in L2), the decode 35 us.  Of the 21 the choice
+// is 4; the products are 9 to 11 on the 64-bit matrix pipe, 17 cycles each, half of
+// their eight columns empty for groups of four heads; the rest is the launch and the
+// chain from lengths to page ids to rows.  Built too: fp32 scores with proven bounds and 64
+// bits where those overlap (164 instructions for two rows, a second order
+// statistic, and the rare 64-bit path in some block of every launch: 34 us against
+// 26), and plain 64-bit multiply-adds of the four heads alone with the rows through a ring in
+// shared memory (20 us against 21, and groups of one head 15.5 against 14.4).  One sequence
+// of 32768 tokens, 128 pages: 12 us + 10 us, launches and the chain of dependent reads.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
