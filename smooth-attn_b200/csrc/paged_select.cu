@@ -31,7 +31,7 @@
 // statistic, and the rare 64-bit path in some block of every launch: 34 us against
 // 26), and plain 64-bit multiply-adds of the four heads alone with the rows through a ring in
 // shared memory (20 us against 21, and groups of one head 15.5 against 14.4).  One sequence
-// of 32768 tokens, 128 pages: 12 us + 10 us, launches and the chain of dependent reads.
+// of 32768 tokens, 128 pages: 11 us + 10 us, launches and the chain of dependent reads.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
@@ -225,14 +225,18 @@ __device__ __forceinline__ void choose_pages(const SelectArgs& a, int u, ChooseS
   const int32_t* bt = a.bt + (int64_t)b * a.max_blocks;
   const unsigned long long* keys = a.keys + (int64_t)u * a.max_blocks;
   // read beside the length, not after it: what lies behind the candidates is not looked at
+  // (so are the pages' places in the cache, which only what is chosen needs)
   unsigned long long mine[kKeep];
+  int place[kKeep];
 #pragma unroll
   for (int j = 0; j < kKeep; ++j) {
     const int i = j * kSelThreads + tid;
+    place[j] = i < a.max_blocks && a.table ? __ldg(bt + i) : 0;
     mine[j] = i < a.max_blocks && a.max_blocks > a.K ? __ldcg(keys + i) : 0;  // (other SMs' writes)
   }
   const Seq s = seq_of(a, b);
   const int m = s.n - 1, need = min(a.K, s.n) - 1;  // of the m candidates
+  const int last_place = tid == 0 && m >= 0 && a.table ? __ldg(bt + m) : 0;
   // keys above hi are chosen, and `rest` of those in [lo, hi], lowest pages first
   unsigned long long lo = 0, hi = ~0ull;
   int rest = need;
@@ -339,11 +343,10 @@ __device__ __forceinline__ void choose_pages(const SelectArgs& a, int u, ChooseS
   // ordered write: pages in ascending order, the last one behind them
   int* const pg = a.pages ? a.pages + (int64_t)u * a.K : nullptr;
   int* const tb = a.table ? a.table + (int64_t)u * a.K : nullptr;
-  auto put = [&](int at, int page) {
+  auto put = [&](int at, int page, int64_t phys) {
     if (!SA_DCHECK(at < a.K && page < a.max_blocks)) return;
     if (pg) pg[at] = page;
     if (tb) {
-      int64_t phys = bt[page];
       if (phys < 0 || phys >= a.num_blocks) {
         if (h == 0) atomicAdd(&g_bad_pages, 1u);
         phys = 0;
@@ -352,7 +355,10 @@ __device__ __forceinline__ void choose_pages(const SelectArgs& a, int u, ChooseS
     }
   };
   if (m <= need) {
-    for (int i = tid; i < m; i += kSelThreads) put(i, i);
+#pragma unroll
+    for (int j = 0; j < kKeep; ++j)
+      if (j * kSelThreads + tid < m) put(j * kSelThreads + tid, j * kSelThreads + tid, place[j]);
+    for (int i = kKeep * kSelThreads + tid; i < m; i += kSelThreads) put(i, i, __ldg(bt + i));
   } else if (need > 0) {
     // a batch of kKeep * kSelThreads pages at a time; a count is in-range keys, and above ones << 16
     int base = 0, base_in = 0;  // chosen and in-range keys of earlier batches
@@ -395,7 +401,9 @@ __device__ __forceinline__ void choose_pages(const SelectArgs& a, int u, ChooseS
         const int ab_before = (c >> 16) + __popc(ab_w[j] & below);
         const bool in = (in_w[j] >> lane) & 1, above = (ab_w[j] >> lane) & 1;
         // chosen before this page: the above ones, and of the in-range ones the first `rest`
-        if (above || (in && in_before < rest)) put(base + ab_before + min(in_before, rest) - min(base_in, rest), i);
+        if (above || (in && in_before < rest))
+          put(base + ab_before + min(in_before, rest) - min(base_in, rest), i,
+              i0 == 0 ? place[j] : a.table ? __ldg(bt + i) : 0);
       }
       const int c = found_count;
       base += (c >> 16) + min(base_in + (c & 0xffff), rest) - min(base_in, rest);
@@ -405,7 +413,7 @@ __device__ __forceinline__ void choose_pages(const SelectArgs& a, int u, ChooseS
   }
   const int chosen = s.n > 0 ? need + 1 : 0;
   if (tid == 0) {
-    if (s.n > 0) put(need, m);
+    if (s.n > 0) put(need, m, last_place);
     a.lens[u] = s.n > 0 ? need * a.bs + s.ctx - m * a.bs : 0;
   }
   for (int i = chosen + tid; i < a.K; i += kSelThreads) {
