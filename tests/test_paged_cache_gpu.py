@@ -455,6 +455,17 @@ def test_choice_of_a_long_context():
     _attend(out, q, kc, vc, bt, ctx, want)
 
 
+@pytest.mark.parametrize("K", [9000, 8999, 8300])
+def test_choice_of_nearly_all_of_a_long_table(K):
+    """Every page taken, or all but a few, among more than a block keeps in registers."""
+    q, kc, vc, means, bt = _cache(2, 2, 1, 32, 9000, 1, torch.float16, 15)
+    ctx = [9000, 8301]
+    want = choose64(q, means, bt, ctx, K, 32 ** -0.5, 1)
+    out, pages = sa.sp2norm_sparse_paged_attention(q, kc, vc, means, bt, _i32(ctx), K, block_size=1, return_pages=True)
+    assert pages.tolist() == [[r + [-1] * (K - len(r)) for r in row] for row in want]
+    _attend(out, q, kc, vc, bt, ctx, want)
+
+
 def test_rows_past_the_context_do_not_matter():
     """NaN in the cache behind the last token and in unused pages, -1 in the table behind it."""
     q, kc, vc, means, bt = _cache(2, 8, 2, 128, 12, 16, torch.bfloat16, 8)
