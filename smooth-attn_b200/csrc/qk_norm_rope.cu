@@ -14,7 +14,7 @@
 // saves nothing.
 //
 // Bound: HBM.  Forward reads x and writes y (2 x 168 MB at [4, 32 + 8, 4096, 128]
-// bf16: 58 us, 0.90 of the measured copy rate), backward reads x and dy and writes
+// bf16: 57 us, 0.92 of the measured copy rate), backward reads x and dy and writes
 // dx (85 us, 0.92).  The rows go through the walk of qk_rope.cuh, q's and k's warps
 // side by side in one launch, shared out by the work of each.  dw: every lane keeps
 // fp32 sums of its own 16 channels over the rows it meets, a block adds its warps'

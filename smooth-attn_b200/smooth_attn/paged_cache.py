@@ -141,8 +141,9 @@ def paged_assign_slots(block_table, context_lens, new_lens, free_pages, free_hea
 
 def _assign_plan(block_table, free_pages, num_tokens, block_size):
     B, max_blocks = block_table.shape
-    return (block_table.get_device(), _ld(block_table), free_pages.shape[0], B,
-            [num_tokens, B + 1, B, 1], (B, num_tokens, max_blocks, block_size))
+    return (block_table.get_device(), *R._held("sa_paged_assign_slots", 1, _ld(block_table)),
+            *R._held("sa_paged_assign_slots", 5, free_pages.shape[0]), [num_tokens, B + 1, B, 1],
+            R._held("sa_paged_assign_slots", 12, B, num_tokens, max_blocks, block_size))
 
 
 def _assign_direct(block_table, context_lens, new_lens, free_pages, free_head, num_tokens, block_size):
@@ -152,8 +153,8 @@ def _assign_direct(block_table, context_lens, new_lens, free_pages, free_head, n
 
 
 def _assign_call(plan, block_table, context_lens, new_lens, free_pages, free_head):
-    device, ld, num_free, B, parts, dims = plan
-    N = dims[1]
+    device, ld, num_free, parts, dims = plan
+    N, _, B, _ = parts
     slots = block_table.new_empty(N, dtype=torch.int64)
     i32 = block_table.new_empty(N + 2 * B + 2)
     p = i32.data_ptr()
@@ -204,7 +205,9 @@ def paged_release_pages(block_table, context_lens, done, free_pages, free_head, 
 
 
 def _release_plan(block_table, free_pages, block_size):
-    return (block_table.get_device(), _ld(block_table), free_pages.shape[0], (*block_table.shape, block_size))
+    return (block_table.get_device(), *R._held("sa_paged_release_pages", 1, _ld(block_table)),
+            *R._held("sa_paged_release_pages", 5, free_pages.shape[0]),
+            R._held("sa_paged_release_pages", 9, *block_table.shape, block_size))
 
 
 def _release_direct(block_table, context_lens, done, free_pages, free_head, block_size):
@@ -307,10 +310,13 @@ class _AppendPlan:
     def __init__(self, q, k, v, k_cache, cos, q_weight, k_weight, positions, eps):
         N, H_q, D = q.shape
         num_blocks, H_kv, block_size, _ = k_cache.shape
-        self.w, self.cs, pos_bytes, _, rows = R._row_args(cos, cos, q_weight, k_weight, positions, N)
-        self.rest = (pos_bytes, rows, N, H_q, H_kv, D, 0 if cos is None else 2 * cos.shape[1], num_blocks, block_size,
-                     R._strides(q), R._strides(k), R._strides(v), 0.0 if eps is None else float(eps),
-                     int(eps is not None), K._DTYPE_CODE[q.dtype])
+        w, cs, pos_bytes, _, rows = R._row_args(cos, cos, q_weight, k_weight, positions, N)
+        (self.w,) = R._held("sa_qk_norm_rope_paged_append", 9, w)
+        (self.cs,) = R._held("sa_qk_norm_rope_paged_append", 12, cs)
+        self.rest = R._held(
+            "sa_qk_norm_rope_paged_append", 14, pos_bytes, rows, N, H_q, H_kv, D, 0 if cos is None else 2 * cos.shape[1],
+            num_blocks, block_size, R._strides(q), R._strides(k), R._strides(v), 0.0 if eps is None else float(eps),
+            int(eps is not None), K._DTYPE_CODE[q.dtype])
         self.device = q.get_device()
 
     def run(self, q, k, v, k_cache, v_cache, slot_mapping, cos, sin, positions, q_weight, k_weight):
@@ -410,7 +416,8 @@ def paged_key_means(key_means, k_cache, block_table, context_lens, *, start_lens
 def _means_plan(k_cache, block_table):
     num_blocks, H_kv, block_size, D = k_cache.shape
     B, max_blocks = block_table.shape
-    return k_cache.get_device(), (B, H_kv, num_blocks, block_size, max_blocks, D, K._DTYPE_CODE[k_cache.dtype])
+    return k_cache.get_device(), R._held("sa_paged_key_means", 5, B, H_kv, num_blocks, block_size, max_blocks, D,
+                                         K._DTYPE_CODE[k_cache.dtype])
 
 
 def _means_direct(key_means, k_cache, block_table, context_lens, start_lens):
@@ -549,7 +556,8 @@ def _sparse_plan(q, key_means, block_table, n, scale, block_size):
     if nbytes < 0:
         _lib.check(nbytes, "sa_sparse_paged_decode_workspace_size")
     return (q.get_device(), nbytes, (B, H_q, D), (B, H_kv, n),
-            (B, H_q, H_kv, num_blocks, block_size, max_blocks, n, D, scale, code))
+            R._held("sa_sparse_paged_decode", 9, nbytes, B, H_q, H_kv, num_blocks, block_size, max_blocks, n, D, scale,
+                    code))
 
 
 def _sparse_call(plan, q, k_cache, v_cache, key_means, block_table, context_lens, with_pages):
@@ -561,7 +569,7 @@ def _sparse_call(plan, q, k_cache, v_cache, key_means, block_table, context_lens
     ws = block_table.new_empty(nbytes, dtype=torch.uint8)
     st = _lib.load().sa_sparse_paged_decode(
         q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), key_means.data_ptr(), out.data_ptr(),
-        block_table.data_ptr(), context_lens.data_ptr(), pages.data_ptr() if with_pages else None, ws.data_ptr(), nbytes,
+        block_table.data_ptr(), context_lens.data_ptr(), pages.data_ptr() if with_pages else None, ws.data_ptr(),
         *dims, torch._C._cuda_getCurrentRawStream(device))
     _lib.check(st, "sa_sparse_paged_decode")
     return out, pages
