@@ -209,7 +209,8 @@ __global__ void __launch_bounds__(kWalkThreads, Blocks)
             gx = ffma2(v2[i], x2[i], gx);
           }
           const float sum = row_sum<L>(ss.x + ss.y), dot = row_sum<L>(gx.x + gx.y);
-          const float r = rsqrtf(fmaf(sum, tb.inv_d, tb.eps));
+          // (a row that does not exist is zeros: without eps its root would be infinite and 0 * inf reach dw)
+          const float r = on ? rsqrtf(fmaf(sum, tb.inv_d, tb.eps)) : 0.f;
           const float2 r2 = splat(r), m2 = splat(-(dot * tb.inv_d) * r * r * r);
 #pragma unroll
           for (int i = 0; i < 4; ++i) {

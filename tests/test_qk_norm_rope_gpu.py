@@ -446,3 +446,21 @@ def test_attention_trains_through_it(compiled):
         # yq / yk may round to the other neighbour and dQ sums in another order: 2^-7 of the gradients' size
         rel = lambda a, b: ((a.double() - b).norm() / b.norm()).item()  # noqa: E731
         assert rel(grads[i], r[2]) < 2.0 ** -7 and rel(grads[3 + i], r[4]) < 2.0 ** -7
+
+
+@pytest.mark.parametrize("eps", [0.0, 1e-50])  # (the second is 0 in fp32)
+@pytest.mark.parametrize("B,Hq,Hkv,T,D,R,dt", [
+    (1, 1, 1, 1, 128, 128, torch.bfloat16), (1, 3, 1, 7, 16, 16, torch.float32), (3, 5, 2, 5, 80, 32, torch.float16),
+    (1, 4, 4, 33, 64, 64, torch.float16), (2, 4, 2, 27, 128, 64, torch.float32), (1, 2, 1, 5, 256, 256, torch.bfloat16),
+])
+def test_gradients_without_eps(B, Hq, Hkv, T, D, R, dt, eps):
+    """Rows that are not zero need no eps; what lies behind the last token adds nothing to the weights' gradients."""
+    q, k, dq, dk, wq, wk, cos, sin, pos, full, _ = _make((B, Hq, Hkv, T, D, R, dt, torch.float32, True, "batch32"))
+    ins = [t.detach().requires_grad_(True) for t in (q, k, wq, wk)]
+    y = sa.qk_norm_rope(ins[0], ins[1], cos, sin, q_weight=ins[2], k_weight=ins[3], eps=eps, positions=pos)
+    g = torch.autograd.grad(y, ins, (dq, dk))
+    for x, w, o, dx, dw, dy in ((q, wq, y[0], g[0], g[2], dq), (k, wk, y[1], g[1], g[3], dk)):
+        ref = _ref64(x, w, cos, sin, full, eps, dy)
+        _check(o.detach(), ref[0], ref[1])
+        _check(dx, ref[2], ref[3])
+        _check(dw, ref[4], ref[5])
