@@ -493,10 +493,12 @@ int kernel_choice() {
   return 1;
 }
 
-// Resident CTAs per SM of one instantiation at one dynamic smem size, and
-// the one-time opt-in to that much dynamic shared memory, cached per device
-// (the per-call cost of the two runtime queries is several microseconds,
-// comparable to a whole short decode).
+// Resident CTAs per SM of one instantiation at one dynamic smem size, cached
+// per device, and the opt-in to that much dynamic shared memory (the per-call
+// cost of the two runtime queries is several microseconds, comparable to a
+// whole short decode).  The opt-in is a limit of the kernel, not of a launch,
+// and only ever raised: a cache of smaller pages in between must not take it
+// away from a size that is found in the cache.
 struct OccEntry {
   const void* fn;
   size_t smem;
@@ -515,13 +517,17 @@ int occupancy(size_t smem) {
   std::lock_guard<std::mutex> lk(g_occ_mu);
   for (int i = 0; i < g_nocc; ++i)
     if (g_occ[i].fn == (const void*)kfn && g_occ[i].smem == smem && g_occ[i].dev == dev) return g_occ[i].occ;
+  static size_t limit = 0;  // the largest that this kernel has had on any device
   int n = 0;
   bool cached = true;
-  if (cudaFuncSetAttribute(kfn, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) != cudaSuccess ||
+  const size_t want = std::max(limit, smem);
+  if (cudaFuncSetAttribute(kfn, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)want) != cudaSuccess ||
       cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, kfn, kPgWarps * 32, smem) != cudaSuccess || n <= 0) {
     cudaGetLastError();
     n = std::max<int>(1, std::min<int>(8, (int)((227 * 1024) / (smem + 1024))));
     cached = false;  // no device here: estimate, retry next time
+  } else {
+    limit = want;
   }
   if (cached && g_nocc < 256) g_occ[g_nocc++] = {(const void*)kfn, smem, dev, n};
   return n;

@@ -654,3 +654,18 @@ def test_a_captured_decode_step():
         want = step(eager)
         assert torch.equal(out, want)
     assert all(torch.equal(a, b) for a, b in zip(st, eager))
+
+
+@pytest.mark.parametrize("Hq,Hkv,D,sizes", [(2, 2, 32, (16, 8, 16)), (4, 1, 32, (16, 8, 1, 16)),
+                                            (2, 2, 128, (16, 20, 16)), (3, 1, 256, (16, 5, 16)), (8, 1, 64, (64, 8, 64))])
+def test_decode_of_several_page_sizes_in_one_process(Hq, Hkv, D, sizes):
+    """A cache of smaller pages in between does not take the larger ones' shared memory away."""
+    for dt in (torch.float16, torch.bfloat16):
+        for bs in sizes:
+            mb = 320 // bs
+            q, kc, vc, means, bt = _cache(2, Hq, Hkv, D, mb, bs, dt, 40 + bs)
+            ctx = [mb * bs, mb * bs - bs // 2 - 1]
+            every = [[list(range(-(-c // bs)))] * Hkv for c in ctx]
+            _attend(sa.sp2norm_paged_attention(q, kc, vc, bt, _i32(ctx), block_size=bs), q, kc, vc, bt, ctx, every)
+            out = sa.sp2norm_sparse_paged_attention(q, kc, vc, means, bt, _i32(ctx), mb, block_size=bs)
+            _attend(out, q, kc, vc, bt, ctx, every)
