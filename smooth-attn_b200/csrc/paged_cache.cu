@@ -295,7 +295,7 @@ template <int L> struct Where {
   }
 };
 
-template <typename E, int L>
+template <typename E, int L, bool Partial>
 __global__ void __launch_bounds__(kWalkThreads, kAppendBlocks) qk_norm_rope_append(AppendArgs a, Tables tb) {
   extern __shared__ __align__(16) uint4 ring[];
   const int64_t warp = (int64_t)blockIdx.x * (kWalkThreads / 32) + (threadIdx.x >> 5);
@@ -360,7 +360,7 @@ __global__ void __launch_bounds__(kWalkThreads, kAppendBlocks) qk_norm_rope_appe
         y += h * yh + ln.o1;
       },
       [&](Raw8<E> (&rows)[2]) {
-        if (side < 2) norm_rope<E, L>(tb, map, rows[0], rows[1]);
+        if (side < 2) norm_rope<E, L, Partial>(tb, ln, map, rows[0], rows[1]);
         if (padding) rows[0].zero(), rows[1].zero();
         if (write && SA_DCHECK(ln.o2 + ln.ps + 4 <= tb.D)) {
           rows[0].store(y, ln.ps);
@@ -376,15 +376,20 @@ template <typename F> static int opt_in(F* f, size_t bytes) {
   return sa_record_cuda_error(cudaFuncSetAttribute(f, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes));
 }
 
-template <typename E, int L>
-static int launch_append_l(const AppendArgs& a, const Tables& tb, cudaStream_t st) {
+template <typename E, int L, bool Partial>
+static int launch_append_lp(const AppendArgs& a, const Tables& tb, cudaStream_t st) {
   constexpr int smem = Ring<E, 1, kAppendRing>::kBytesPerThread * kWalkThreads;
   static_assert(smem <= 56 * 1024, "three blocks an SM");
-  const int rc = sa_record_cuda_error(opt_in_once<&qk_norm_rope_append<E, L>, smem>());
+  const int rc = sa_record_cuda_error(opt_in_once<&qk_norm_rope_append<E, L, Partial>, smem>());
   if (rc != SA_OK) return rc;
   const unsigned blocks = (unsigned)(a.warps / (kWalkThreads / 32));
-  qk_norm_rope_append<E, L><<<blocks, kWalkThreads, smem, st>>>(a, tb);
+  qk_norm_rope_append<E, L, Partial><<<blocks, kWalkThreads, smem, st>>>(a, tb);
   return sa_record_cuda_error(cudaGetLastError());
+}
+
+template <typename E, int L>
+static int launch_append_l(const AppendArgs& a, const Tables& tb, cudaStream_t st) {
+  return tb.R < tb.D ? launch_append_lp<E, L, true>(a, tb, st) : launch_append_lp<E, L, false>(a, tb, st);
 }
 
 template <typename E>

@@ -111,7 +111,7 @@ constexpr int kBwdBlocks = 3;  // at most
 
 // ---- forward ----------------------------------------------------------------
 
-template <typename E, int L>
+template <typename E, int L, bool Partial>
 __global__ void __launch_bounds__(kWalkThreads, kFwdBlocks<E>)
     qk_norm_rope_fwd(Side q, Side k, Tables tb, Shape sh) {
   extern __shared__ __align__(16) uint4 ring[];
@@ -142,7 +142,7 @@ __global__ void __launch_bounds__(kWalkThreads, kFwdBlocks<E>)
         y = static_cast<E*>(sd.y) + tk.b * sd.yb + tk.t * sd.yt + h * sd.yh + ln.o1;
       },
       [&](Raw8<E> (&rows)[2]) {
-        norm_rope<E, L>(tb, map, rows[0], rows[1]);
+        norm_rope<E, L, Partial>(tb, ln, map, rows[0], rows[1]);
         if (on && SA_DCHECK(ln.o2 + ln.ps + 4 <= tb.D)) {
           rows[0].store(y, ln.ps);
           rows[1].store(y + (ln.o2 - ln.o1), ln.ps);
@@ -154,7 +154,7 @@ __global__ void __launch_bounds__(kWalkThreads, kFwdBlocks<E>)
 // ---- backward ---------------------------------------------------------------
 
 // part_sums: [2][gridDim.x][D] fp32 (q's rows, then k's), or null without dw.
-template <typename E, int L, int Blocks>
+template <typename E, int L, int Blocks, bool Partial>
 __global__ void __launch_bounds__(kWalkThreads, Blocks)
     qk_norm_rope_bwd(Side q, Side k, Tables tb, Shape sh, float* part_sums) {
   extern __shared__ __align__(16) uint4 ring[];
@@ -193,8 +193,10 @@ __global__ void __launch_bounds__(kWalkThreads, Blocks)
         rows[3].get(g2);
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          const float2 n1 = ffma2(g1[i], c[i], fmul2(g2[i], s[i]));
-          g2[i] = fsub2(fmul2(g2[i], c[i]), fmul2(g1[i], s[i]));
+          float2 t1 = fmul2(g2[i], s[i]), t2 = fmul2(g1[i], s[i]);
+          if constexpr (Partial) t1 = pair_only(ln, t1, -0.f), t2 = pair_only(ln, t2, 0.f);
+          const float2 n1 = ffma2(g1[i], c[i], t1);
+          g2[i] = fsub2(fmul2(g2[i], c[i]), t2);
           g1[i] = n1;
         }
         if (tb.normalize) {
@@ -348,15 +350,22 @@ static int64_t plan(const Side& q, const Side& k, Shape* sh, int per_sm) {
   return blocks;
 }
 
-template <typename E, int L>
-static int launch_fwd_l(const Side& q, const Side& k, const Tables& tb, const Shape& sh, int64_t blocks,
+template <typename E, int L, bool Partial>
+static int launch_fwd_lp(const Side& q, const Side& k, const Tables& tb, const Shape& sh, int64_t blocks,
                         cudaStream_t st) {
   constexpr int smem = Ring<E, 1, kFwdRing<E>>::kBytesPerThread * kWalkThreads;
   static_assert(smem <= 56 * 1024, "four blocks an SM");
-  const int rc = sa_record_cuda_error(opt_in_once<&qk_norm_rope_fwd<E, L>, smem>());
+  const int rc = sa_record_cuda_error(opt_in_once<&qk_norm_rope_fwd<E, L, Partial>, smem>());
   if (rc != SA_OK) return rc;
-  qk_norm_rope_fwd<E, L><<<(unsigned)blocks, kWalkThreads, smem, st>>>(q, k, tb, sh);
+  qk_norm_rope_fwd<E, L, Partial><<<(unsigned)blocks, kWalkThreads, smem, st>>>(q, k, tb, sh);
   return sa_record_cuda_error(cudaGetLastError());
+}
+
+template <typename E, int L>
+static int launch_fwd_l(const Side& q, const Side& k, const Tables& tb, const Shape& sh, int64_t blocks,
+                        cudaStream_t st) {
+  return tb.R < tb.D ? launch_fwd_lp<E, L, true>(q, k, tb, sh, blocks, st)
+                     : launch_fwd_lp<E, L, false>(q, k, tb, sh, blocks, st);
 }
 
 template <typename E>
@@ -385,16 +394,23 @@ static int bwd_blocks(const Side& q, const Side& k, int64_t D, int dtype) {
   return dtype != SA_F32 && (D == 64 || D == 128) && full && many ? 2 : kBwdBlocks;
 }
 
-template <typename E, int L, int Blocks>
-static int launch_bwd_lb(const Side& q, const Side& k, const Tables& tb, const Shape& sh, float* part, int64_t blocks,
+template <typename E, int L, int Blocks, bool Partial>
+static int launch_bwd_lbp(const Side& q, const Side& k, const Tables& tb, const Shape& sh, float* part, int64_t blocks,
                          cudaStream_t st) {
   constexpr int smem = Ring<E, 2, kBwdRing<E, Blocks>>::kBytesPerThread * kWalkThreads;
   static_assert(smem >= kWalkThreads / 32 * 256 * 4, "the block's dw sums");
   static_assert(Blocks * (smem + 1024) <= 227 * 1024, "the blocks of an SM");
-  const int rc = sa_record_cuda_error(opt_in_once<&qk_norm_rope_bwd<E, L, Blocks>, smem>());
+  const int rc = sa_record_cuda_error(opt_in_once<&qk_norm_rope_bwd<E, L, Blocks, Partial>, smem>());
   if (rc != SA_OK) return rc;
-  qk_norm_rope_bwd<E, L, Blocks><<<(unsigned)blocks, kWalkThreads, smem, st>>>(q, k, tb, sh, part);
+  qk_norm_rope_bwd<E, L, Blocks, Partial><<<(unsigned)blocks, kWalkThreads, smem, st>>>(q, k, tb, sh, part);
   return sa_record_cuda_error(cudaGetLastError());
+}
+
+template <typename E, int L, int Blocks>
+static int launch_bwd_lb(const Side& q, const Side& k, const Tables& tb, const Shape& sh, float* part, int64_t blocks,
+                         cudaStream_t st) {
+  return tb.R < tb.D ? launch_bwd_lbp<E, L, Blocks, true>(q, k, tb, sh, part, blocks, st)
+                     : launch_bwd_lbp<E, L, Blocks, false>(q, k, tb, sh, part, blocks, st);
 }
 
 template <typename E, int L>

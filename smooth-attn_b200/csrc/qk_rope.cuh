@@ -182,16 +182,29 @@ struct Map {
   }
 };
 
-// y of one row from its two raw chunks (zeros in lanes without one).
-template <typename E, int L>
-__device__ __forceinline__ void norm_rope(const Tables& t, const Map& m, Raw8<E>& a, Raw8<E>& b) {
+// v where the lane's chunks are a rotated pair, else `none`: -0 in a sum, 0 behind a minus, which leave even the
+// sign of a zero alone.
+__device__ __forceinline__ float2 pair_only(const Lane& l, float2 v, float none) {
+  return make_float2(l.rotated ? v.x : none, l.rotated ? v.y : none);
+}
+
+// y of one row from its two raw chunks (zeros in lanes without one).  Partial:
+// some channels are not rotated, and there the other one of the pair is left out:
+// times a sine of 0 an infinity in it would arrive as NaN.  (The selects cost rows of
+// 80 channels of which 16 are rotated 3 % in both directions, a branch 5 to 8 %; rows
+// that are rotated throughout need none, hence the parameter: with a branch for all the
+// backward of [4, 32 + 8, 4096, 128] took 90 us for 87.5.)
+template <typename E, int L, bool Partial>
+__device__ __forceinline__ void norm_rope(const Tables& t, const Lane& l, const Map& m, Raw8<E>& a, Raw8<E>& b) {
   float2 x1[4], x2[4], y1[4], y2[4];
   a.get(x1);
   b.get(x2);
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
-    y1[i] = ffma2(x1[i], m.a1[i], fmul2(x2[i], m.b1[i]));
-    y2[i] = ffma2(x2[i], m.a2[i], fmul2(x1[i], m.b2[i]));
+    float2 t1 = fmul2(x2[i], m.b1[i]), t2 = fmul2(x1[i], m.b2[i]);
+    if constexpr (Partial) t1 = pair_only(l, t1, -0.f), t2 = pair_only(l, t2, -0.f);
+    y1[i] = ffma2(x1[i], m.a1[i], t1);
+    y2[i] = ffma2(x2[i], m.a2[i], t2);
   }
   if (t.normalize) {
     float2 ss = fmul2(x1[0], x1[0]);

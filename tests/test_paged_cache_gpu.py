@@ -669,3 +669,30 @@ def test_decode_of_several_page_sizes_in_one_process(Hq, Hkv, D, sizes):
             _attend(sa.sp2norm_paged_attention(q, kc, vc, bt, _i32(ctx), block_size=bs), q, kc, vc, bt, ctx, every)
             out = sa.sp2norm_sparse_paged_attention(q, kc, vc, means, bt, _i32(ctx), mb, block_size=bs)
             _attend(out, q, kc, vc, bt, ctx, every)
+
+
+# ------------------------------------------------------------------ odd calls
+
+
+def test_append_copies_infinities_without_touching_their_neighbours():
+    """An infinity in channel R + n of token n's query and key, without a norm: copied, and nothing else changes."""
+    R, D, bs = 16, 64, 8
+    N = D - R
+    cos, sin = _angles(N, R)
+    n = torch.arange(N, device=CUDA)
+    for dt in (torch.bfloat16, torch.float16):
+        q, k, v = (t.contiguous() for t in _append_inputs(N, 4, 2, D, dt, 31))
+        for value in (math.inf, math.nan):
+            res = []
+            for bad in (False, True):
+                kc, vc = (torch.zeros(N // bs, 2, bs, D, device=CUDA, dtype=dt) for _ in range(2))
+                if bad:
+                    q[n, :, R + n] = value
+                    k[n, :, R + n] = value
+                res.append((sa.qk_norm_rope_paged_append(q, k, v, kc, vc, n, cos, sin, positions=n, eps=None),
+                            kc.transpose(1, 2).reshape(N, 2, D), vc))
+            for x, got, clean in ((q, res[1][0], res[0][0]), (k, res[1][1], res[0][1])):
+                assert torch.equal(got[..., R:].nan_to_num(7.0), x[..., R:].nan_to_num(7.0))
+                assert torch.equal(got[..., :R], clean[..., :R])
+            assert torch.equal(res[0][2], res[1][2])
+            q, k, v = (t.contiguous() for t in _append_inputs(N, 4, 2, D, dt, 31))

@@ -464,3 +464,46 @@ def test_gradients_without_eps(B, Hq, Hkv, T, D, R, dt, eps):
         _check(o.detach(), ref[0], ref[1])
         _check(dx, ref[2], ref[3])
         _check(dw, ref[4], ref[5])
+
+
+@pytest.mark.parametrize("R", [0, 16, 32, 48])
+@pytest.mark.parametrize("dt", [torch.bfloat16, torch.float16, torch.float32])
+def test_channels_that_are_not_rotated_keep_to_themselves(dt, R):
+    """An infinity or NaN in channel R + t of token t: no other channel that is not rotated may see it."""
+    D = 64
+    T = D - R
+    cos, sin = (None, None) if R == 0 else _angles(T, R)
+    t = torch.arange(T, device=CUDA)
+    for value in (math.inf, -math.inf, math.nan):
+        q, k = randn((1, 3, T, D), 1, dt, CUDA), randn((1, 1, T, D), 2, dt, CUDA)
+        clean = sa.qk_norm_rope(q, k, cos, sin, eps=None)
+        x = [v.clone() for v in (q, k)]
+        for v in x:
+            v[:, :, t, R + t] = value
+        x = [v.requires_grad_(True) for v in x]
+        y = sa.qk_norm_rope(x[0], x[1], cos, sin, eps=None)
+        for a, b, c in zip(x, y, clean):  # without a norm they are copied
+            assert torch.equal(a[..., R:].nan_to_num(7.0), b[..., R:].nan_to_num(7.0))
+            assert torch.equal(b[..., :R], c[..., :R])
+        g = [randn(v.shape, 3, dt, CUDA) for v in y]
+        clean_g = torch.autograd.grad(y, x, g, retain_graph=True)
+        for v in g:
+            v[:, :, t, R + t] = value
+        for a, b, c in zip(g, torch.autograd.grad(y, x, g), clean_g):
+            assert torch.equal(a[..., R:].nan_to_num(7.0), b[..., R:].nan_to_num(7.0))
+            assert torch.equal(b[..., :R], c[..., :R])
+    # with a norm a row that holds an infinity is x / inf * w: NaN there, 0 elsewhere
+    x = randn((1, 2, T, D), 4, dt, CUDA)
+    x[:, :, t, R + t] = math.inf
+    w = 1 + randn((D,), 5, torch.float32, CUDA, 0.3)
+    y = sa.qk_norm_rope(x, x, cos, sin, q_weight=w)
+    for v in y:
+        at = torch.zeros(T, D, dtype=torch.bool, device=CUDA)
+        at[t, R + t] = True
+        assert v[:, :, at].isnan().all() and (v[:, :, ~at] == 0).all()
+    # an infinite weight reaches its own channel alone
+    q, w2 = randn((1, 2, T, D), 6, dt, CUDA), w.clone()
+    w2[R + 1] = math.inf
+    rest = torch.arange(D, device=CUDA) != R + 1
+    a, b = (sa.qk_norm_rope(q, q, cos, sin, q_weight=v)[0] for v in (w, w2))
+    assert torch.equal(a[..., rest], b[..., rest]) and b[..., R + 1].isinf().all()
