@@ -370,11 +370,11 @@ __global__ void __launch_bounds__(kWalkThreads, kAppendBlocks) qk_norm_rope_appe
       });
 }
 
-// Opt-in to `bytes` of dynamic shared memory (the requests' scans).
-template <typename F> static int opt_in(F* f, size_t bytes) {
-  if (bytes <= 48 * 1024) return SA_OK;
-  return sa_record_cuda_error(cudaFuncSetAttribute(f, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes));
-}
+// Dynamic shared memory of the requests' scans.  The kernels are opted in to the largest
+// batch's once: the limit is the kernel's, and set to each call's own size another thread's
+// larger launch between that and its own was refused.
+constexpr int assign_smem(int64_t B) { return (int)((3 * B + 1) * 4); }
+constexpr int release_smem(int64_t B) { return (int)std::max<int64_t>(B, 1) * 8; }
 
 template <typename E, int L, bool Partial>
 static int launch_append_lp(const AppendArgs& a, const Tables& tb, cudaStream_t st) {
@@ -447,7 +447,6 @@ extern "C" int sa_paged_assign_slots(int32_t* block_table, int64_t table_stride,
                reinterpret_cast<long long*>(slots), positions, cu_seqlens, context_lens_out, free_head_out, num_free,
                (int)B, (int)num_tokens, (int)max_blocks, (int)block_size,
                sa::qkr::FastDiv((uint32_t)block_size)};
-  const size_t smem = (3 * (size_t)B + 1) * 4;
   // one token a thread where half a wave (two blocks an SM) holds them, else four in equal rounds
   const int64_t wave = 2ll * sm_count();
   const bool few = num_tokens <= wave * kThreads / 2;
@@ -455,10 +454,11 @@ extern "C" int sa_paged_assign_slots(int32_t* block_table, int64_t table_stride,
   const int64_t tiles = std::max<int64_t>(1, (num_tokens + each - 1) / each), rounds = (tiles + wave - 1) / wave;
   const unsigned blocks = (unsigned)((tiles + rounds - 1) / rounds);
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  const int orc = few ? opt_in(paged_assign_kernel<1>, smem) : opt_in(paged_assign_kernel<4>, smem);
+  const int orc = sa_record_cuda_error(few ? opt_in_once<&paged_assign_kernel<1>, assign_smem(kMaxRequests)>()
+                                           : opt_in_once<&paged_assign_kernel<4>, assign_smem(kMaxRequests)>());
   if (orc != SA_OK) return orc;
-  if (few) paged_assign_kernel<1><<<blocks, kThreads, smem, st>>>(a);
-  else paged_assign_kernel<4><<<blocks, kThreads, smem, st>>>(a);
+  if (few) paged_assign_kernel<1><<<blocks, kThreads, assign_smem(B), st>>>(a);
+  else paged_assign_kernel<4><<<blocks, kThreads, assign_smem(B), st>>>(a);
   return sa_record_cuda_error(cudaGetLastError());
 }
 
@@ -474,11 +474,10 @@ extern "C" int sa_paged_release_pages(const int32_t* block_table, int64_t table_
   if (num_free > 0 && !free_pages) return SA_ERR_ARG;
   ReleaseArgs a{block_table, table_stride, context_lens, done, free_pages, free_head, context_lens_out, free_head_out,
                 num_free, (int)B, (int)max_blocks, (int)block_size};
-  const size_t smem = (size_t)std::max<int64_t>(B, 1) * 8;
-  const int orc = opt_in(paged_release_kernel, smem);
+  const int orc = sa_record_cuda_error(opt_in_once<&paged_release_kernel, release_smem(kMaxRequests)>());
   if (orc != SA_OK) return orc;
   const int64_t blocks = std::max<int64_t>(1, std::min<int64_t>((B + 15) / 16, sm_count()));
-  paged_release_kernel<<<(unsigned)blocks, kThreads, smem, static_cast<cudaStream_t>(stream)>>>(a);
+  paged_release_kernel<<<(unsigned)blocks, kThreads, release_smem(B), static_cast<cudaStream_t>(stream)>>>(a);
   return sa_record_cuda_error(cudaGetLastError());
 }
 

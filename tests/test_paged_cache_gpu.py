@@ -9,6 +9,7 @@ formula is used here); the decode's are derived at ``_attend``."""
 
 import gc
 import math
+import threading
 
 import pytest
 import torch
@@ -696,3 +697,37 @@ def test_append_copies_infinities_without_touching_their_neighbours():
                 assert torch.equal(got[..., :R], clean[..., :R])
             assert torch.equal(res[0][2], res[1][2])
             q, k, v = (t.contiguous() for t in _append_inputs(N, 4, 2, D, dt, 31))
+
+
+def test_large_batches_from_two_threads():
+    """Two host threads whose batches need different shared memory: no launch is refused."""
+    lib, bs, bad, start = _lib.load(), 16, [], threading.Barrier(2)
+    p = lambda t: t.data_ptr()  # noqa: E731
+
+    def work(B):
+        table = torch.arange(B, device=CUDA, dtype=I32)[:, None].contiguous()
+        own, full, ones = (torch.full((B, 1), n, device=CUDA, dtype=I32) for n in (-1, 16, 1))
+        pool, done = torch.zeros(B, device=CUDA, dtype=I32), torch.ones(B, device=CUDA, dtype=torch.bool)
+        head, zero, none = _i32([B]), _i32([0]), torch.zeros(B, device=CUDA, dtype=I32)
+        slots = torch.zeros(B, device=CUDA, dtype=torch.int64)
+        pos, cu, ctx, ctx2 = (torch.zeros(B + 4, device=CUDA, dtype=I32) for _ in range(4))
+        h1, h2 = _i32([0]), _i32([0])
+        st = torch.cuda.Stream()
+        torch.cuda.synchronize()
+        assign = (p(own), 1, p(none), p(ones), p(table), B, p(zero), p(slots), p(pos), p(cu), p(ctx), p(h1), B, B, 1, bs,
+                  st.cuda_stream)
+        release = (p(table), 1, p(full), p(done), p(pool), B, p(head), p(ctx2), p(h2), B, 1, bs, st.cuda_stream)
+        start.wait()
+        for _ in range(3000):
+            bad.extend(r for r in (lib.sa_paged_assign_slots(*assign), lib.sa_paged_release_pages(*release)) if r != 0)
+        st.synchronize()
+        if not (torch.equal(pool, table[:, 0]) and h2.item() == 0 and h1.item() == B
+                and torch.equal(slots, torch.arange(B, device=CUDA) * bs)):
+            bad.append("outputs")
+
+    threads = [threading.Thread(target=work, args=(B,)) for B in (16384, 7000)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not bad, (len(bad), bad[:3])
