@@ -343,7 +343,7 @@ __global__ void __launch_bounds__(kWalkThreads, kAppendBlocks) qk_norm_rope_appe
           ask_slot();
         }
         if (slot >= a.num_slots) {
-          if (side == 0 && ln.o1 == 0) atomicAdd(&g_bad_entries, 1u);
+          if (side == 1 && ln.o1 == 0) atomicAdd(&g_bad_entries, 1u);  // (by k's warps: there may be no query heads)
           slot = -1;
         }
         padding = slot < 0;

@@ -731,3 +731,15 @@ def test_large_batches_from_two_threads():
     for t in threads:
         t.join()
     assert not bad, (len(bad), bad[:3])
+
+
+def test_append_without_queries_reports_slots_past_the_cache():
+    _status()
+    kc, vc = (torch.zeros(2, 1, 4, 64, device=CUDA, dtype=torch.bfloat16) for _ in range(2))
+    q, k, v = _append_inputs(3, 0, 1, 64, torch.bfloat16, 2)
+    call = lambda s: sa.qk_norm_rope_paged_append(q, k, v, kc, vc, torch.tensor(s, device=CUDA))  # noqa: E731
+    assert call([8, 2, 1 << 40]).shape == (3, 0, 64)
+    assert _status() == _lib.SA_ERR_ARG
+    assert torch.equal(vc[0, 0, 2], v[1, 0]) and vc.count_nonzero() == v[1].count_nonzero()
+    call([-1, 2, -1 << 40])  # padding is no error
+    assert _status() == _lib.SA_OK
