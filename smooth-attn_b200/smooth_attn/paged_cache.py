@@ -261,8 +261,10 @@ def qk_norm_rope_paged_append(q, k, v, k_cache, v_cache, slot_mapping, cos=None,
         key, plan = _plan("append", eps, (q, k, v, k_cache, v_cache, slot_mapping, cos, sin, positions, q_weight, k_weight))
     if plan is None:
         _check_append(q, k, v, k_cache, v_cache, slot_mapping, cos, sin, positions, q_weight, k_weight, eps)
-    if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):
-        raise ValueError("the append has no backward: call it under torch.no_grad() or on detached tensors")
+    if (torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad)
+            or R._has_tangent(q, k, v, q_weight, k_weight, cos, sin)):
+        raise ValueError("the append has no backward (nor a forward derivative): call it under torch.no_grad() or on "
+                         "detached tensors")
     if traced:
         return K._ops().qk_norm_rope_paged_append(q, k, v, k_cache, v_cache, slot_mapping, cos, sin, positions,
                                                   q_weight, k_weight, eps)

@@ -14,6 +14,7 @@ import functools
 import math
 
 import torch
+from torch.autograd import forward_ad as _fwd_ad
 from torch.autograd.function import once_differentiable
 
 from . import _lib
@@ -26,6 +27,12 @@ _POS_BYTES = {torch.int32: 4, torch.int64: 8}
 def _traced(t):
     """Whether a call runs under a tracer (``K._tracing`` of its first tensor, without a generator per call)."""
     return (torch.compiler.is_compiling() or K._get_proxy_mode() is not None or isinstance(t, K._TRACED_TYPES))
+
+
+def _has_tangent(*tensors):
+    """Whether one of them carries a forward-mode derivative, which no kernel here computes."""
+    return _fwd_ad._current_level >= 0 and any(t is not None and _fwd_ad.unpack_dual(t).tangent is not None
+                                               for t in tensors)
 
 
 def _check_weight(w, name, D, like):
@@ -412,7 +419,8 @@ def qk_norm_rope(q, k, cos=None, sin=None, *, q_weight=None, k_weight=None, eps=
     table row of each token (None: 0 .. T-1).  A position outside the tables is read as 0 and
     reported by ``sa_device_status``.  q_weight / k_weight: [D], None for 1.  eps=None leaves
     the norm out.  Differentiable once in q, k and the weights; the gradients of the weights are
-    summed in fp32 in a fixed order, bitwise the same from run to run.  No gradient for cos / sin.
+    summed in fp32 in a fixed order, bitwise the same from run to run.  No gradient for cos / sin;
+    forward-mode derivatives are refused.
     To capture a training step in a CUDA graph, let no eager graph of the same leaves live on
     (``torch.cuda.make_graphed_callables`` sees to it): torch ends such a capture with an error.
     """
@@ -423,9 +431,10 @@ def qk_norm_rope(q, k, cos=None, sin=None, *, q_weight=None, k_weight=None, eps=
         plan = None
     else:
         plan = _plan_of(q, k, cos, sin, q_weight, k_weight, eps, positions)
-    if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad
-                                    or (q_weight is not None and q_weight.requires_grad)
-                                    or (k_weight is not None and k_weight.requires_grad)):
+    if (torch.is_grad_enabled() and (q.requires_grad or k.requires_grad
+                                     or (q_weight is not None and q_weight.requires_grad)
+                                     or (k_weight is not None and k_weight.requires_grad))
+            or _has_tangent(q, k, q_weight, k_weight, cos, sin)):  # (the function refuses those)
         return _QkNormRopeFn.apply(q, k, q_weight, k_weight, cos, sin, positions, eps, plan)
     if traced:
         return K._ops().qk_norm_rope(q, k, q_weight, k_weight, cos, sin, positions, eps)

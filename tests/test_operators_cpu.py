@@ -294,3 +294,21 @@ def test_c_abi_refuses_paged_arguments_before_launch():
     assert lib.sa_paged_select_workspace_size(65536, 1, 1) == U
     assert lib.sa_sparse_paged_decode_workspace_size(2, 32, 8, 512, 64, 16, 128, _lib.SA_BF16) > 2 * 8 * 512 * 8
     assert lib.sa_sparse_paged_decode_workspace_size(2, 32, 8, 512, 0, 16, 128, _lib.SA_BF16) == A
+
+
+def test_forward_mode_derivatives_are_refused(fake):
+    q, k, c, w = _t(5, 4, 64), _t(5, 2, 64), _t(6, 2, 16, 64), _t(64)
+    s = _i(5, dtype=torch.int64)
+    fw = torch.autograd.forward_ad
+    with fw.dual_level(), torch.no_grad():
+        dual = lambda t: fw.make_dual(t, torch.ones_like(t))  # noqa: E731
+        f = sa.qk_norm_rope_paged_append
+        for args, kw in (((dual(q), k, k), {}), ((q, dual(k), k), {}), ((q, k, dual(k)), {}),
+                         ((q, k, k), dict(q_weight=dual(w))), ((q, k, k), dict(k_weight=dual(w)))):
+            with pytest.raises(ValueError, match="derivative"):
+                f(*args, c, c, s, **kw)
+        assert f(q, k, k, c, c, s, q_weight=w).shape == q.shape
+        x = q[None].transpose(1, 2)
+        with pytest.raises(NotImplementedError, match="jvp"):
+            sa.qk_norm_rope(dual(x), k[None].transpose(1, 2))
+        assert sa.qk_norm_rope(x, k[None].transpose(1, 2))[0].shape == x.shape

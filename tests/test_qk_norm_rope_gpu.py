@@ -507,3 +507,18 @@ def test_channels_that_are_not_rotated_keep_to_themselves(dt, R):
     rest = torch.arange(D, device=CUDA) != R + 1
     a, b = (sa.qk_norm_rope(q, q, cos, sin, q_weight=v)[0] for v in (w, w2))
     assert torch.equal(a[..., rest], b[..., rest]) and b[..., R + 1].isinf().all()
+
+
+def test_forward_mode_derivatives_are_refused():
+    """As by sp2norm_flash_attention: never an output that has silently lost its tangent."""
+    q, k, dq, _, wq, wk, cos, sin, *_ = _make(CASES[3])
+    fw = torch.autograd.forward_ad
+    with fw.dual_level():
+        plain = sa.qk_norm_rope(q, k, cos, sin, q_weight=wq, k_weight=wk)  # nothing here has one
+        dual = lambda t: fw.make_dual(t, torch.ones_like(t))  # noqa: E731
+        for args, w in (((dual(q), k, cos, sin), wq), ((q, dual(k), cos, sin), wq), ((q, k, cos, sin), dual(wq)),
+                        ((q, k, dual(cos), sin), wq)):
+            for grad in (True, False):
+                with torch.set_grad_enabled(grad), pytest.raises(NotImplementedError, match="jvp"):
+                    sa.qk_norm_rope(*args, q_weight=w, k_weight=wk)
+    assert all(torch.equal(a, b) for a, b in zip(plain, sa.qk_norm_rope(q, k, cos, sin, q_weight=wq, k_weight=wk)))
