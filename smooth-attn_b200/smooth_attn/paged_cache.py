@@ -28,6 +28,7 @@ from . import kernels as K
 from . import qk_rope as R
 
 MAX_REQUESTS = 16384  # one block scans all requests' lengths in shared memory
+_WIDER = (torch.int64, torch.uint32, torch.uint64)
 
 
 class PagedSlots(NamedTuple):
@@ -71,6 +72,8 @@ def _int32(name, t, shape, like, exact=False):
         return t
     if exact or t.dtype.is_floating_point or t.dtype.is_complex:
         raise ValueError(f"{name} must be a contiguous int32 tensor, got {t.dtype} with strides {t.stride()}")
+    if t.dtype in _WIDER:  # what 32 bits do not hold stays as far out as it is (-1 and 2^31 - 1 are out everywhere)
+        t = t.to(torch.int64).clamp(-1, 2 ** 31 - 1)
     return t.to(torch.int32).contiguous()
 
 

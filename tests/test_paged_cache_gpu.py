@@ -743,3 +743,29 @@ def test_append_without_queries_reports_slots_past_the_cache():
     assert torch.equal(vc[0, 0, 2], v[1, 0]) and vc.count_nonzero() == v[1].count_nonzero()
     call([-1, 2, -1 << 40])  # padding is no error
     assert _status() == _lib.SA_OK
+
+
+def test_64_bit_integers_are_not_cut_to_32():
+    """Lengths and pages outside 32 bits are as far out as they say, not their last 32 bits."""
+    q, kc, vc, means, bt = _cache(2, 4, 2, 128, 6, 16, torch.bfloat16, 12)
+    far, cut = torch.tensor([2 ** 32 + 5, -2 ** 32 + 40], device=CUDA), _i32([96, 0])
+    a, b = (sa.sp2norm_sparse_paged_attention(q, kc, vc, means, bt, c, 3, return_pages=True) for c in (far, cut))
+    assert torch.equal(a[0], b[0]) and torch.equal(a[1], b[1])
+    m = [torch.zeros_like(means) for _ in range(2)]
+    for n, (ctx, start) in enumerate(((far, torch.tensor([-2 ** 33 + 48, 0], device=CUDA)), (cut, _i32([0, 0])))):
+        sa.paged_key_means(m[n], kc, bt, ctx, start_lens=start)
+    assert torch.equal(*m) and m[0].count_nonzero() > 0
+    _status()
+    wide = bt.long()
+    wide[0, 2] += 2 ** 32
+    sa.sp2norm_sparse_paged_attention(q, kc, vc, means, wide, cut, 3)
+    assert _status() == _lib.SA_ERR_ARG and _status() == _lib.SA_OK
+    # slots: a request longer than its row, more new tokens than fit, a list's head past its end
+    t = [_i32([[3, -1], [-1, -1]]) for _ in range(2)]
+    big = 2 ** 32
+    args = [(torch.tensor([big + 3, 0], device=CUDA), torch.tensor([1, big + 20], device=CUDA)),
+            (_i32([32, 0]), _i32([1, 2 ** 31 - 1]))]
+    s = [sa.paged_assign_slots(x, *y, _i32([7, 8]), _i32([0]), 50) for x, y in zip(t, args)]
+    assert all(torch.equal(x, y) for x, y in zip(*s)) and torch.equal(*t) and s[0].context_lens.tolist() == [32, 32]
+    s = sa.paged_assign_slots(t[0], _i32([3, 0]), _i32([20, 0]), _i32([7, 8]), torch.tensor([big], device=CUDA), 20)
+    assert s.free_head.item() == 2 and s.context_lens.tolist() == [16, 0]
