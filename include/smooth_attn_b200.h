@@ -466,9 +466,11 @@ SA_API int sa_paged_decode(const void* q, const void* k_cache, const void* v_cac
  * positions[num_tokens] = the token's position in its sequence; -1 and 0 for a
  * token without a place (row or list full, behind the last request);
  * cu_seqlens[B + 1], clamped to num_tokens; context_lens_out[B] counts the
- * placed tokens; free_head_out[1].  The inputs other than block_table are not
- * changed and no output may alias one.  Negative lengths count as 0.  B <= 16384.
- * One launch.  (No reference counterpart: the reference is handed a table.)
+ * placed tokens; free_head_out[1].  A page below 0, held or from the list, gives
+ * its tokens slot -1 too and is reported by sa_device_status (SA_ERR_ARG).  The
+ * inputs other than block_table are not changed and no output may alias one.
+ * Negative lengths count as 0.  B <= 16384.  One launch.  (No reference
+ * counterpart: the reference is handed a table.)
  */
 SA_API int sa_paged_assign_slots(int32_t* block_table, int64_t table_stride, const int32_t* context_lens,
                                  const int32_t* new_lens, const int32_t* free_pages, int64_t num_free,
@@ -481,8 +483,9 @@ SA_API int sa_paged_assign_slots(int32_t* block_table, int64_t table_stride, con
  * order they go to free_pages[free_head[0] - total .. free_head[0]), so they are
  * taken next; context_lens_out is context_lens with 0 for them, free_head_out
  * the list's new head.  More pages than the list has room for in front of its
- * head are left out and reported by sa_device_status (SA_ERR_ARG).  No output
- * may alias an input.  B <= 16384.  (No reference counterpart.)
+ * head are left out and reported by sa_device_status (SA_ERR_ARG), as is a page
+ * below 0 (which goes to the list).  No output may alias an input.  B <= 16384.
+ * (No reference counterpart.)
  */
 SA_API int sa_paged_release_pages(const int32_t* block_table, int64_t table_stride, const int32_t* context_lens,
                                   const uint8_t* done, int32_t* free_pages, int64_t num_free,

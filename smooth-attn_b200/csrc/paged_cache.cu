@@ -39,7 +39,7 @@ int sa_record_cuda_error(cudaError_t e);
 namespace sa {
 namespace pgc {
 
-static __device__ unsigned g_bad_entries;  // slots past the cache, positions past the tables, a pool given too much back
+static __device__ unsigned g_bad_entries;  // slots past the cache, positions past the tables, negative pages, a pool given too much back
 
 constexpr int kThreads = 512;
 constexpr int kMaxRequests = 16384;  // 12 bytes each of shared memory
@@ -175,6 +175,7 @@ __global__ void __launch_bounds__(kThreads, 2) paged_assign_kernel(AssignArgs a)
           page = __ldg(a.pool + at[b] + pi);
           if (p == pi * a.bs) *entry = page;
         }
+        if (page < 0) atomicAdd(&g_bad_entries, 1u);  // its tokens have no slot
         seen = pi;
       }
       pos[j] = p;
@@ -243,10 +244,16 @@ __global__ void __launch_bounds__(kThreads) paged_release_kernel(ReleaseArgs a) 
   for (int64_t b = (int64_t)blockIdx.x * (kThreads / 32) + (threadIdx.x >> 5); b < a.B;
        b += (int64_t)gridDim.x * (kThreads / 32)) {
     const int n = pages_of((int)b);
+    bool none = false;
     for (int j = lane; j < n; j += 32) {
       const int64_t to = first + off[b] + j;
-      if (to >= 0 && SA_DCHECK(to < a.num_free && j < a.max_blocks)) a.pool[to] = a.table[b * a.ld + j];
+      if (to >= 0 && SA_DCHECK(to < a.num_free && j < a.max_blocks)) {
+        const int32_t page = a.table[b * a.ld + j];
+        none |= page < 0;
+        a.pool[to] = page;
+      }
     }
+    if (none) atomicAdd(&g_bad_entries, 1u);  // the list is short of a page
   }
 }
 

@@ -113,8 +113,10 @@ def paged_assign_slots(block_table, context_lens, new_lens, free_pages, free_hea
 
     A token for which there is no room (its table row is full, the pool is empty, num_tokens is too
     small) gets slot -1 and is not counted in ``PagedSlots.context_lens``; so do the tokens behind the
-    last request.  Negative lengths count as 0.  free_pages: int32 [P]; free_head: int32 [1];
-    context_lens, new_lens: [B], at most 16384 requests.  One launch, no host synchronisation.
+    last request.  Negative lengths count as 0.  A page below 0, in the list or in the held part of
+    a row, gives its tokens slot -1 too and is reported by ``sa_device_status``.  free_pages: int32
+    [P]; free_head: int32 [1]; context_lens, new_lens: [B], at most 16384 requests.  One launch, no
+    host synchronisation.
     """
     num_tokens, block_size = int(num_tokens), int(block_size)
     traced = R._traced(block_table)
@@ -177,8 +179,8 @@ def paged_release_pages(block_table, context_lens, done, free_pages, free_head, 
     the next to be taken.  Returns (context_lens with 0 for those requests, the new free_head); the
     arguments themselves are not changed.  block_table keeps its entries.  Giving back more pages than
     were taken (a request released twice from stale lengths) leaves those out that have no entry and
-    is reported by ``sa_device_status``.  A page belongs to one request: pages that requests share
-    would be given back once for each.  done: bool [B].
+    is reported by ``sa_device_status``, as is a page below 0 that goes to the list.  A page belongs
+    to one request: pages that requests share would be given back once for each.  done: bool [B].
     """
     block_size = int(block_size)
     traced = R._traced(block_table)

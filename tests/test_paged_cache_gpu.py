@@ -769,3 +769,22 @@ def test_64_bit_integers_are_not_cut_to_32():
     assert all(torch.equal(x, y) for x, y in zip(*s)) and torch.equal(*t) and s[0].context_lens.tolist() == [32, 32]
     s = sa.paged_assign_slots(t[0], _i32([3, 0]), _i32([20, 0]), _i32([7, 8]), torch.tensor([big], device=CUDA), 20)
     assert s.free_head.item() == 2 and s.context_lens.tolist() == [16, 0]
+
+
+def test_pages_that_are_none_are_reported():
+    """A negative page, in a row's held part or in the list: its tokens have no slot, and it is said."""
+    _status()
+    t = _i32([[3, -1], [-5, -1]])
+    s = sa.paged_assign_slots(t, _i32([16, 3]), _i32([2, 2]), _i32([6]), _i32([0]), 4)
+    assert s.slot_mapping.tolist() == [96, 97, -1, -1]
+    assert _status() == _lib.SA_ERR_ARG
+    s = sa.paged_assign_slots(_i32([[-1]]), _i32([0]), _i32([1]), _i32([-2]), _i32([0]), 1)
+    assert s.slot_mapping.tolist() == [-1] and _status() == _lib.SA_ERR_ARG
+    free = _i32([0, 1, 2])
+    sa.paged_release_pages(_i32([[7, -1]]), _i32([20]), torch.tensor([True], device=CUDA), free, _i32([3]))
+    assert _status() == _lib.SA_ERR_ARG
+    # rows and lists whose unused entries are negative are ordinary
+    t = _i32([[3, -1], [-1, -1]])
+    sa.paged_assign_slots(t, _i32([15, 0]), _i32([1, 1]), _i32([-9, 6, -9]), _i32([1]), 5)
+    sa.paged_release_pages(t, _i32([16, 0]), torch.tensor([True, True], device=CUDA), free, _i32([3]))
+    assert _status() == _lib.SA_OK
