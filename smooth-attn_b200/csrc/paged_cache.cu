@@ -529,7 +529,7 @@ extern "C" int sa_qk_norm_rope_paged_append(const void* q, const void* k, const 
   a.cache[1] = v_cache;
   a.slots = reinterpret_cast<const long long*>(slots);
   const void* xs[3] = {q, k, v};
-  const void* ws[3] = {q_weight, k_weight, nullptr};
+  const void* ws[3] = {normalize ? q_weight : nullptr, normalize ? k_weight : nullptr, nullptr};  // else n = x
   const int C = sa::qkr::unit_heads(groups * (Hq + 2 * Hkv), (int64_t)kAppendBlocks * sa::qkr::sm_count() * (sa::qkr::kWalkThreads / 32));
   int64_t units = 0;
   for (int i = 0; i < 3; ++i) {

@@ -473,6 +473,7 @@ extern "C" int sa_qk_norm_rope(const void* q, const void* k, void* q_out, void* 
     return rc;
   if (Hkv > 0 && ((rc = check_rows(k, k_strides, es)) != SA_OK || (rc = check_rows(k_out, ko_strides, es)) != SA_OK))
     return rc;
+  if (!normalize) q_weight = k_weight = nullptr;  // n = x
   const int64_t groups = groups_of(B * T, D);
   const int per_sm = dtype == SA_F32 ? kFwdBlocks<float> : kFwdBlocks<__half>;
   const int C = unit_heads(groups * (Hq + Hkv), (int64_t)per_sm * sm_count() * (kWalkThreads / 32));
@@ -522,6 +523,7 @@ extern "C" int sa_qk_norm_rope_bwd(const void* q, const void* k, const void* dq_
   if (hk > 0 && ((rc = check_rows(k, k_strides, es)) != SA_OK || (rc = check_rows(dk_out, dko_strides, es)) != SA_OK ||
                  (rc = check_rows(dk, dk_strides, es)) != SA_OK))
     return rc;
+  if (!normalize) q_weight = k_weight = nullptr;  // n = x
   const int64_t groups = work ? groups_of(B * T, D) : 0;
   const int C = unit_heads(groups * (hq + hk), (int64_t)kBwdBlocks * sm_count() * (kWalkThreads / 32));
   const Side a = side_of(q, dq, dq_out, q_weight, hq, q_strides, dq_strides, dqo_strides, groups, C);

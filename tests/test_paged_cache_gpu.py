@@ -7,6 +7,7 @@ serving run of all of them together.
 Tolerances count roundings as in test_qk_norm_rope_gpu.py (whose 64-bit row
 formula is used here); the decode's are derived at ``_attend``."""
 
+import ctypes
 import gc
 import math
 import threading
@@ -788,3 +789,18 @@ def test_pages_that_are_none_are_reported():
     sa.paged_assign_slots(t, _i32([15, 0]), _i32([1, 1]), _i32([-9, 6, -9]), _i32([1]), 5)
     sa.paged_release_pages(t, _i32([16, 0]), torch.tensor([True, True], device=CUDA), free, _i32([3]))
     assert _status() == _lib.SA_OK
+
+
+def test_c_abi_append_without_a_norm_leaves_the_weights_out():
+    """normalize = 0 is n = x, whatever weights come with it."""
+    lib, N, Hq, Hkv, D, bs = _lib.load(), 5, 2, 1, 64, 8
+    q, k, v = (t.contiguous() for t in _append_inputs(N, Hq, Hkv, D, torch.bfloat16, 3))
+    kc, vc = (torch.zeros(1, Hkv, bs, D, device=CUDA, dtype=torch.bfloat16) for _ in range(2))
+    w, out, slots = torch.full((D,), 3.0, device=CUDA), torch.zeros_like(q), torch.arange(N, device=CUDA)
+    s = [(ctypes.c_int64 * 3)(H * D, D, 1) for H in (Hq, Hkv, Hkv)]
+    p = lambda t: t.data_ptr()  # noqa: E731
+    assert lib.sa_qk_norm_rope_paged_append(p(q), p(k), p(v), p(out), p(kc), p(vc), p(slots), p(w), p(w), _lib.SA_F32, None,
+                                            None, 0, None, 0, 0, N, Hq, Hkv, D, 0, 1, bs, *s, 1e-6, 0, _lib.SA_BF16,
+                                            None) == _lib.SA_OK
+    torch.cuda.synchronize()
+    assert torch.equal(out, q) and torch.equal(kc[0, :, :N].transpose(0, 1), k)

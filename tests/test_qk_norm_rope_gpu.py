@@ -12,6 +12,7 @@ subtraction for the rotation give 24 * 2^-24 of |n1| + |n2|.  dx and the
 weights' gradients are bounded the same way by their terms' magnitudes (see
 each check)."""
 
+import ctypes
 import gc
 import math
 
@@ -522,3 +523,25 @@ def test_forward_mode_derivatives_are_refused():
                 with torch.set_grad_enabled(grad), pytest.raises(NotImplementedError, match="jvp"):
                     sa.qk_norm_rope(*args, q_weight=w, k_weight=wk)
     assert all(torch.equal(a, b) for a, b in zip(plain, sa.qk_norm_rope(q, k, cos, sin, q_weight=wq, k_weight=wk)))
+
+
+def test_c_abi_without_a_norm_leaves_the_weights_out():
+    """normalize = 0 is n = x, in both directions, whatever weights come with it."""
+    lib, T, D = _lib.load(), 5, 64
+    x, dy = randn((1, 2, T, D), 1, torch.float32, CUDA), randn((1, 2, T, D), 2, torch.float32, CUDA)
+    w = 1 + randn((D,), 3, torch.float32, CUDA, 0.5)
+    cos, sin = _angles(T, 32)
+    s = (ctypes.c_int64 * 4)(2 * T * D, T * D, D, 1)
+    y, dx = torch.full_like(x, 9.0), torch.full_like(x, 9.0)
+    p = lambda t: t.data_ptr()  # noqa: E731
+    tables = (p(cos), p(sin), _lib.SA_F32, None, 0, 0, T)
+    for weight in (None, p(w)):
+        assert lib.sa_qk_norm_rope(p(x), None, p(y), None, weight, weight, _lib.SA_F32, *tables, 1, 2, 0, T, D, 32, s, s, s,
+                                   s, 1e-6, 0, _lib.SA_F32, None) == _lib.SA_OK
+        assert lib.sa_qk_norm_rope_bwd(p(x), None, p(dy), None, p(dx), None, weight, weight, _lib.SA_F32, None, None,
+                                       *tables, None, 0, 1, 2, 0, T, D, 32, s, s, s, s, s, s, 1e-6, 0, _lib.SA_F32,
+                                       None) == _lib.SA_OK
+        torch.cuda.synchronize()
+        ref = _ref64(x, None, cos, sin, torch.arange(T, device=CUDA)[None], None, dy)
+        _check(y, ref[0], ref[1])
+        _check(dx, ref[2], ref[3])
