@@ -804,3 +804,47 @@ def test_c_abi_append_without_a_norm_leaves_the_weights_out():
                                             None) == _lib.SA_OK
     torch.cuda.synchronize()
     assert torch.equal(out, q) and torch.equal(kc[0, :, :N].transpose(0, 1), k)
+
+
+def test_sparse_decode_repeats_bitwise():
+    """The same call on other memory, over workspaces of other contents, on another stream."""
+    ctx = [8192, 5003, 7777, 17, 0, 6001, 8191, 5120]
+    first = None
+    for run in range(6):
+        filler = torch.full((64 << 20,), (0x7F, 0xFF, 0x00)[run % 3], device=CUDA, dtype=torch.uint8)
+        del filler  # (what the next tensors and workspaces are made of)
+        q, kc, vc, means, bt = _cache(8, 32, 8, 128, 512, 16, torch.bfloat16, 77)
+        with torch.cuda.stream(torch.cuda.Stream() if run % 2 else torch.cuda.current_stream()):
+            torch.cuda.current_stream().wait_stream(torch.cuda.default_stream())
+            got = [sa.sp2norm_sparse_paged_attention(q, kc, vc, means, bt, _i32(ctx), 64, return_pages=True)
+                   for _ in range(20)]
+        torch.cuda.synchronize()
+        first = got[0] if first is None else first
+        for out, pages in got:
+            assert torch.equal(out, first[0]) and torch.equal(pages, first[1])
+
+
+def test_key_means_of_a_mixed_batch():
+    """One new prompt among sequences of one token: only its full pages, and theirs that the token fills."""
+    Hkv, D, bs, mb, B = 8, 128, 16, 512, 64
+    P = 1300
+    kc = randn((P, Hkv, bs, D), 1, torch.bfloat16, CUDA)
+    bt = torch.full((B, mb), -1, dtype=I32, device=CUDA)
+    order = torch.randperm(P, generator=torch.Generator().manual_seed(3)).to(I32).to(CUDA)
+    ctx, start, at = [], [], 0
+    for b in range(B):
+        n = 8191 if b == 17 else 5 * b + 1  # those of 16, 96, .. tokens end on a page
+        ctx.append(n)
+        start.append(0 if b == 17 else n - 1)
+        p = -(-n // bs)
+        bt[b, :p] = order[at:at + p]
+        at += p
+    assert at <= P
+    means = randn((P, Hkv, D), 2, torch.bfloat16, CUDA)
+    before = means.clone()
+    sa.paged_key_means(means, kc, bt, _i32(ctx), start_lens=_i32(start))
+    ids = torch.cat([bt[b, s // bs:c // bs] for b, (s, c) in enumerate(zip(start, ctx))]).long()
+    assert ids.numel() > 511
+    _check(means[ids], kc[ids].double().mean(2), (bs + 1) * U * kc[ids].double().abs().mean(2))
+    means[ids] = before[ids]
+    assert torch.equal(means, before)
