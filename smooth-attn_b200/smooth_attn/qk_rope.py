@@ -435,6 +435,9 @@ def qk_norm_rope(q, k, cos=None, sin=None, *, q_weight=None, k_weight=None, eps=
                                      or (q_weight is not None and q_weight.requires_grad)
                                      or (k_weight is not None and k_weight.requires_grad))
             or _has_tangent(q, k, q_weight, k_weight, cos, sin)):  # (the function refuses those)
+        if traced:  # a traced autograd function drops a gradient of one tensor passed twice: k's as views are others
+            k = k.view_as(k)
+            k_weight = None if k_weight is None else k_weight.view_as(k_weight)
         return _QkNormRopeFn.apply(q, k, q_weight, k_weight, cos, sin, positions, eps, plan)
     if traced:
         return K._ops().qk_norm_rope(q, k, q_weight, k_weight, cos, sin, positions, eps)

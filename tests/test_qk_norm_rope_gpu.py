@@ -545,3 +545,19 @@ def test_c_abi_without_a_norm_leaves_the_weights_out():
         ref = _ref64(x, None, cos, sin, torch.arange(T, device=CUDA)[None], None, dy)
         _check(y, ref[0], ref[1])
         _check(dx, ref[2], ref[3])
+
+
+@pytest.mark.parametrize("dynamic", [False, True])
+def test_one_tensor_for_queries_and_keys(dynamic):
+    """The same tensor as q and k, and one weight for both: the gradients of both uses add up, compiled too."""
+    x, _, dq, dk, w, *_ = _make((2, 3, 3, 17, 64, 64, torch.float32, torch.float32, True, "none"))
+    cos, sin = _angles(17, 64)
+    full = torch.arange(17, device=CUDA).expand(2, 17)
+    ref = [_ref64(x, w, cos, sin, full, 1e-6, dy) for dy in (dq, dk)]
+    f = lambda q, k, a, b: sa.qk_norm_rope(q, k, cos, sin, q_weight=a, k_weight=b)  # noqa: E731
+    for call in (f, torch.compile(f, fullgraph=True, backend="aot_eager", dynamic=dynamic)):
+        ins = [t.clone().requires_grad_(True) for t in (x, w)]
+        gx, gw = torch.autograd.grad(call(ins[0], ins[0], ins[1], ins[1]), ins, (dq, dk))
+        # the two are added once more
+        _check(gx, ref[0][2] + ref[1][2], ref[0][3] + ref[1][3] + 4 * U * (ref[0][2].abs() + ref[1][2].abs()))
+        _check(gw, ref[0][4] + ref[1][4], ref[0][5] + ref[1][5] + 4 * U * (ref[0][4].abs() + ref[1][4].abs()))
