@@ -672,6 +672,8 @@ def sp2norm_flash_attention(q, k, v, *, scale=None, window_size=0, exact_math=Fa
     _flash_check(q, k, v)
     if scale is None:
         scale = 1.0 / math.sqrt(D)
+    if torch.compiler.is_compiling():  # (a traced autograd function drops a gradient of one tensor passed twice)
+        k, v = k.view_as(k), v.view_as(v)
     return _SP2NormFlashAttentionFn.apply(q, k, v, scale, H_q // H_kv, window_size, not exact_math, deterministic)
 
 

@@ -45,6 +45,23 @@ def test_compiled_flash_fwd_bwd_matches_eager(backend):
         torch.testing.assert_close(a, b, rtol=0, atol=0)
 
 
+def test_compiled_flash_of_one_tensor_keeps_all_its_gradients():
+    """q, k and v (or two of them) the same tensor: the gradients of every use add up, as in the eager call."""
+    x, y = randn((1, 4, 200, 64), 1, torch.bfloat16, CUDA), randn((1, 4, 200, 64), 2, torch.bfloat16, CUDA)
+    f = lambda q, k, v: sa.sp2norm_flash_attention(q, k, v, deterministic=True)  # noqa: E731
+    for pick in ((0, 0, 0), (0, 1, 1), (0, 0, 1), (0, 1, 0)):
+        torch._dynamo.reset()
+        g = lambda *t: f(*(t[i] for i in pick))  # noqa: E731
+        o_e, parts = _grads(f, *((x, y)[i] for i in pick))  # three tensors: the parts by themselves
+        o_c, got = _grads(torch.compile(g, fullgraph=True, backend="aot_eager"), *(x, y)[:max(pick) + 1])
+        assert torch.equal(o_e, o_c)
+        for n, c in enumerate(got):
+            mine = [p.float() for p, i in zip(parts, pick) if i == n]
+            # bf16 parts added in bf16: each of at most two sums is off by half a step of at most the parts' sizes
+            tol = 2 * 2.0 ** -8 * sum(p.abs() for p in mine)
+            assert ((c.float() - sum(mine)).abs() <= tol).all()
+
+
 @pytest.mark.parametrize("backend", ["aot_eager", "inductor"])
 def test_compiled_norm_fwd_bwd_matches_eager(backend):
     x = randn((2, 4, 256, 256), 4, torch.bfloat16, CUDA)
