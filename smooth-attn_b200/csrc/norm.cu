@@ -652,9 +652,14 @@ static BulkShape bulk_shape(int slot_bytes) {
   return b;
 }
 
+// The opt-in is a limit of the kernel, not of a launch: always the largest that a slot of
+// two fp32 rows of 4096 (backward) asks for.  Set to each call's own size, another thread's
+// call could lower it before this one's launch, which was then refused.
+constexpr int kBulkMaxSmem = kBulkWarps * (kMaxStages * 8 + 2 * 4096 * 4);
+
 template <typename K>
 static unsigned bulk_grid(K kernel, size_t smem, int64_t rows) {
-  cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+  cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kBulkMaxSmem);
   int occ = 0;
   cudaOccupancyMaxActiveBlocksPerMultiprocessor(&occ, kernel, kBulkWarps * 32, smem);
   if (occ < 1) occ = 1;

@@ -3,6 +3,7 @@ numpy oracle and the committed golden vectors.  Mirrors the reference's
 ``tests/test_training_api.py:19-78`` plus odd sizes, all dtypes, all powers,
 strided outputs and full-size (BASELINE config) property checks."""
 
+import threading
 from pathlib import Path
 
 import numpy as np
@@ -10,6 +11,7 @@ import pytest
 import torch
 
 import smooth_attn as sa
+from smooth_attn import _lib
 from oracle import sa_oracle as O
 from tests._util import TOL, assert_close, np32, randn
 
@@ -238,3 +240,33 @@ def test_zz_no_device_timeouts_recorded():
     from smooth_attn import _lib
 
     assert _lib.load().sa_device_status(1) == _lib.SA_OK
+
+
+def test_two_threads_with_rows_of_different_lengths():
+    """Two host threads on one kernel whose rows need different shared memory: no launch is refused."""
+    lib, bad, start = _lib.load(), [], threading.Barrier(2)
+
+    def work(cols):
+        x = randn((64, cols), cols, device="cuda")
+        row = torch.empty(64, device="cuda")
+        out = torch.empty_like(x)
+        st = torch.cuda.Stream()
+        torch.cuda.synchronize()
+        fwd = (x.data_ptr(), out.data_ptr(), row.data_ptr(), 64, cols, cols, cols, _lib.SA_F32, 0, 1.0, 0.5, 2, st.cuda_stream)
+        start.wait()
+        for _ in range(4000):
+            bad.extend(r for r in (lib.sa_norm_fwd(*fwd),) if r != 0)
+        st.synchronize()
+        y = torch.empty_like(x)
+        if lib.sa_norm_fwd(x.data_ptr(), y.data_ptr(), *fwd[2:]) != 0:
+            bad.append("alone")
+        st.synchronize()
+        if not torch.equal(y, out):
+            bad.append("outputs")
+
+    threads = [threading.Thread(target=work, args=(cols,)) for cols in (4096, 2052)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not bad, (len(bad), bad[:3])
