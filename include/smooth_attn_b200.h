@@ -421,9 +421,9 @@ SA_API int sa_fp8_flash_fwd(const void* q8, const void* k8, const void* vq, void
                             const int64_t* o_strides, float scale, int64_t window_size, void* stream);
 
 /*
- * Workspace bytes sa_paged_decode needs for this shape (0 when the launch
- * does not split sequences over several CTAs), or a negative sa_status when
- * the shape is rejected.  Depends on the current device's SM count.
+ * Workspace bytes sa_paged_decode needs for this shape, or a negative
+ * sa_status when the shape is rejected.  Depends on the current device's SM
+ * count.
  */
 SA_API int64_t sa_paged_decode_workspace_size(int64_t B, int64_t Hq, int64_t Hkv, int64_t max_blocks,
                                               int64_t block_size, int64_t D, int dtype);
@@ -439,10 +439,10 @@ SA_API int64_t sa_paged_decode_workspace_size(int64_t B, int64_t Hq, int64_t Hkv
  * block_size]).  out: bf16 [B, Hq, D] contiguous.  dtype (q and caches):
  * SA_BF16 or SA_F16; D in {32, 64, 128, 256}; Hq % Hkv == 0.  Pointers
  * 16-byte aligned.  workspace: sa_paged_decode_workspace_size() bytes,
- * 256-byte aligned; its first bytes hold per-(sequence, head) arrival
- * tickets that must be zero before the first call and that every completed
- * call leaves zero again, so one zero-filled workspace can be reused by
- * calls that do not overlap on the GPU.  Page indices outside
+ * 256-byte aligned; its first 64 KB hold arrival tickets that must be zero
+ * before the first call and that every completed call leaves zero again, so
+ * one zero-filled workspace can be reused by calls of any shapes that do not
+ * overlap on the GPU.  Page indices outside
  * [0, num_blocks) are read as page 0 and reported by sa_device_status.
  *
  * Replaces: sp2norm_paged_attention / _sp2norm_paged_attention_kernel

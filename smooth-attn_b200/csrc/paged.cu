@@ -37,7 +37,8 @@
 // result is deterministic).  The CTAs that touch a unit are a contiguous
 // range known by arithmetic; the last of them to arrive (atomic ticket, no
 // waiting) adds the partials, divides and writes the output, then resets the
-// ticket to zero for the next call.
+// ticket to zero for the next call, which may be of another shape: the tickets
+// have a part of the workspace to themselves (paged_tc.h).
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
@@ -605,7 +606,7 @@ int make_plan(int64_t B, int64_t Hq, int64_t Hkv, int64_t max_blocks, int64_t bs
   p->grid = std::max<int64_t>(1, std::min<int64_t>(wave, (p->W + 4 * kPgWarps - 1) / (4 * kPgWarps)));
   const int64_t share = std::max<int64_t>(1, p->W / p->grid);  // fewest chunks a non-empty CTA holds
   p->slots = (int)std::min<int64_t>(p->grid, (p->M + share - 1) / share + 2);
-  p->ticket_bytes = (p->units * 4 + 255) / 256 * 256;
+  p->ticket_bytes = ticket_bytes_of(p->units);
   p->part_bytes = p->units * p->slots * (int64_t)paged_rec_floats(GT, (int)D) * 4;
   return SA_OK;
 }
@@ -667,6 +668,11 @@ extern "C" int sa_paged_decode(const void* q, const void* k_cache, const void* v
   if (!sa::al16(q) || !sa::al16(k_cache) || !sa::al16(v_cache) || !sa::al16(out)) return SA_ERR_ALIGN;
   if (!workspace || workspace_bytes < p.ticket_bytes + p.part_bytes) return SA_ERR_ARG;
   if ((reinterpret_cast<uintptr_t>(workspace) & 255u) != 0) return SA_ERR_ALIGN;
+  if (p.ticket_bytes > sa::kTicketReserve) {  // (another shape's records may lie there)
+    const int mrc = sa_record_cuda_error(
+        cudaMemsetAsync(workspace, 0, (size_t)p.ticket_bytes, static_cast<cudaStream_t>(stream)));
+    if (mrc != SA_OK) return mrc;
+  }
   if (p.tc)
     return sa::paged_tc_launch(q, k_cache, v_cache, out, block_table, context_lens, workspace, B, Hq, Hkv,
                                num_blocks, block_size, max_blocks, scale, p.ptc, static_cast<cudaStream_t>(stream));

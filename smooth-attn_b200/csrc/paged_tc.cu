@@ -577,7 +577,7 @@ bool paged_tc_plan(int64_t B, int64_t Hq, int64_t Hkv, int64_t max_blocks, int64
   p->grid = std::max<int64_t>(1, std::min<int64_t>(sms, W));
   const int64_t share = std::max<int64_t>(1, W / p->grid);  // fewest tiles a non-empty CTA holds
   p->slots = (int)std::min<int64_t>(p->grid, (M + share - 1) / share + 2);
-  p->ticket_bytes = (units * 4 + 255) / 256 * 256;
+  p->ticket_bytes = ticket_bytes_of(units);
   p->part_bytes = units * (int64_t)p->slots * (gt * ptc::D + ptc::NH) * 4;
   return true;
 }

@@ -4,13 +4,21 @@
 #include <cuda_runtime.h>
 #include <stdint.h>
 
+#include <algorithm>
+
 namespace sa {
+
+// The tickets come first in a workspace that calls of other shapes have used before, and
+// must be found zero.  So much of it is theirs whatever the shape, and no partial record
+// lies there; a call of more units than that holds (16384) clears its tickets itself.
+constexpr int64_t kTicketReserve = 65536;
+inline int64_t ticket_bytes_of(int64_t units) { return std::max(kTicketReserve, (units * 4 + 255) / 256 * 256); }
 
 struct PtcPlan {
   int GT;                // query heads per unit (the MMA's N columns in use)
   int64_t grid;          // CTAs (one per SM at most)
   int slots;             // partial-record slots per unit
-  int64_t ticket_bytes;  // tickets [units], padded to 256 bytes
+  int64_t ticket_bytes;  // tickets [units]: ticket_bytes_of(units)
   int64_t part_bytes;    // partial records [units][slots][GT*128 + 16] fp32
 };
 

@@ -228,3 +228,39 @@ def test_paged_rejects_bad_arguments():
                                      cl.data_ptr(), None, 0, 1, 4, 3, kc.shape[0], 16, bt.shape[1], 64,
                                      0.125, _lib.SA_BF16, None)
     assert st == _lib.SA_ERR_ARG
+
+
+@pytest.mark.parametrize("kernel", ["tc", "simt"])
+def test_calls_of_other_shapes_do_not_leave_marks_in_the_workspace(kernel, monkeypatch):
+    """A few long sequences, whose partial records fill the workspace, then many short ones, whose
+    tickets are many: the same as on a workspace of their own, and the other way round."""
+    monkeypatch.setenv("SA_PAGED_DECODE_KERNEL", kernel)
+    shapes = [(10, 16, 8, 256), (1, 8, 1, 65536), (1, 8, 2, 65536), (40, 16, 8, 48), (2, 4, 2, 32768), (100, 16, 8, 160),
+              (1, 2, 1, 160)]
+    cases = [_case(B, Hq, Hkv, T, 128, 16, seed=10 * i) for i, (B, Hq, Hkv, T) in enumerate(shapes)]
+    want = []
+    for c in cases:
+        sa.kernels._paged_ws.clear()
+        want.append(sa.sp2norm_paged_attention(*c))
+    for order in (range(len(cases)), [1, 0, 2, 3, 4, 5, 1, 0], reversed(range(len(cases)))):
+        sa.kernels._paged_ws.clear()
+        for i in order:
+            torch.full_like(want[i], float("nan"))  # (the memory that the output is likely to get)
+            assert torch.equal(sa.sp2norm_paged_attention(*cases[i]), want[i]), shapes[i]
+
+
+@pytest.mark.parametrize("kernel", ["tc", "simt"])
+def test_more_units_than_the_workspace_reserves_tickets_for(kernel, monkeypatch):
+    monkeypatch.setenv("SA_PAGED_DECODE_KERNEL", kernel)
+    B, T = 16500, 160
+    q, kc, vc, bt, cl = _case(64, 2, 1, T, 128, 16, seed=3)
+    few = sa.sp2norm_paged_attention(q, kc, vc, bt, cl)
+    pick = torch.arange(B, device=CUDA) % 64
+    many = (q[pick], kc, vc, bt[pick], cl[pick])
+    long = _case(1, 8, 1, 65536, 128, 16, seed=4)
+    for _ in range(2):
+        got = sa.sp2norm_paged_attention(*many)
+        # (64 sequences are cut at other places than 16500: other sums of the same terms, then one rounding)
+        torch.testing.assert_close(got.float(), few[pick].float(), rtol=2.0 ** -7, atol=1e-5)
+        assert torch.equal(got, sa.sp2norm_paged_attention(*many))
+        sa.sp2norm_paged_attention(*long)
