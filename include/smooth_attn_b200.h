@@ -52,6 +52,12 @@ SA_API const char* sa_status_string(int status);
 SA_API const char* sa_last_cuda_error(void);
 
 /*
+ * The id of the CUDA graph capture that `stream` takes part in, 0 if none: two
+ * calls with the same id become parts of one graph.  (No reference counterpart.)
+ */
+SA_API int64_t sa_stream_capture_id(void* stream);
+
+/*
  * Device-side status of the current device: SA_ERR_TIMEOUT if any kernel of
  * this library gave up a bounded wait (an mbarrier / copy that never
  * completed) since the last reset, else SA_OK.  Synchronises the device.

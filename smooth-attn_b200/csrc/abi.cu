@@ -198,6 +198,16 @@ extern "C" int sa_debug_checks(void) {
 
 extern "C" const char* sa_last_cuda_error(void) { return g_last_err; }
 
+extern "C" int64_t sa_stream_capture_id(void* stream) {
+  cudaStreamCaptureStatus status = cudaStreamCaptureStatusNone;
+  unsigned long long id = 0;
+  if (cudaStreamGetCaptureInfo(static_cast<cudaStream_t>(stream), &status, &id) != cudaSuccess) {
+    cudaGetLastError();
+    return 0;
+  }
+  return status == cudaStreamCaptureStatusActive ? (int64_t)id : 0;
+}
+
 extern "C" const char* sa_status_string(int status) {
   switch (status) {
     case SA_OK: return "ok";

@@ -46,6 +46,7 @@ SIGNATURES = {
     "sa_debug_checks": (_int, []),
     "sa_copy_causal_bands": (_int, [_p, _p, _i64, _i64, _i64, _i64, _int, _i64p, _p]),
     "sa_host_zero_causal_tail": (_int, [_p, _i64, _i64, _i64, _i64, _int]),
+    "sa_stream_capture_id": (_i64, [_p]),
     "sa_norm_fwd": (_int, [_p, _p, _p, _i64, _i64, _i64, _i64, _int, _int, _f, _f, _int, _p]),
     "sa_norm_bwd": (_int, [_p, _p, _p, _p, _i64, _i64, _i64, _i64, _i64, _int, _int, _int, _f, _f, _int, _p]),
     "sa_flash_fwd": (_int, [_p, _p, _p, _p, _p, _p, _i64, _i64, _i64, _i64, _i64,

@@ -974,7 +974,9 @@ def _fp8_flash_fwd_direct(q, k, v, scale, window_size):
 # ---------------------------------------------------------------------------
 
 PAGED_HEAD_DIMS = (32, 64, 128, 256)
+_PAGED_TICKET_BYTES = 1 << 16  # of a workspace: tickets, to be zero before its first call
 _paged_ws = {}  # (device index, stream handle) -> zero-ticketed workspace
+_paged_capture_ws = {}  # the same -> (the stream's last capture, its workspace)
 _paged_ws_lock = threading.Lock()
 
 
@@ -994,12 +996,26 @@ def _paged_ws_size_cached(B, H_q, H_kv, max_blocks, block_size, D, dtype_code, d
 def _paged_workspace(device, stream_handle, nbytes):
     """A workspace whose ticket words are zero (every completed call leaves
     them zero), reused per (device, stream) so calls on one stream never
-    overlap on the GPU."""
+    overlap on the GPU.
+
+    The calls of one capture on one stream share one that is cleared by the
+    graph: its replays may run on any stream, beside those of other graphs, and
+    its memory is the graph's own (held here so that nothing else of the same
+    capture gets it).  The clearing costs a replay 2 us once, not once a call."""
     key = (device.index, stream_handle)
+    if stream_handle and torch._C._cuda_isCurrentStreamCapturing():  # (the default stream never is)
+        capture = _lib.load().sa_stream_capture_id(stream_handle)
+        with _paged_ws_lock:
+            held, ws = _paged_capture_ws.get(key, (0, None))
+            if held != capture or ws.numel() < nbytes:
+                ws = torch.empty(max(nbytes, _PAGED_TICKET_BYTES), dtype=torch.uint8, device=device)
+                ws[:_PAGED_TICKET_BYTES].zero_()
+                _paged_capture_ws[key] = (capture, ws)
+            return ws
     with _paged_ws_lock:
         ws = _paged_ws.get(key)
         if ws is None or ws.numel() < nbytes:
-            ws = torch.zeros(max(nbytes, 1 << 16), dtype=torch.uint8, device=device)
+            ws = torch.zeros(max(nbytes, _PAGED_TICKET_BYTES), dtype=torch.uint8, device=device)
             _paged_ws[key] = ws
         return ws
 

@@ -116,3 +116,44 @@ def test_forward_only_paths_replay():
         g.replay()
         torch.cuda.synchronize()
         assert torch.equal(out, f())
+
+
+def _decode_case(B, Hq, Hkv, T, seed):
+    nb = B * (T // 16)
+    q = randn((B, Hq, 1, 128), seed, torch.bfloat16, CUDA)
+    kc, vc = (randn((nb, Hkv, 16, 128), seed + i, torch.bfloat16, CUDA) for i in (1, 2))
+    bt = torch.arange(nb, device=CUDA, dtype=torch.int32).view(B, -1)
+    return q, kc, vc, bt, torch.full((B,), T, device=CUDA, dtype=torch.int32)
+
+
+def test_paged_decode_graphs_keep_to_themselves():
+    """Two graphs of many decodes, one of a growing workspace: each alone, then both at once on two
+    streams with eager calls beside them; neither needs the other's workspace, tickets included."""
+    small, large = _decode_case(2, 8, 2, 4096, 1), _decode_case(1, 8, 1, 65536, 9)
+    other = _decode_case(3, 8, 2, 4096, 5)
+    calls = [[small] * 20 + [large] * 2 + [small] * 20, [other] * 40]
+    sa.kernels._paged_ws.clear()
+    graphs = [_capture(lambda cs=cs: [sa.sp2norm_paged_attention(*c) for c in cs]) for cs in calls]
+    want = [[sa.sp2norm_paged_attention(*c) for c in cs] for cs in calls]
+    streams = [torch.cuda.Stream() for _ in range(3)]
+
+    def replay(which):
+        for n in which:
+            for out in graphs[n][1]:
+                out.fill_(float("nan"))
+        torch.cuda.synchronize()
+        for _ in range(3):
+            for n in which:
+                with torch.cuda.stream(streams[n]):
+                    graphs[n][0].replay()
+        with torch.cuda.stream(streams[2]):
+            eager = [sa.sp2norm_paged_attention(*large) for _ in range(10)]
+        torch.cuda.synchronize()
+        assert all(torch.equal(o, want[0][20]) for o in eager)
+        for n in which:
+            assert all(torch.equal(a, b) for a, b in zip(graphs[n][1], want[n]))
+
+    replay([1])
+    replay([0])
+    for _ in range(5):
+        replay([0, 1])
