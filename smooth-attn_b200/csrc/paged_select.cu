@@ -4,10 +4,13 @@
 // reference's decode, src/smooth_attn/kernels.py:2681-2829, reads every page.)
 //
 // Score.  The normaliser of squareplus attention is a plain sum, so a page's
-// share of it is the sum of its tokens' weights; the score estimates that at
-// the page's mean key, summed over the group's query heads:
+// share of one head's is the sum of its tokens' weights; the score estimates that
+// at the page's mean key and adds it up over the group's query heads:
 //   score(page) = sum_g y(2 scale q_g . mean_key(page) - 1),
 //   y(a) = squareplus(a)^2
+// The heads' weights are added as they are, not divided by each head's normaliser
+// (which would take every page's score of every head first), so a head with
+// large queries has more say in what the group reads.
 // A sequence of n pages keeps its last page (the newest tokens; it may be part
 // filled and needs no mean) and the num_pages - 1 others of the highest score,
 // ties to the lowest page; NaN counts as the highest.  The

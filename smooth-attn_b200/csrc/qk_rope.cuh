@@ -35,7 +35,6 @@ template <typename E> struct Raw8 {
 #pragma unroll
     for (int i = 0; i < (int)sizeof(E) / 2; ++i) u[i] = make_uint4(0, 0, 0, 0);
   }
-  __device__ __forceinline__ void get(float (&f)[8]) const { unpack<E, 8>(u, f); }
   __device__ __forceinline__ void get(float2 (&f)[4]) const {
     float g[8];
     unpack<E, 8>(u, g);
@@ -59,10 +58,6 @@ template <typename E> struct Raw8 {
       for (int i = 0; i < 4; ++i) h[i] = __float22half2_rn(f[i]);
       u[0] = *reinterpret_cast<const uint4*>(h);
     }
-  }
-  __device__ __forceinline__ void set(const float (&f)[8]) {
-    const float2 g[4] = {{f[0], f[1]}, {f[2], f[3]}, {f[4], f[5]}, {f[6], f[7]}};
-    set(g);
   }
   __device__ __forceinline__ void store(E* p) const {
 #pragma unroll
@@ -191,7 +186,7 @@ __device__ __forceinline__ float2 pair_only(const Lane& l, float2 v, float none)
 // y of one row from its two raw chunks (zeros in lanes without one).  Partial:
 // some channels are not rotated, and there the other one of the pair is left out:
 // times a sine of 0 an infinity in it would arrive as NaN.  (The selects cost rows of
-// 80 channels of which 16 are rotated 3 % in both directions, a branch 5 to 8 %; rows
+// 80 channels of which 16 are rotated 3 to 4 %, a branch 5 to 8 %; rows
 // that are rotated throughout need none, hence the parameter: with a branch for all the
 // backward of [4, 32 + 8, 4096, 128] took 90 us for 87.5.)
 template <typename E, int L, bool Partial>

@@ -472,8 +472,9 @@ def sp2norm_paged_select(q, key_means, block_table, context_lens, num_pages, *, 
 
         score(page) = sum over the group's query heads of squareplus(2 scale q . key_mean - 1)^2
 
-    (the weight the attention would give the page's mean token, in 64 bits; ties go to the lowest
-    page, NaN counts as the highest).  pages: int32 [B, H_kv, min(num_pages, max_blocks)], indices
+    (the weight the attention would give the page's mean token, before it is normalised: of a group's
+    heads one with large queries has more say; in 64 bits; ties go to the lowest page, NaN counts as
+    the highest).  pages: int32 [B, H_kv, min(num_pages, max_blocks)], indices
     into the sequence's row of block_table, ascending, then -1; lens: int32 [B, H_kv], the tokens in
     them.  Lengths outside [0, max_blocks * block_size] are clamped; block_table entries outside the
     cache are read as page 0 and reported by ``sa_device_status``.  At most 65535 sequences times key
