@@ -499,6 +499,13 @@ SA_API int sa_paged_release_pages(const int32_t* block_table, int64_t table_stri
                                   int64_t B, int64_t max_blocks, int64_t block_size, void* stream);
 
 /*
+ * dst[i] = src[i] clamped to [-1, 2^31 - 1], i < n: lengths and pages for the
+ * paged calls, which a conversion would cut to their last 32 bits.  (No
+ * reference counterpart.)
+ */
+SA_API int sa_narrow_i64(const int64_t* src, int32_t* dst, int64_t n, void* stream);
+
+/*
  * sa_qk_norm_rope of N flat tokens whose keys and values go into a paged
  * cache.  q [N, Hq, D], k and v [N, Hkv, D] with strides {token, head, dim} in
  * elements (dim stride 1, the others multiples of 8); q_out: contiguous

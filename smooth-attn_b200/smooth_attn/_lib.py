@@ -90,6 +90,7 @@ SIGNATURES = {
     "sa_qk_norm_rope_paged_append": (_int, [_p, _p, _p, _p, _p, _p, _p, _p, _p, _int, _p, _p, _int, _p, _int, _i64,
                                             _i64, _i64, _i64, _i64, _i64, _i64, _i64, _i64p, _i64p, _i64p, _f, _int,
                                             _int, _p]),
+    "sa_narrow_i64": (_int, [_p, _p, _i64, _p]),
     "sa_paged_key_means": (_int, [_p, _p, _p, _p, _p, _i64, _i64, _i64, _i64, _i64, _i64, _int, _p]),
     "sa_paged_select_workspace_size": (_i64, [_i64, _i64, _i64]),
     "sa_paged_select": (_int, [_p, _p, _p, _p, _p, _p, _p, _i64,

@@ -73,7 +73,13 @@ def _int32(name, t, shape, like, exact=False):
     if exact or t.dtype.is_floating_point or t.dtype.is_complex:
         raise ValueError(f"{name} must be a contiguous int32 tensor, got {t.dtype} with strides {t.stride()}")
     if t.dtype in _WIDER:  # what 32 bits do not hold stays as far out as it is (-1 and 2^31 - 1 are out everywhere)
-        t = t.to(torch.int64).clamp(-1, 2 ** 31 - 1)
+        t = t.to(torch.int64).contiguous()
+        if not t.is_cuda or R._traced(t):
+            return t.clamp(-1, 2 ** 31 - 1).to(torch.int32)
+        out = torch.empty(shape, dtype=torch.int32, device=t.device)
+        with K._on(t.device):
+            _lib.check(_lib.load().sa_narrow_i64(t.data_ptr(), out.data_ptr(), t.numel(), K._stream(t)), "sa_narrow_i64")
+        return out
     return t.to(torch.int32).contiguous()
 
 

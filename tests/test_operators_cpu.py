@@ -312,3 +312,10 @@ def test_forward_mode_derivatives_are_refused(fake):
         with pytest.raises(NotImplementedError, match="jvp"):
             sa.qk_norm_rope(dual(x), k[None].transpose(1, 2))
         assert sa.qk_norm_rope(x, k[None].transpose(1, 2))[0].shape == x.shape
+
+
+def test_c_abi_refuses_narrowing_arguments_before_launch():
+    lib = _lib.load()
+    for args in ((16, 16, -1), (None, 16, 1), (16, None, 1)):
+        assert lib.sa_narrow_i64(*args, None) == _lib.SA_ERR_ARG
+    assert lib.sa_narrow_i64(None, None, 0, None) == _lib.SA_OK

@@ -848,3 +848,15 @@ def test_key_means_of_a_mixed_batch():
     _check(means[ids], kc[ids].double().mean(2), (bs + 1) * U * kc[ids].double().abs().mean(2))
     means[ids] = before[ids]
     assert torch.equal(means, before)
+
+
+def test_narrowing_of_64_bit_integers():
+    from smooth_attn import paged_cache as P
+
+    edge = [0, 1, -1, -2, 2 ** 31 - 1, 2 ** 31, -2 ** 31, 2 ** 32, 2 ** 32 + 7, -2 ** 32 + 7, 2 ** 63 - 1, -2 ** 63, 12345]
+    for n in (0, 1, len(edge), 300_001):
+        wide = torch.tensor((edge * (n // len(edge) + 1))[:n], dtype=torch.int64, device=CUDA)
+        for t in (wide, torch.stack((wide, wide), 1)[:, 1]):  # contiguous, and not
+            got = P._int32("t", t, (n,), t)
+            assert got.dtype == I32 and torch.equal(got.long(), wide.clamp(-1, 2 ** 31 - 1))
+    assert torch.equal(P._int32("t", wide[:6].view(2, 3), (2, 3), wide), wide[:6].view(2, 3).clamp(-1, 2 ** 31 - 1).to(I32))
