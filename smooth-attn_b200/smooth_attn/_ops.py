@@ -192,7 +192,8 @@ def _(q, k, v, scale, window_size):
 @torch.library.custom_op(f"{NS}::paged_decode", mutates_args=(), device_types="cuda")
 def paged_decode(q: Tensor, k_cache: Tensor, v_cache: Tensor, block_table: Tensor, context_lens: Tensor,
                  scale: float, block_size: int) -> Tensor:
-    return K._paged_decode_direct(q, k_cache, v_cache, block_table, context_lens, scale, block_size)
+    # (the graphs of mode="reduce-overhead" allow no allocation that outlives the call: no kept workspace)
+    return K._paged_decode_direct(q, k_cache, v_cache, block_table, context_lens, scale, block_size, False)
 
 
 @paged_decode.register_fake

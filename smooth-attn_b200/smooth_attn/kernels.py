@@ -993,6 +993,12 @@ def _paged_ws_size_cached(B, H_q, H_kv, max_blocks, block_size, D, dtype_code, d
     return int(_lib.load().sa_paged_decode_workspace_size(B, H_q, H_kv, max_blocks, block_size, D, dtype_code))
 
 
+def _cleared_workspace(device, nbytes):
+    ws = torch.empty(max(nbytes, _PAGED_TICKET_BYTES), dtype=torch.uint8, device=device)
+    ws[:_PAGED_TICKET_BYTES].zero_()
+    return ws
+
+
 def _paged_workspace(device, stream_handle, nbytes):
     """A workspace whose ticket words are zero (every completed call leaves
     them zero), reused per (device, stream) so calls on one stream never
@@ -1008,8 +1014,7 @@ def _paged_workspace(device, stream_handle, nbytes):
         with _paged_ws_lock:
             held, ws = _paged_capture_ws.get(key, (0, None))
             if held != capture or ws.numel() < nbytes:
-                ws = torch.empty(max(nbytes, _PAGED_TICKET_BYTES), dtype=torch.uint8, device=device)
-                ws[:_PAGED_TICKET_BYTES].zero_()
+                ws = _cleared_workspace(device, nbytes)
                 _paged_capture_ws[key] = (capture, ws)
             return ws
     with _paged_ws_lock:
@@ -1053,7 +1058,7 @@ def sp2norm_paged_attention(q, k_cache, v_cache, block_table, context_lens, *, s
     return _paged_decode_direct(q, k_cache, v_cache, block_table, context_lens, scale, block_size)
 
 
-def _paged_decode_direct(q, k_cache, v_cache, block_table, context_lens, scale, block_size):
+def _paged_decode_direct(q, k_cache, v_cache, block_table, context_lens, scale, block_size, keep_workspace=True):
     B, H_q, _, D = q.shape
     H_kv = k_cache.shape[1]
     max_blocks_per_seq = block_table.shape[1]
@@ -1082,11 +1087,14 @@ def _paged_decode_direct(q, k_cache, v_cache, block_table, context_lens, scale, 
         if nbytes < 0:
             _lib.check(int(nbytes), "sa_paged_decode_workspace_size")
         stream = _stream(q)
-        ws = _paged_workspace(q.device, stream.value, nbytes) if nbytes > 0 else None
+        if keep_workspace:
+            ws = _paged_workspace(q.device, stream.value, nbytes)
+        else:
+            ws = _cleared_workspace(q.device, nbytes)
         st = lib.sa_paged_decode(
             q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), out.data_ptr(),
             block_table.data_ptr(), context_lens.data_ptr(),
-            ws.data_ptr() if ws is not None else None, ws.numel() if ws is not None else 0,
+            ws.data_ptr(), ws.numel(),
             B, H_q, H_kv, k_cache.shape[0], block_size, max_blocks_per_seq, D, float(scale),
             _DTYPE_CODE[q.dtype], stream,
         )

@@ -123,3 +123,24 @@ def test_opcheck_all_ops():
     ]
     for op, args in cases:
         torch.library.opcheck(op, args)
+
+
+def test_decodes_in_the_graphs_of_reduce_overhead():
+    """mode="reduce-overhead" captures the ops into graphs of its own, in whose memory nothing may stay behind."""
+    B, Hq, Hkv, D, mb = 2, 8, 2, 128, 256
+    q = randn((B, Hq, 1, D), 1, torch.bfloat16, CUDA)
+    kc, vc = (randn((B * mb, Hkv, 16, D), i, torch.bfloat16, CUDA) for i in (2, 3))
+    means = kc.float().mean(2).to(torch.bfloat16)
+    bt = torch.arange(B * mb, device=CUDA, dtype=torch.int32).view(B, mb)
+    cl = torch.tensor([4000, 900], device=CUDA, dtype=torch.int32)
+
+    def f(q):
+        return (sa.sp2norm_paged_attention(q * 1, kc, vc, bt, cl) + 1,
+                sa.sp2norm_sparse_paged_attention(q * 1, kc, vc, means, bt, cl, 8) + 1)
+
+    g = torch.compile(f, mode="reduce-overhead", fullgraph=True)
+    for step in range(5):
+        x = randn(q.shape, 10 + step, torch.bfloat16, CUDA)
+        torch.compiler.cudagraph_mark_step_begin()
+        got = [t.clone() for t in g(x)]
+        assert all(torch.equal(a, b) for a, b in zip(got, f(x)))
